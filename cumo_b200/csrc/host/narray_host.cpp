@@ -1033,6 +1033,119 @@ cb200_na_t* cb200_na_cum(const char* op_c, cb200_na_t* a, int axis, int nan) {
     return out;
 }
 
+// ---- gated running sums ---------------------------------------------------------------------
+// Steps of `x` against a loop of `nd` dimensions (aligned at the last, repeated where its extent is 1 or missing; a single
+// element repeats everywhere), or an error.
+static bool repeated_steps(const cb200_na* x, int nd, const int64_t* shape, const char* what, int64_t* step) {
+    if (size_of(x) == 1) { for (int d = 0; d < nd; ++d) step[d] = 0; return true; }
+    bool fits = x->ndim <= nd;
+    for (int d = 0; d < nd; ++d) {
+        const int od = d - (nd - x->ndim);
+        step[d] = od >= 0 && x->shape[od] != 1 ? x->step[od] : 0;
+        if (fits && od >= 0 && x->shape[od] != 1 && x->shape[od] != shape[d]) fits = false;
+    }
+    if (!fits) fail("ShapeError", "%s does not fit the shape of the running sums", what);
+    return fits;
+}
+
+// `full` (of the loop's shape) summed over what `like` was repeated over, in `like`'s shape.  Takes `full` over.
+static cb200_na* sum_to_shape_of(cb200_na* full, const cb200_na* like) {
+    uint32_t mask = 0;
+    for (int d = 0; d < full->ndim; ++d) {
+        const int od = d - (full->ndim - like->ndim);
+        if ((size_of(like) == 1 || od < 0 || like->shape[od] == 1) && full->shape[d] != 1) mask |= 1u << d;
+    }
+    cb200_na* r = full;
+    if (mask) {
+        r = size_of(full) ? (cb200_na*)cb200_na_reduce("sum", full, mask, 1, 0) : nullptr;
+        if (!size_of(full)) r = make(like->dtype, like->ndim, like->shape, true);
+        cb200_na_release(full);
+        if (!r) return nullptr;
+    }
+    r->ndim = like->ndim;                                   // a fresh contiguous array: only extents of 1 come or go
+    for (int d = 0; d < like->ndim; ++d) r->shape[d] = like->shape[d];
+    contiguous_steps(r->dtype, r->ndim, r->shape, r->step);
+    return r;
+}
+
+// The axis and type checks both directions share; the state's shape (the axis left out) into `state`.
+static bool gated_args(const char* what, const cb200_na* x, const cb200_na* gate, const cb200_na* initial, int axis, int64_t* gstep, int64_t* state, int64_t* istep) {
+    if (!is_float_type(x->dtype) || gate->dtype != x->dtype || (initial && initial->dtype != x->dtype)) {
+        fail("TypeError", "%s needs operands that are all SFloat or all DFloat", what);
+        return false;
+    }
+    if (axis < 0 || axis >= x->ndim) { fail("ArgumentError", "axis %d out of range for %d dimensions", axis, x->ndim); return false; }
+    if (!repeated_steps(gate, x->ndim, x->shape, "gate", gstep)) return false;
+    int k = 0;
+    for (int d = 0; d < x->ndim; ++d) if (d != axis) state[k++] = x->shape[d];
+    return !initial || repeated_steps(initial, x->ndim - 1, state, "initial", istep);
+}
+
+cb200_na_t* cb200_na_gated_cumsum(cb200_na_t* x, cb200_na_t* gate, cb200_na_t* initial, int axis) {
+    int64_t gstep[kMaxD], state[kMaxD], istep[kMaxD];
+    if (!gated_args("gated_cumsum", x, gate, initial, axis, gstep, state, istep)) return nullptr;
+    cb200_na* out = make(x->dtype, x->ndim, x->shape, false);
+    if (!out || size_of(x) == 0) return out;
+    size_t oshape[kMaxD];
+    ssize_t ox[kMaxD], og[kMaxD], oi[kMaxD], oh[kMaxD];
+    int k = 0;
+    for (int d = 0; d < x->ndim; ++d) {
+        if (d == axis) continue;
+        oshape[k] = (size_t)x->shape[d]; ox[k] = (ssize_t)x->step[d]; og[k] = (ssize_t)gstep[d]; oh[k] = (ssize_t)out->step[d];
+        oi[k] = initial ? (ssize_t)istep[k] : 0;
+        ++k;
+    }
+    auto f = x->dtype == CB200_SFLOAT ? cb200_sfloat_gated_cumsum_runs_kernel_launch : cb200_dfloat_gated_cumsum_runs_kernel_launch;
+    const int status = f(data_ptr(x), data_ptr(gate), initial ? data_ptr(initial) : nullptr, data_ptr(out), (ssize_t)x->step[axis], (ssize_t)gstep[axis],
+                         (ssize_t)out->step[axis], (uint64_t)x->shape[axis], k, oshape, ox, og, oi, oh);
+    if (status) { fail("CudaError", "gated_cumsum: %s", cudaGetErrorString((cudaError_t)status)); cb200_na_release(out); return nullptr; }
+    if (!launch_ok()) { cb200_na_release(out); return nullptr; }
+    return out;
+}
+
+int cb200_na_gated_cumsum_grad(cb200_na_t* grad, cb200_na_t* gate, cb200_na_t* h, cb200_na_t* initial, int axis, cb200_na_t** dx_out,
+                               cb200_na_t** dgate_out, cb200_na_t** dinitial_out) {
+    *dx_out = *dgate_out = *dinitial_out = nullptr;
+    int64_t gstep[kMaxD], state[kMaxD], istep[kMaxD], hstep[kMaxD];
+    if (!gated_args("gated_cumsum_grad", grad, gate, initial, axis, gstep, state, istep)) return 1;
+    bool same = h->dtype == grad->dtype && h->ndim == grad->ndim;
+    for (int d = 0; same && d < h->ndim; ++d) same = h->shape[d] == grad->shape[d];
+    if (!same) { fail(h->dtype == grad->dtype ? "ShapeError" : "TypeError", "h must have the type and shape of grad"); return 1; }
+    repeated_steps(h, grad->ndim, grad->shape, "h", hstep);
+    cb200_na* dx = make(grad->dtype, grad->ndim, grad->shape, false);
+    cb200_na* dgate = dx ? make(grad->dtype, grad->ndim, grad->shape, false) : nullptr;
+    cb200_na* dinit = dgate && initial ? make(grad->dtype, grad->ndim - 1, state, size_of(grad) == 0) : nullptr;
+    auto give_up = [&]() { cb200_na_release(dx); cb200_na_release(dgate); cb200_na_release(dinit); return 1; };
+    if (!dx || !dgate || (initial && !dinit)) return give_up();
+    if (size_of(grad) != 0) {
+        size_t oshape[kMaxD];
+        ssize_t o1[kMaxD], o2[kMaxD], o3[kMaxD], o4[kMaxD], o5[kMaxD], o6[kMaxD], o7[kMaxD];
+        int k = 0;
+        for (int d = 0; d < grad->ndim; ++d) {
+            if (d == axis) continue;
+            oshape[k] = (size_t)grad->shape[d];
+            o1[k] = (ssize_t)grad->step[d]; o2[k] = (ssize_t)gstep[d]; o3[k] = (ssize_t)h->step[d]; o5[k] = (ssize_t)dx->step[d]; o6[k] = (ssize_t)dgate->step[d];
+            o4[k] = initial ? (ssize_t)istep[k] : 0;
+            o7[k] = dinit ? (ssize_t)dinit->step[k] : 0;
+            ++k;
+        }
+        auto f = grad->dtype == CB200_SFLOAT ? cb200_sfloat_gated_cumsum_grad_runs_kernel_launch : cb200_dfloat_gated_cumsum_grad_runs_kernel_launch;
+        const int status = f(data_ptr(grad), data_ptr(gate), data_ptr(h), initial ? data_ptr(initial) : nullptr, data_ptr(dx), data_ptr(dgate),
+                             dinit ? data_ptr(dinit) : nullptr, (ssize_t)grad->step[axis], (ssize_t)gstep[axis], (ssize_t)h->step[axis], (ssize_t)dx->step[axis],
+                             (ssize_t)dgate->step[axis], (uint64_t)grad->shape[axis], k, oshape, o1, o2, o3, o4, o5, o6, o7);
+        if (status) { fail("CudaError", "gated_cumsum_grad: %s", cudaGetErrorString((cudaError_t)status)); return give_up(); }
+        if (!launch_ok()) return give_up();
+    }
+    dgate = sum_to_shape_of(dgate, gate);
+    if (!dgate) return give_up();
+    if (dinit) {
+        dinit = sum_to_shape_of(dinit, initial);
+        if (!dinit) return give_up();
+    }
+    *dx_out = dx; *dgate_out = dgate; *dinitial_out = dinit;
+    return 0;
+}
+
 // ---- bincount ------------------------------------------------------------------------------
 cb200_na_t* cb200_na_bincount(cb200_na_t* a, cb200_na_t* weight, int64_t minlength) {
     if (a->dtype != CB200_INT32 && a->dtype != CB200_INT64) return (cb200_na*)fail("NoMethodError", "undefined method bincount for %s", kTypeName[a->dtype]);

@@ -721,6 +721,47 @@ class NArray:
     def cumsum(self, axis=None, nan=False): return self._cum("cumsum", axis, nan)
     def cumprod(self, axis=None, nan=False): return self._cum("cumprod", axis, nan)
 
+    def _scan_axis(self, axis):
+        if axis is None and self.ndim == 1:
+            return 0
+        if not isinstance(axis, int) or isinstance(axis, bool):
+            raise TypeError("gated_cumsum takes one axis (it may be left out for a vector)")
+        ax = axis + self.ndim if axis < 0 else axis
+        if not 0 <= ax < self.ndim:
+            raise ValueError(f"axis {axis} out of range for ndim {self.ndim}")
+        return ax
+
+    def _scan_operand(self, value, what):
+        if value is None or isinstance(value, NArray):
+            return value
+        if isinstance(value, (list, tuple, np.ndarray, int, float)):
+            return type(self).cast(value if not isinstance(value, (int, float)) else [value])
+        raise TypeError(f"{what} must be an array or a number")
+
+    def gated_cumsum(self, gate, axis=None, initial=None):
+        """`cumsum` with a coefficient per step: h[t] = gate[t] * h[t-1] + self[t] along `axis` (SFloat / DFloat).  `gate`
+        is repeated to this array's shape like any operand, `initial` (the state before the first step) to the shape without
+        the axis; without it h[0] = self[0] and gate[0] is not used.  Returns h; its last entry along the axis is the state
+        to carry on with."""
+        gate, initial = self._scan_operand(gate, "gate"), self._scan_operand(initial, "initial")
+        if gate is None:
+            raise TypeError("gate must be an array or a number")
+        return NArray._from_handle(_lib.load().cb200_na_gated_cumsum(self._h, gate._h, initial._h if initial is not None else None, self._scan_axis(axis)))
+
+    def gated_cumsum_grad(self, gate, h, axis=None, initial=None):
+        """The gradients of `h = x.gated_cumsum(gate, axis, initial)` for this array dL/dh: (dx, dgate), and dinitial where
+        an initial state was given.  dx[t] = self[t] + gate[t+1] * dx[t+1], dgate[t] = dx[t] * h[t-1], dinitial = gate[0] *
+        dx[0]; dgate and dinitial are summed over whatever gate and initial were repeated over."""
+        gate, initial = self._scan_operand(gate, "gate"), self._scan_operand(initial, "initial")
+        if gate is None or not isinstance(h, NArray):
+            raise TypeError("gated_cumsum_grad needs the gate and the h that gated_cumsum returned")
+        dx, dgate, dinitial = c_void_p(), c_void_p(), c_void_p()
+        if _lib.load().cb200_na_gated_cumsum_grad(self._h, gate._h, h._h, initial._h if initial is not None else None, self._scan_axis(axis),
+                                                  byref(dx), byref(dgate), byref(dinitial)):
+            _raise_last()
+        out = (NArray._from_handle(dx.value), NArray._from_handle(dgate.value))
+        return out if initial is None else out + (NArray._from_handle(dinitial.value),)
+
     def bincount(self, weight=None, minlength=0):
         """Occurrences (or summed weights) of each value along the last axis (Int32 / Int64 only)."""
         if weight is not None and not isinstance(weight, NArray):

@@ -598,6 +598,39 @@ unsigned long long cb200_tile_pipeline_launches(void);
  *     capture begins. */
 int cb200_sfloat_sum_noalloc_kernel_launch(cumo_na_reduction_arg_t* arg, char* errbuf, size_t errlen);
 
+/* Gated running sums of every run of a loop in one launch (no counterpart in the reference, whose scans are cumsum and
+ * cumprod): h[t] = gate[t] * h[t-1] + x[t], t = 0 .. n-1, s_* the byte steps along t, the *_step arrays those of the n_outer
+ * other dimensions (host arrays; a step of 0 repeats).  `initial` (may be NULL) is h[-1] per run; without it h[0] = x[0] and
+ * gate[0] is not read.  The second function writes the gradients for grad = dL/dh, given the h of the first:
+ * dx[t] = grad[t] + gate[t+1] * dx[t+1], dgate[t] = dx[t] * h[t-1] (0 at t = 0 without an initial state) and, where
+ * dinitial is not NULL, gate[0] * dx[0].  Outputs may not overlap inputs and their steps may not be 0.  Both return a cudaError_t. */
+#define CB200_DECL_GATED(T) \
+    int cb200_##T##_gated_cumsum_runs_kernel_launch(char* x, char* gate, char* initial, char* h, ssize_t s_x, ssize_t s_gate, ssize_t s_h, uint64_t n, int n_outer, \
+        const size_t* shape, const ssize_t* x_step, const ssize_t* gate_step, const ssize_t* initial_step, const ssize_t* h_step); \
+    int cb200_##T##_gated_cumsum_grad_runs_kernel_launch(char* grad, char* gate, char* h, char* initial, char* dx, char* dgate, char* dinitial, \
+        ssize_t s_grad, ssize_t s_gate, ssize_t s_h, ssize_t s_dx, ssize_t s_dgate, uint64_t n, int n_outer, const size_t* shape, \
+        const ssize_t* grad_step, const ssize_t* gate_step, const ssize_t* h_step, const ssize_t* initial_step, const ssize_t* dx_step, \
+        const ssize_t* dgate_step, const ssize_t* dinitial_step);
+CB200_DECL_GATED(sfloat) CB200_DECL_GATED(dfloat)
+
+/* The linear layer (the reference stops at gemm: gen/tmpl/gemm.c): z = x . w + bias, y = act(z) + residual, for x (m, k),
+ * w (k, n), bias (n) and residual (m, n) with any byte steps (multiples of the element size; 0 repeats); bias, residual and
+ * pre may be NULL.  y and, where given, pre (which receives z) are contiguous (m, n).  activation: 0 none, 1 relu, 2 silu,
+ * 3 gelu (with the normal distribution function), 4 gelu in its tanh form, 5 sigmoid, 6 tanh.
+ * The second function: with dz = grad * act'(pre) (pre may be NULL for activation 0), dx (m, k) = dz . w^T,
+ * dw (k, n) = x^T . dz and dbias (n) = the column sums of dz; outputs are contiguous and each may be NULL.  Scratch comes from
+ * the pool callback or, while the stream is captured, is part of the graph.  Both return a cudaError_t and do not synchronise.
+ * The third: `batch` matrices (rows, columns) with any byte steps; X = g / (|g|_F + eps), then for each of `steps`
+ * triples (a, b, c) of coefs (host): X <- a X + (b P + c P P) X with P = X X^T; out is contiguous. */
+#define CB200_DECL_LINEAR(T, C) \
+    int cb200_##T##_linear_kernel_launch(int64_t m, int64_t n, int64_t k, const C* x, ssize_t x_row, ssize_t x_col, const C* w, ssize_t w_row, ssize_t w_col, \
+        const C* bias, ssize_t bias_step, const C* residual, ssize_t r_row, ssize_t r_col, int activation, C* y, C* pre); \
+    int cb200_##T##_linear_grad_kernel_launch(int64_t m, int64_t n, int64_t k, const C* grad, ssize_t g_row, ssize_t g_col, const C* x, ssize_t x_row, ssize_t x_col, \
+        const C* w, ssize_t w_row, ssize_t w_col, const C* pre, ssize_t p_row, ssize_t p_col, int activation, C* dx, C* dw, C* dbias); \
+    int cb200_##T##_orthogonalize_kernel_launch(int64_t batch, int64_t rows, int64_t columns, const C* g, ssize_t g_batch, ssize_t g_row, ssize_t g_col, \
+        int steps, const double* coefs, double eps, C* out);
+CB200_DECL_LINEAR(sfloat, float) CB200_DECL_LINEAR(dfloat, double)
+
 #ifdef __cplusplus
 }
 #endif

@@ -100,6 +100,13 @@ cb200_na_t* cb200_na_where(cb200_na_t* bits, int want_zeros);
 /* cumsum / cumprod (narray/gen/tmpl/cum.c:41-70): axis < 0 runs over all elements in row-major order, else along
  * that axis; the result has the operand's shape and type.  nan: the NaN-skipping operator (float types). */
 cb200_na_t* cb200_na_cum(const char* op, cb200_na_t* a, int axis, int nan);
+/* h[t] = gate[t] * h[t-1] + x[t] along `axis`, in x's shape; gate is repeated to x's shape, initial (may be NULL: h[0] = x[0])
+ * to the shape without the axis.  All SFloat or all DFloat. */
+cb200_na_t* cb200_na_gated_cumsum(cb200_na_t* x, cb200_na_t* gate, cb200_na_t* initial, int axis);
+/* Its gradients from grad = dL/dh and the h it returned: dx in grad's shape, dgate in gate's, dinitial in initial's (NULL
+ * without one).  Returns 0, or 1 with cb200_host_error() set. */
+int cb200_na_gated_cumsum_grad(cb200_na_t* grad, cb200_na_t* gate, cb200_na_t* h, cb200_na_t* initial, int axis,
+                               cb200_na_t** dx, cb200_na_t** dgate, cb200_na_t** dinitial);
 /* bincount along the last axis (narray/gen/tmpl/bincount.c:176-240): counts as UInt32 (UInt64 when the length
  * exceeds 2^32-1), or sums of `weight` (SFloat stays SFloat, anything else is summed as DFloat); the length is
  * max+1 or `minlength` if larger; a negative element raises ArgumentError.  Reads the extremes back: synchronises. */
