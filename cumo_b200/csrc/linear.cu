@@ -4,7 +4,7 @@
 // dr = g itself).  All three products are contractions of two operands with arbitrary steps, so one product kernel serves
 // them, and its epilogue adds the bias, keeps z where the caller wants it for the gradients, and applies the rest before the
 // element leaves the registers: y is written once and z is never read back.
-#include "linear.cuh"
+#include "split_product.cuh"
 
 namespace cb200 {
 
@@ -149,6 +149,72 @@ static int launch_dz(int64_t m, int64_t n, const Steps2<T>& grad, const Steps2<T
     return (int)cudaGetLastError();
 }
 
+// ---- single precision on the tensor cores -----------------------------------------------------------------------------
+// An operand of the layer split once, whichever of its axes the products contract over.
+struct SplitMatrix {
+    SplitSource src;
+    int64_t R, C;                     // planes are [R][ld >= C]: the axis the source has contiguous runs along is the inner one
+    bool swapped;                     // R, C are the matrix's columns and rows
+    uint16_t* planes;
+    int64_t ld;
+    Marks marks;
+    // as operand of a contraction over the matrix's columns (over_columns) or rows
+    Planes operand(bool over_columns) const {
+        Planes p;
+        p.p = planes; p.batch = 1; p.ld = ld;
+        p.k_major = over_columns != swapped;
+        p.rows = over_columns != swapped ? R : C;
+        p.k = over_columns != swapped ? C : R;
+        return p;
+    }
+    const uint8_t* marks_of(bool over_columns) const { return over_columns != swapped ? marks.row : marks.col; }
+    bool turned(bool over_columns) const { return over_columns == swapped; }
+};
+
+struct SplitSet {
+    SplitMatrix x[3];
+    int count = 0;
+    int add(const SplitSource& s, int64_t rows, int64_t cols) {
+        SplitMatrix& a = x[count];
+        a.src = s; a.R = rows; a.C = cols; a.swapped = false;
+        if (s.col != 1 && s.row == 1) {
+            a.swapped = true;
+            a.R = cols; a.C = rows;
+            a.src.row = s.col; a.src.col = s.row; a.src.pre_row = s.pre_col; a.src.pre_col = s.pre_row;
+        }
+        a.ld = planes_ld(a.C);
+        return count++;
+    }
+    // scratch for all of them, marks cleared by one memset, then the splits
+    int split(Scratch& scratch, cudaStream_t st) {
+        size_t marks = 16;
+        for (int i = 0; i < count; ++i) marks += (size_t)(x[i].R + x[i].C);
+        char* mk = scratch.take(marks);
+        if (!mk) return (int)cudaErrorMemoryAllocation;
+        int rc = (int)cudaMemsetAsync(mk, 0, marks, st);
+        int* any = reinterpret_cast<int*>(mk);
+        mk += 16;
+        for (int i = 0; i < count && rc == 0; ++i) {
+            SplitMatrix& a = x[i];
+            a.planes = reinterpret_cast<uint16_t*>(scratch.take((size_t)3 * a.R * a.ld * 2));
+            if (!a.planes) return (int)cudaErrorMemoryAllocation;
+            a.marks = {reinterpret_cast<uint8_t*>(mk), reinterpret_cast<uint8_t*>(mk) + a.R, any};
+            mk += a.R + a.C;
+            rc = launch_split(a.src, a.R, a.C, a.planes, a.ld, a.marks, st);
+        }
+        return rc;
+    }
+    int product(int a, bool a_over_columns, int b, bool b_over_columns, const Epilogue<float>& e, cudaStream_t st) const {
+        const Planes pa = x[a].operand(a_over_columns), pb = x[b].operand(b_over_columns);
+        int rc = launch_split_product(kSplitBf16x3, pa, pb, e, st);
+        if (rc) return rc;
+        return launch_fix_marked(pa.rows, pb.rows, pa.k, x[a].src, x[a].turned(a_over_columns), x[a].marks_of(a_over_columns), x[b].src,
+                                 x[b].turned(b_over_columns), x[b].marks_of(b_over_columns), x[a].marks.any, e, st);
+    }
+};
+
+static bool worth_splitting(int64_t m, int64_t n, int64_t k) { return m >= 32 && n >= 32 && k >= 32 && m * n * k >= (1LL << 22); }
+
 // ---- entry points ------------------------------------------------------------------------------------------------------
 template <typename T>
 static int linear(int64_t m, int64_t n, int64_t k, const T* x, ssize_t x_row, ssize_t x_col, const T* w, ssize_t w_row, ssize_t w_col,
@@ -164,6 +230,18 @@ static int linear(int64_t m, int64_t n, int64_t k, const T* x, ssize_t x_row, ss
     e.act = activation;
     e.res = residual; e.res_row = r_row / es; e.res_col = r_col / es;
     e.y = y; e.ld = n; e.pre = pre;
+    if constexpr (sizeof(T) == 4) {
+        if (worth_splitting(m, n, k)) {
+            const int late = product_gave_up();
+            if (late) return late;
+            Scratch scratch(current_stream());
+            SplitSet set;
+            const int ix = set.add(SplitSource{x, x_row / es, x_col / es, nullptr, 0, 0, kActNone}, m, k);
+            const int iw = set.add(SplitSource{w, w_row / es, w_col / es, nullptr, 0, 0, kActNone}, k, n);
+            int rc = set.split(scratch, current_stream());
+            return rc ? rc : set.product(ix, true, iw, false, e, current_stream());
+        }
+    }
     const Operand<T> a = {x, x_row / es, x_col / es, 0}, b = {w, w_col / es, w_row / es, 0};
     return launch_product_cc<T>(m, n, k, 1, a, b, e, current_stream());
 }
@@ -186,6 +264,26 @@ static int linear_grad(int64_t m, int64_t n, int64_t k, const T* grad, ssize_t g
     Scratch scratch(st);
     Steps2<T> g = {grad, g_row / es, g_col / es}, p = {pre, p_row / es, p_col / es};
     Operand<T> dz = {grad, g.row, g.col, 0};
+    if constexpr (sizeof(T) == 4) {
+        if ((dx || dw) && worth_splitting(m, n, k)) {
+            int rc = product_gave_up();
+            if (rc) return rc;
+            if (dbias) rc = launch_dz<T>(m, n, g, p, activation, nullptr, dbias, scratch, st);
+            if (rc) return rc;
+            SplitSet set;
+            const int iz = set.add(SplitSource{grad, g.row, g.col, pre, p.row, p.col, activation}, m, n);
+            const int iw = dx ? set.add(SplitSource{w, w_row / es, w_col / es, nullptr, 0, 0, kActNone}, k, n) : 0;
+            const int ix = dw ? set.add(SplitSource{x, x_row / es, x_col / es, nullptr, 0, 0, kActNone}, m, k) : 0;
+            rc = set.split(scratch, st);
+            Epilogue<float> e = {};
+            e.alpha = 1.f;
+            e.y = dx; e.ld = k;
+            if (rc == 0 && dx) rc = set.product(iz, true, iw, true, e, st);
+            e.y = dw; e.ld = n;
+            if (rc == 0 && dw) rc = set.product(ix, false, iz, false, e, st);
+            return rc;
+        }
+    }
     if (activation != kActNone || dbias) {
         T* z = nullptr;
         if (activation != kActNone && (dx || dw)) {

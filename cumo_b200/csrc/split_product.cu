@@ -1,0 +1,482 @@
+// The tensor-core product of split operands (split_product.cuh says what the parts are): tcgen05 with tensor-memory
+// accumulators, operands brought by the tensor memory accelerator.
+//
+// Roles of the 10 warps of a CTA:
+//   warp 0      one thread issues the TMA loads of a K-block (64 elements of K, all planes of both operands) into a ring of
+//               128-byte-swizzled stages
+//   warp 1      allocates tensor memory; one thread issues the tcgen05.mma's: smallest products first
+//   warps 2..9  epilogue: every 24 instructions' worth of products (a chunk) they add the accumulator from tensor memory
+//               to registers, two accumulators taking turns so that the MMAs never wait; at the end of a tile the sums pass
+//               through a small shared-memory tile per warp, so that global memory is read and written along rows
+// With CG = 2 two CTAs of a cluster share a 256 x 256 tile: each loads its 128 rows of A and its half of B, the first CTA
+// issues the instructions for both.  Shared memory feeds 64 bytes per cycle to the tensor cores then, instead of the 128 of
+// a 128 x 128 tile (its limit), and each operand byte loaded is used twice as often.  Small problems take 128-row tiles of one
+// CTA, 128 or 64 columns wide.  Every wait is bounded; when one runs out the kernel raises a word in host memory that the next
+// call finds.
+#include "split_product.cuh"
+#include "tc_common.cuh"
+#include "tile_tma.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <mutex>
+
+namespace cb200 {
+
+constexpr int kSpThreads = 320;
+constexpr int kSpKB = 64;                       // K per stage: one 128-byte swizzle row of 16-bit elements
+constexpr int kSpStageCols = 33;                // epilogue tile: 32 x 32 floats, rows padded by one
+
+template <int P, int CG, int BN>
+struct SplitShape {
+    static constexpr int kBRows = BN / CG;                               // rows of B a CTA loads
+    static constexpr int kABytes = 128 * 128, kBBytes = kBRows * 128;    // per plane
+    static constexpr int kStageBytes = P * (kABytes + kBBytes);
+    static constexpr int kEpilogueBytes = 8 * 32 * kSpStageCols * 4;
+    static constexpr int kStages = (232448 - 1024 - kEpilogueBytes) / kStageBytes < 4 ? (232448 - 1024 - kEpilogueBytes) / kStageBytes : 4;
+    static constexpr int kChunkBlocks = P == 3 ? 1 : 2;                  // K-blocks per accumulator: 24 instructions
+    static constexpr size_t kSmem = (size_t)kStages * kStageBytes + kEpilogueBytes + 256;
+    static_assert(kStages >= 2, "two stages at least");
+};
+
+struct SplitArgs {
+    int64_t m, n;
+    int kblocks;
+    int64_t tiles_m, tiles_n, n_tiles;          // n_tiles counts all batch entries
+    int64_t batch;
+    int a_k_major, b_k_major;
+    uint32_t idesc;
+    int* gave_up;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_cta(uint32_t saddr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+    return r;
+}
+
+template <int CG>
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x0, int x1, int x2) {
+    if constexpr (CG == 1)
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                     ::"r"(dst), "l"(map), "r"(bar), "r"(x0), "r"(x1), "r"(x2) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                     ::"r"(dst), "l"(map), "r"(bar), "r"(x0), "r"(x1), "r"(x2) : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void split_commit(uint64_t* bar) {
+    if constexpr (CG == 1)
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                     ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+}
+
+// mbar_wait for barriers that the other CTA of the pair arrives at
+__device__ __forceinline__ bool mbar_wait_pair(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    const uint32_t addr = smem_u32(bar);
+    for (uint32_t spin = 0; spin < kSpinLimit; ++spin) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(done) : "r"(addr), "r"(parity) : "memory");
+        if (done) return true;
+        if (spin > 16) __nanosleep(32);
+        if ((spin & 255u) == 255u && *abort_flag) return false;
+    }
+    *abort_flag = 1;
+    return false;
+}
+
+// MN-major, 128-byte swizzle: 8 rows of k (1024 bytes) per group, next 64 elements of the row axis 8192 bytes on
+__device__ __forceinline__ uint64_t umma_desc_mn(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr & 0x3ffffu) >> 4);
+    d |= (uint64_t)(8192u >> 4) << 16;
+    d |= (uint64_t)(1024u >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
+// Out: how a finished 32-row x 32-column piece leaves.  The float form.
+struct FloatOut {
+    Epilogue<float> e;
+    static constexpr int kind = 0;
+    __device__ __forceinline__ void piece(const float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n) const {
+        const int64_t j = j0 + lane;
+        if (j >= n) return;
+        const int rows = m - i0 < 32 ? (int)(m - i0) : 32;
+        const float bias = e.bias ? e.bias[j * e.bias_step] : 0.f;
+        const float* res = e.res ? e.res + j * e.res_col : nullptr;
+        int64_t at = batch * e.y_batch + i0 * e.ld + j;
+#pragma unroll 4
+        for (int r = 0; r < rows; ++r, at += e.ld) {
+            float z = tile[r * kSpStageCols + lane];
+            if (e.bias) z += bias;
+            if (e.pre) e.pre[at] = z;
+            float y = e.act == kActNone ? z : activate(z, e.act);
+            if (res) y += res[(i0 + r) * e.res_row];
+            e.y[at] = y;
+        }
+    }
+};
+
+// ... and the form that leaves as two half-precision planes.
+struct PlaneOut {
+    PlaneEpilogue e;
+    static constexpr int kind = 1;
+    __device__ __forceinline__ void piece(const float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n) const {
+        const int64_t j = j0 + lane;
+        if (j >= n) return;
+        const int rows = m - i0 < 32 ? (int)(m - i0) : 32;
+        int64_t at = batch * e.batch_step + i0 * e.ld + j;
+        const __half* d = reinterpret_cast<const __half*>(e.d);
+        __half* out = reinterpret_cast<__half*>(e.out);
+#pragma unroll 4
+        for (int r = 0; r < rows; ++r, at += e.ld) {
+            float v = tile[r * kSpStageCols + lane] * e.acc_scale;
+            if (d) v += e.beta * ((__half2float(d[at]) + __half2float(d[at + e.plane])) * e.d_scale);
+            v *= e.out_scale;
+            const __half hi = __float2half_rn(v);
+            out[at] = hi;
+            out[at + e.plane] = __float2half_rn(v - __half2float(hi));
+        }
+    }
+};
+
+template <int P, int CG, int BN, typename Out>
+__global__ void __launch_bounds__(kSpThreads, 1)
+split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Out out) {
+    using S = SplitShape<P, CG, BN>;
+    extern __shared__ __align__(1024) char smem_raw[];
+    char* base = smem_raw;
+    float* pieces = reinterpret_cast<float*>(base + S::kStages * S::kStageBytes);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(base + S::kStages * S::kStageBytes + S::kEpilogueBytes);
+    uint64_t* full = bars;                          // [4] TMA -> MMA
+    uint64_t* empty = bars + 4;                     // [4] MMA -> TMA
+    uint64_t* acc_full = bars + 8;                  // [2] MMA -> epilogue
+    uint64_t* acc_empty = bars + 10;                // [2] epilogue -> MMA, 8 warps of each CTA
+    uint64_t* drain = bars + 12;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = CG == 2 ? cluster_rank() : 0;
+    const bool misplaced = (smem_u32(base) & 1023u) != 0;       // the same in every CTA; nothing is launched into it then
+    if (tid == 0) {
+        for (int i = 0; i < 4; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(acc_full + i, 1); mbar_init(acc_empty + i, 8 * CG); }
+        mbar_init(drain, 1);
+        abort_flag[0] = misplaced ? 1 : 0;
+        abort_flag[1] = 0;                                       // never set: what the last waits poll
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    if (warp == 1) {
+        if constexpr (CG == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)(2 * BN)) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)(2 * BN)) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync_all();                   // the peer's barriers exist before anything arrives at them
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = *tmem_slot;
+
+    const int64_t cluster = blockIdx.x / CG, clusters = gridDim.x / CG;
+    const int64_t my_tiles = misplaced || cluster >= g.n_tiles ? 0 : (g.n_tiles - cluster + clusters - 1) / clusters;
+    const uint32_t chunks = (uint32_t)((g.kblocks + S::kChunkBlocks - 1) / S::kChunkBlocks);
+    // bands of eight tile rows, walked column by column: the tiles in flight share rows of A and columns of B in L2
+    auto tile_of = [&](int64_t t, int64_t* batch, int64_t* i0, int64_t* j0) {
+        int64_t f = cluster + t * clusters;
+        const int64_t per = g.tiles_m * g.tiles_n;
+        *batch = f / per;
+        f -= *batch * per;
+        const int64_t band = f / (8 * g.tiles_n);
+        const int64_t height = g.tiles_m - band * 8 < 8 ? g.tiles_m - band * 8 : 8;
+        f -= band * 8 * g.tiles_n;
+        *j0 = (f / height) * BN;
+        *i0 = (band * 8 + f % height) * (128 * CG) + rank * 128;
+    };
+
+    if (warp == 0) {
+        // ---- loads ------------------------------------------------------------------------------
+        if (lane == 0) {
+            uint32_t it = 0;
+            bool ok = true;
+            for (int64_t t = 0; t < my_tiles && ok; ++t) {
+                int64_t batch, i0, j0;
+                tile_of(t, &batch, &i0, &j0);
+                j0 += rank * S::kBRows;
+                for (int kb = 0; kb < g.kblocks; ++kb, ++it) {
+                    const uint32_t slot = it % S::kStages;
+                    if (!mbar_wait(empty + slot, ((it / S::kStages) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                    if (rank == 0) mbar_expect_tx(full + slot, (uint32_t)(S::kStageBytes * CG));
+                    const uint32_t bar = CG == 2 ? in_cta(smem_u32(full + slot), 0) : smem_u32(full + slot);
+                    uint32_t dst = smem_u32(base + slot * S::kStageBytes);
+                    const int k0 = kb * kSpKB;
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        const int z = (int)(p * g.batch + batch);
+                        if (g.a_k_major) tma_load_3d<CG>(dst, &map_a, bar, k0, (int)i0, z);
+                        else { tma_load_3d<CG>(dst, &map_a, bar, (int)i0, k0, z); tma_load_3d<CG>(dst + 8192, &map_a, bar, (int)i0 + 64, k0, z); }
+                        dst += S::kABytes;
+                    }
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        const int z = (int)(p * g.batch + batch);
+                        if (g.b_k_major) tma_load_3d<CG>(dst, &map_b, bar, k0, (int)j0, z);
+                        else {
+#pragma unroll
+                            for (int h = 0; h < S::kBRows / 64; ++h) tma_load_3d<CG>(dst + h * 8192, &map_b, bar, (int)j0 + h * 64, k0, z);
+                        }
+                        dst += S::kBBytes;
+                    }
+                }
+            }
+            if (!ok) for (int i = 0; i < 1000; ++i) __nanosleep(1000);      // gave up: copies still in flight land before the CTA leaves
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ---- products ---------------------------------------------------------------------------
+        if (lane == 0 && rank == 0) {
+            uint32_t it = 0, item = 0;
+            bool ok = true;
+            const uint32_t a_step = g.a_k_major ? 32u : 2048u, b_step = g.b_k_major ? 32u : 2048u;     // bytes per 16 of K
+            for (int64_t t = 0; t < my_tiles && ok; ++t) {
+                for (int kb0 = 0; kb0 < g.kblocks && ok; kb0 += S::kChunkBlocks, ++item) {
+                    const uint32_t acc = item & 1u;
+                    if (!mbar_wait_pair(acc_empty + acc, ((item >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t d_tmem = tmem_base + acc * (uint32_t)BN;
+                    const int kb1 = kb0 + S::kChunkBlocks < g.kblocks ? kb0 + S::kChunkBlocks : g.kblocks;
+                    for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                        const uint32_t slot = it % S::kStages;
+                        if (!mbar_wait(full + slot, (it / S::kStages) & 1u, abort_flag)) { ok = false; break; }
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint32_t sa = smem_u32(base + slot * S::kStageBytes), sb = sa + P * S::kABytes;
+                        constexpr int kTerms = P == 3 ? 6 : 3;
+                        constexpr int ta[6] = {P == 3 ? 2 : 1, 0, P == 3 ? 1 : 0, 1, 0, 0};
+                        constexpr int tb[6] = {0, P == 3 ? 2 : 1, P == 3 ? 1 : 0, 0, 1, 0};
+#pragma unroll
+                        for (int term = 0; term < kTerms; ++term) {
+#pragma unroll
+                            for (int ks = 0; ks < 4; ++ks) {
+                                const uint32_t aa = sa + ta[term] * S::kABytes + ks * a_step, bb = sb + tb[term] * S::kBBytes + ks * b_step;
+                                const uint64_t da = g.a_k_major ? umma_desc(aa) : umma_desc_mn(aa);
+                                const uint64_t db = g.b_k_major ? umma_desc(bb) : umma_desc_mn(bb);
+                                const uint32_t accumulate = (uint32_t)((kb - kb0) | term | ks) != 0;
+                                if constexpr (CG == 1)
+                                    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                                                 ::"r"(d_tmem), "l"(da), "l"(db), "r"(g.idesc), "r"(accumulate) : "memory");
+                                else
+                                    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                                                 ::"r"(d_tmem), "l"(da), "l"(db), "r"(g.idesc), "r"(accumulate) : "memory");
+                            }
+                        }
+                        split_commit<CG>(empty + slot);
+                    }
+                    if (!ok) break;
+                    split_commit<CG>(acc_full + acc);
+                }
+            }
+            // what was issued finishes before tensor memory is freed, whatever happened above
+            if constexpr (CG == 1) asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(drain)) : "memory");
+            else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(drain)) : "memory");
+            mbar_wait(drain, 0u, abort_flag + 1);
+        }
+        __syncwarp();
+    } else {
+        // ---- epilogue ---------------------------------------------------------------------------
+        const int ew = warp - 2;                                   // 0..7
+        const uint32_t quarter = (uint32_t)(warp & 3);             // the 32 lanes of tensor memory this warp may read
+        const int half = ew >> 2;                                  // which half of the columns
+        constexpr int kCols = BN / 2;
+        float* piece = pieces + ew * 32 * kSpStageCols;
+        float sum[kCols];
+        uint32_t item = 0;
+        bool ok = true;
+        for (int64_t t = 0; t < my_tiles && ok; ++t) {
+            int64_t batch, i0, j0;
+            tile_of(t, &batch, &i0, &j0);
+            for (uint32_t c = 0; c < chunks; ++c, ++item) {
+                const uint32_t acc = item & 1u;
+                if (!__all_sync(0xffffffffu, mbar_wait(acc_full + acc, (item >> 1) & 1u, abort_flag))) { ok = false; break; }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t taddr = tmem_base + acc * (uint32_t)BN + (uint32_t)(half * kCols) + ((quarter * 32u) << 16);
+#pragma unroll
+                for (int q = 0; q < kCols / 16; ++q) {
+                    uint32_t r[16];
+                    tmem_ld16(taddr + q * 16u, r);
+                    tmem_ld_wait(r);
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) sum[q * 16 + x] = c == 0 ? __uint_as_float(r[x]) : sum[q * 16 + x] + __uint_as_float(r[x]);
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (CG == 1) mbar_arrive(acc_empty + acc);
+                    else asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_cta(smem_u32(acc_empty + acc), 0)) : "memory");
+                }
+            }
+            if (!ok) break;
+            const int64_t row0 = i0 + (int64_t)quarter * 32, col0 = j0 + half * kCols;
+#pragma unroll
+            for (int q = 0; q < kCols / 32; ++q) {
+#pragma unroll
+                for (int x = 0; x < 32; ++x) piece[lane * kSpStageCols + x] = sum[q * 32 + x];
+                __syncwarp();
+                if (row0 < g.m) out.piece(piece, lane, batch, row0, col0 + q * 32, g.m, g.n);
+                __syncwarp();
+            }
+        }
+    }
+
+    // ---- wind-down: everyone meets here, also after a bounded wait ran out ----------------------
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync_all();                     // neither CTA leaves while the other may still arrive at its barriers
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == 1) {
+        if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)(2 * BN)) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)(2 * BN)) : "memory");
+    }
+    if ((abort_flag[0] | abort_flag[1]) && tid == 0) *reinterpret_cast<volatile int*>(g.gave_up) = 1;
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------
+// One word of mapped host memory per process that a kernel sets when a bounded wait ran out; read without synchronising.
+static int* gave_up_word(int** dev) {
+    static std::mutex mu;
+    static int* host = nullptr;
+    std::lock_guard<std::mutex> lock(mu);
+    if (!host) {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;       // the first call may come during a capture
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        void* p = nullptr;
+        const cudaError_t rc = cudaHostAlloc(&p, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (rc != cudaSuccess) { cudaGetLastError(); return nullptr; }
+        host = static_cast<int*>(p);
+        *host = 0;
+    }
+    void* d = nullptr;
+    if (dev) { if (cudaHostGetDevicePointer(&d, host, 0) != cudaSuccess) { cudaGetLastError(); return nullptr; } *dev = static_cast<int*>(d); }
+    return host;
+}
+
+int product_gave_up() {
+    const int* w = gave_up_word(nullptr);
+    return w && *const_cast<const volatile int*>(w) ? (int)cudaErrorLaunchTimeout : 0;
+}
+
+static bool planes_map(CUtensorMap* map, const Planes& x, int planes, int box_rows, SplitKind kind) {
+    TensorMapEncodeFn enc = tensor_map_encoder();
+    if (!enc || !aligned16(x.p) || x.ld % 8 != 0) return false;
+    if (x.inner() > (1LL << 31) - 1024 || x.outer() > (1LL << 31) - 1024 || planes * x.batch > 0x7fffffff) return false;
+    cuuint64_t dim[3] = {(cuuint64_t)x.inner(), (cuuint64_t)x.outer(), (cuuint64_t)(planes * x.batch)};
+    cuuint64_t stride[2] = {(cuuint64_t)x.ld * 2, (cuuint64_t)(x.outer() * x.ld * 2)};
+    cuuint32_t box[3] = {64, (cuuint32_t)(x.k_major ? box_rows : kSpKB), 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return enc(map, kind == kSplitBf16x3 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, x.p, dim, stride, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int P, int CG, int BN, typename Out>
+static int launch_shape(SplitKind kind, const Planes& a, const Planes& b, const Out& out, cudaStream_t st) {
+    using S = SplitShape<P, CG, BN>;
+    SplitArgs g;
+    memset(&g, 0, sizeof g);
+    g.m = a.rows; g.n = b.rows; g.batch = a.batch;
+    g.kblocks = (int)((a.k + kSpKB - 1) / kSpKB);
+    g.tiles_m = (a.rows + 128 * CG - 1) / (128 * CG);
+    g.tiles_n = (b.rows + BN - 1) / BN;
+    g.n_tiles = g.tiles_m * g.tiles_n * a.batch;
+    g.a_k_major = a.k_major; g.b_k_major = b.k_major;
+    const uint32_t fmt = kind == kSplitBf16x3 ? 1u : 0u;
+    g.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((a.k_major ? 0u : 1u) << 15) | ((b.k_major ? 0u : 1u) << 16) | ((uint32_t)(BN >> 3) << 17) |
+              ((uint32_t)((128 * CG) >> 4) << 24);
+    if (!gave_up_word(&g.gave_up)) return (int)cudaErrorMemoryAllocation;
+    CUtensorMap ma, mb;
+    if (!planes_map(&ma, a, P, 128, kind) || !planes_map(&mb, b, P, S::kBRows, kind)) return (int)cudaErrorNotSupported;
+    auto kernel = split_product_kernel<P, CG, BN, Out>;
+    static std::mutex mu;
+    static bool ready[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        if (!ready[dev]) {
+            const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem);
+            if (rc != cudaSuccess) { cudaGetLastError(); return (int)rc; }
+            ready[dev] = true;
+        }
+    }
+    const int64_t slots = sm_count() / CG;
+    const unsigned grid = (unsigned)((g.n_tiles < slots ? g.n_tiles : slots) * CG);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kSpThreads);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CG; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t rc = cudaLaunchKernelEx(&cfg, kernel, g, ma, mb, out);
+    if (rc != cudaSuccess) { cudaGetLastError(); return (int)rc; }
+    count_launch();
+    return 0;
+}
+
+// The tile is the one with the least rounds x (cycles per 16 of K and product): a 256 x 256 pair runs at the tensor cores'
+// 128 cycles, a 128 x 128 or 128 x 64 tile at what shared memory feeds (64 and 48), on twice as many slots.
+template <int P, typename Out>
+static int launch_any(SplitKind kind, const Planes& a, const Planes& b, const Out& out, cudaStream_t st) {
+    if (a.k != b.k || a.batch != b.batch || a.k < 1) return (int)cudaErrorInvalidValue;
+    const int64_t sms = sm_count();
+    auto rounds = [&](int64_t tm, int64_t tn, int64_t slots) {
+        const int64_t tiles = ((a.rows + tm - 1) / tm) * ((b.rows + tn - 1) / tn) * a.batch;
+        return (tiles + slots - 1) / slots;
+    };
+    const int64_t big = rounds(256, 256, sms / 2) * 128, mid = rounds(128, 128, sms) * 72, small = rounds(128, 64, sms) * 50;
+    if (big <= mid && big <= small) return launch_shape<P, 2, 256, Out>(kind, a, b, out, st);
+    if (mid <= small) return launch_shape<P, 1, 128, Out>(kind, a, b, out, st);
+    return launch_shape<P, 1, 64, Out>(kind, a, b, out, st);
+}
+
+int launch_split_product(SplitKind kind, const Planes& a, const Planes& b, const Epilogue<float>& e, cudaStream_t st) {
+    if (e.alpha != 1.0f || e.d) return (int)cudaErrorInvalidValue;
+    const FloatOut out = {e};
+    return kind == kSplitBf16x3 ? launch_any<3>(kind, a, b, out, st) : launch_any<2>(kind, a, b, out, st);
+}
+int launch_split_product(const Planes& a, const Planes& b, const PlaneEpilogue& e, cudaStream_t st) {
+    const PlaneOut out = {e};
+    return launch_any<2>(kSplitHalfx2, a, b, out, st);
+}
+
+}  // namespace cb200
+
+// 0: no bounded wait of the tensor-core product has run out in this process since the last call; 1: one did, and results since
+// then are not valid; -1: the word could not be read.  Synchronises the device; clears the word.
+extern "C" int cb200_product_status(void) {
+    int* w = cb200::gave_up_word(nullptr);
+    if (!w || cudaDeviceSynchronize() != cudaSuccess) return -1;
+    const int v = *const_cast<volatile int*>(w);
+    *const_cast<volatile int*>(w) = 0;
+    return v;
+}

@@ -1,0 +1,70 @@
+// Single-precision products on the 16-bit tensor cores: operands held as a few 16-bit parts ("planes") each.
+//
+// A float is the sum of three bfloat16 numbers to its last bit (8 + 8 + 8 bits, the float's own exponent range), and of two
+// half-precision numbers to 2^-22 of it while it is well inside their narrower range.  With a = a1 + a2 + a3, b alike,
+//     a b = a1 b1 + (a1 b2 + a2 b1) + (a2 b2 + a1 b3 + a3 b1) + terms of 2^-24 a b and below,
+// six bfloat16 products; with two half-precision parts a1 b1 + (a1 b2 + a2 b1), three products.  Products of two 16-bit
+// numbers are exact in the tensor core; what it adds them into is 32 bits wide but truncates, an error that leans one way and
+// grows with the number of additions (2e-8 of the accumulator each, measured), so an accumulator takes 24 instructions'
+// worth of them at most and is then added into registers with ordinary rounded additions.
+#pragma once
+
+#include "linear.cuh"
+
+namespace cb200 {
+
+enum SplitKind { kSplitBf16x3 = 0, kSplitHalfx2 = 1 };
+
+// A matrix of `rows` x `k` (per batch entry) as planes in global memory.  k_major: rows of k contiguous elements, ld apart;
+// otherwise k rows of `rows` contiguous elements.  Plane p of batch entry b starts at (p * batch + b) * rows_or_k * ld.
+struct Planes {
+    uint16_t* p;
+    int64_t rows, k, batch, ld;
+    bool k_major;
+    int64_t outer() const { return k_major ? rows : k; }
+    int64_t inner() const { return k_major ? k : rows; }
+    int64_t plane_elements() const { return batch * outer() * ld; }
+};
+inline int64_t planes_ld(int64_t inner) { return (inner + 7) / 8 * 8; }
+
+// Out of a product of planes into planes (orthogonalisation): v = acc * acc_scale + beta * d * d_scale, stored as two
+// halves of v * out_scale.  All scales are powers of two.
+struct PlaneEpilogue {
+    float acc_scale, beta, d_scale, out_scale;
+    const uint16_t* d;                  // planes of the same shape as the output (two), or null
+    uint16_t* out;
+    int64_t ld, plane;                  // elements per row; elements from one plane to the next
+    int64_t batch_step;
+};
+
+// C = A . B^T (per batch entry), contraction over k; the result leaves through `e` (float) or `pe` (planes).  Returns a
+// cudaError_t; cudaErrorNotSupported when tensor maps cannot be had, in which case nothing was launched.
+int launch_split_product(SplitKind kind, const Planes& a, const Planes& b, const Epilogue<float>& e, cudaStream_t st);
+int launch_split_product(const Planes& a, const Planes& b, const PlaneEpilogue& e, cudaStream_t st);
+
+// Elements that have no parts (infinities, NaN, what bfloat16 rounds to infinity) are left out of the planes and marked by
+// row and by column; fix_marked() then computes the outputs they touch from the operands themselves.
+struct Marks {
+    uint8_t* row;
+    uint8_t* col;
+    int* any;
+};
+// v(i, j) = p[i * row + j * col], times act'(pre(i, j)) when act is not kActNone.
+struct SplitSource {
+    const float* p; int64_t row, col;
+    const float* pre; int64_t pre_row, pre_col;
+    int act;
+};
+
+// The R x C source as three bfloat16 planes, [plane][R][ld].
+int launch_split(const SplitSource& s, int64_t R, int64_t C, uint16_t* planes, int64_t ld, const Marks& marks, cudaStream_t st);
+
+// Outputs i, j with a[i] or b[j] marked, in float from the operands: element (row, k) of A at (row, k) of `a`, or (k, row)
+// if a_turned; B alike.  Returns at once on the device when nothing was marked.
+int launch_fix_marked(int64_t m, int64_t n, int64_t k, const SplitSource& a, bool a_turned, const uint8_t* a_marks, const SplitSource& b, bool b_turned,
+                      const uint8_t* b_marks, const int* any, const Epilogue<float>& e, cudaStream_t st);
+
+// 0, or cudaErrorLaunchTimeout once a bounded wait inside a product has run out on this device (see cb200_product_status).
+int product_gave_up();
+
+}  // namespace cb200

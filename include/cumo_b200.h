@@ -631,6 +631,11 @@ CB200_DECL_GATED(sfloat) CB200_DECL_GATED(dfloat)
         int steps, const double* coefs, double eps, C* out);
 CB200_DECL_LINEAR(sfloat, float) CB200_DECL_LINEAR(dfloat, double)
 
+/* The tensor-core product behind them waits for its copies and instructions with bounds.  0: no wait has run out in this
+ * process since the last call; 1: one did, and results since then are not valid (the entry points above return
+ * cudaErrorLaunchTimeout until this is called); -1: unknown.  Synchronises the device. */
+int cb200_product_status(void);
+
 #ifdef __cplusplus
 }
 #endif
