@@ -197,14 +197,14 @@ static int orthogonalize_split(int64_t batch, int64_t m, int64_t n, bool tall, c
         const Planes X = {x, m, n, batch, ldx, true}, Xn = {x, n, m, batch, ldx, false}, P = {p, m, m, batch, ldp, true}, Q = {q, m, m, batch, ldp, true};
         PlaneEpilogue e = {};
         e.acc_scale = two(-2 * sc.ex[s]); e.out_scale = two(sc.ep[s]); e.out = p; e.ld = ldp; e.plane = pp; e.batch_step = m * ldp;          // P = X X^T
-        rc = launch_split_product(X, X, e, st);
+        rc = launch_split_product(X, X, e, true, st);
         if (rc) break;
         e.acc_scale = c * two(-2 * sc.ep[s]); e.beta = b; e.d = p; e.d_scale = two(-sc.ep[s]); e.out_scale = two(sc.eq[s]); e.out = q;      // Q = b P + c P P
-        rc = launch_split_product(P, P, e, st);
+        rc = launch_split_product(P, P, e, true, st);
         if (rc) break;
         e.acc_scale = two(-sc.eq[s] - sc.ex[s]); e.beta = a; e.d = x; e.d_scale = two(-sc.ex[s]); e.out_scale = two(sc.ex[s + 1]);           // X <- a X + Q X
         e.out = x2; e.ld = ldx; e.plane = px; e.batch_step = m * ldx;
-        rc = launch_split_product(Q, Xn, e, st);
+        rc = launch_split_product(Q, Xn, e, false, st);
         uint16_t* t = x; x = x2; x2 = t;
     }
     if (rc) return rc;

@@ -1,11 +1,12 @@
 // The tensor-core product of split operands (split_product.cuh says what the parts are): tcgen05 with tensor-memory
 // accumulators, operands brought by the tensor memory accelerator.
 //
-// Roles of the 10 warps of a CTA:
+// Roles of the 12 warps of a CTA:
 //   warp 0      one thread issues the TMA loads of a K-block (64 elements of K, all planes of both operands) into a ring of
 //               128-byte-swizzled stages
 //   warp 1      allocates tensor memory; one thread issues the tcgen05.mma's: smallest products first
-//   warps 2..9  epilogue: every 24 instructions' worth of products (a chunk) they add the accumulator from tensor memory
+//   warps 2, 3  idle; this warpgroup gives most of its registers to the others
+//   warps 4..11 epilogue: every 24 instructions' worth of products (a chunk) they add the accumulator from tensor memory
 //               to registers, two accumulators taking turns so that the MMAs never wait; at the end of a tile the sums pass
 //               through a small shared-memory tile per warp, so that global memory is read and written along rows
 // With CG = 2 two CTAs of a cluster share a 256 x 256 tile: each loads its 128 rows of A and its half of B, the first CTA
@@ -24,7 +25,7 @@
 
 namespace cb200 {
 
-constexpr int kSpThreads = 320;
+constexpr int kSpThreads = 384;                 // a warpgroup for loads and products, two for the epilogue
 constexpr int kSpKB = 64;                       // K per stage: one 128-byte swizzle row of 16-bit elements
 constexpr int kSpStageCols = 33;                // epilogue tile: 32 x 32 floats, rows padded by one
 
@@ -46,6 +47,7 @@ struct SplitArgs {
     int64_t tiles_m, tiles_n, n_tiles;          // n_tiles counts all batch entries
     int64_t batch;
     int a_k_major, b_k_major;
+    int symmetric;                              // square tiles on and above the diagonal; what lies above is written to both sides
     uint32_t idesc;
     int* gave_up;
 };
@@ -106,49 +108,120 @@ __device__ __forceinline__ uint64_t umma_desc_mn(uint32_t saddr) {
     return d;
 }
 
-// Out: how a finished 32-row x 32-column piece leaves.  The float form.
+// Out: how a finished 32-row x 32-column piece leaves shared memory.  Loads are issued ahead of the stores that they might
+// alias, several 16-byte packets per lane; rows of the piece are padded by one float, which keeps every access below free of
+// bank conflicts.  The float form:
 struct FloatOut {
     Epilogue<float> e;
-    static constexpr int kind = 0;
-    __device__ __forceinline__ void piece(const float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n) const {
-        const int64_t j = j0 + lane;
-        if (j >= n) return;
+    bool packets;                      // y (and residual) take 16-byte accesses
+    __device__ __forceinline__ void piece(float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n, bool) const {
         const int rows = m - i0 < 32 ? (int)(m - i0) : 32;
-        const float bias = e.bias ? e.bias[j * e.bias_step] : 0.f;
-        const float* res = e.res ? e.res + j * e.res_col : nullptr;
-        int64_t at = batch * e.y_batch + i0 * e.ld + j;
-#pragma unroll 4
-        for (int r = 0; r < rows; ++r, at += e.ld) {
-            float z = tile[r * kSpStageCols + lane];
-            if (e.bias) z += bias;
-            if (e.pre) e.pre[at] = z;
-            float y = e.act == kActNone ? z : activate(z, e.act);
-            if (res) y += res[(i0 + r) * e.res_row];
-            e.y[at] = y;
+        const int64_t y0 = batch * e.y_batch + i0 * e.ld + j0;
+        const bool whole = packets && rows == 32 && j0 + 32 <= n;
+        if (!whole || e.bias || e.pre || e.act != kActNone) {
+            const int64_t j = j0 + lane;
+            if (j < n) {
+                const float bias = e.bias ? e.bias[j * e.bias_step] : 0.f;
+#pragma unroll 2
+                for (int r = 0; r < rows; ++r) {
+                    float z = tile[r * kSpStageCols + lane];
+                    if (e.bias) z += bias;
+                    if (e.pre) e.pre[y0 + r * e.ld + lane] = z;
+                    if (e.act != kActNone) z = activate(z, e.act);
+                    if (whole) { tile[r * kSpStageCols + lane] = z; continue; }
+                    if (e.res) z += e.res[(i0 + r) * e.res_row + j * e.res_col];
+                    e.y[y0 + r * e.ld + lane] = z;
+                }
+            }
+            __syncwarp();
+        }
+        if (!whole) return;
+        const int r0 = lane >> 3, c0 = (lane & 7) * 4;
+#pragma unroll 1
+        for (int h = 0; h < 32; h += 16) {
+            float4 res[4];
+            if (e.res)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) res[q] = __ldcs(reinterpret_cast<const float4*>(e.res + (i0 + h + q * 4 + r0) * e.res_row + j0 + c0));
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int r = h + q * 4 + r0;
+                const float* t = tile + r * kSpStageCols + c0;
+                float4 v = make_float4(t[0], t[1], t[2], t[3]);
+                if (e.res) { v.x += res[q].x; v.y += res[q].y; v.z += res[q].z; v.w += res[q].w; }
+                *reinterpret_cast<float4*>(e.y + y0 + r * e.ld + c0) = v;
+            }
         }
     }
 };
 
-// ... and the form that leaves as two half-precision planes.
+// ... and the form that leaves as two half-precision planes (ld is a multiple of 8, so packets are always aligned; columns
+// between n and ld are padding that nothing reads).
 struct PlaneOut {
     PlaneEpilogue e;
-    static constexpr int kind = 1;
-    __device__ __forceinline__ void piece(const float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n) const {
-        const int64_t j = j0 + lane;
-        if (j >= n) return;
-        const int rows = m - i0 < 32 ? (int)(m - i0) : 32;
-        int64_t at = batch * e.batch_step + i0 * e.ld + j;
-        const __half* d = reinterpret_cast<const __half*>(e.d);
-        __half* out = reinterpret_cast<__half*>(e.out);
-#pragma unroll 4
-        for (int r = 0; r < rows; ++r, at += e.ld) {
-            float v = tile[r * kSpStageCols + lane] * e.acc_scale;
-            if (d) v += e.beta * ((__half2float(d[at]) + __half2float(d[at + e.plane])) * e.d_scale);
-            v *= e.out_scale;
-            const __half hi = __float2half_rn(v);
-            out[at] = hi;
-            out[at + e.plane] = __float2half_rn(v - __half2float(hi));
+    __device__ __forceinline__ void piece(float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n, bool mirror) const {
+        const int r0 = lane >> 2, c0 = (lane & 3) * 8;
+        const int64_t at0 = batch * e.batch_step + (i0 + r0) * e.ld + j0 + c0;
+        const bool here = j0 + c0 < e.ld;
+#pragma unroll 1
+        for (int h = 0; h < 32; h += 16) {
+            uint4 dh[2], dl[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+                if (e.d && here && i0 + h + q * 8 + r0 < m) {
+                    const uint16_t* d = e.d + at0 + (h + q * 8) * e.ld;
+                    dh[q] = *reinterpret_cast<const uint4*>(d);
+                    dl[q] = *reinterpret_cast<const uint4*>(d + e.plane);
+                }
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int r = h + q * 8 + r0;
+                if (!here || i0 + r >= m) continue;
+                float* t = tile + r * kSpStageCols + c0;
+                float v[8];
+                const __half2* ph = reinterpret_cast<const __half2*>(&dh[q]);
+                const __half2* pl = reinterpret_cast<const __half2*>(&dl[q]);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) v[x] = t[x] * e.acc_scale;
+                if (e.d)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const float2 a = __half22float2(ph[x]), b = __half22float2(pl[x]);
+                        v[2 * x] += e.beta * ((a.x + b.x) * e.d_scale);
+                        v[2 * x + 1] += e.beta * ((a.y + b.y) * e.d_scale);
+                    }
+#pragma unroll
+                for (int x = 0; x < 8; ++x) v[x] *= e.out_scale;
+                store(v, at0 + (h + q * 8) * e.ld);
+                if (mirror)
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) t[x] = v[x];
+            }
         }
+        if (!mirror) return;
+        __syncwarp();
+        // the same piece turned: row j0 + r, columns i0 + c ..
+#pragma unroll 1
+        for (int r = r0; r < 32; r += 8) {
+            if (j0 + r >= n || i0 + c0 >= e.ld) continue;
+            float v[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) v[x] = tile[(c0 + x) * kSpStageCols + r];
+            store(v, batch * e.batch_step + (j0 + r) * e.ld + i0 + c0);
+        }
+    }
+    __device__ __forceinline__ void store(const float (&v)[8], int64_t at) const {
+        uint4 oh, ol;
+        __half2* qh = reinterpret_cast<__half2*>(&oh);
+        __half2* ql = reinterpret_cast<__half2*>(&ol);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            qh[x] = __floats2half2_rn(v[2 * x], v[2 * x + 1]);
+            const float2 f = __half22float2(qh[x]);
+            ql[x] = __floats2half2_rn(v[2 * x] - f.x, v[2 * x + 1] - f.y);
+        }
+        *reinterpret_cast<uint4*>(e.out + at) = oh;
+        *reinterpret_cast<uint4*>(e.out + at + e.plane) = ol;
     }
 };
 
@@ -201,9 +274,17 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
     // bands of eight tile rows, walked column by column: the tiles in flight share rows of A and columns of B in L2
     auto tile_of = [&](int64_t t, int64_t* batch, int64_t* i0, int64_t* j0) {
         int64_t f = cluster + t * clusters;
-        const int64_t per = g.tiles_m * g.tiles_n;
+        const int64_t per = g.symmetric ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
         *batch = f / per;
         f -= *batch * per;
+        if (g.symmetric) {                                       // column by column: tile column c holds rows 0 .. c
+            int64_t c = (int64_t)((sqrtf(8.f * (float)f + 1.f) - 1.f) * 0.5f);
+            while (c * (c + 1) / 2 > f) --c;
+            while ((c + 1) * (c + 2) / 2 <= f) ++c;
+            *j0 = c * BN;
+            *i0 = (f - c * (c + 1) / 2) * (128 * CG) + rank * 128;
+            return;
+        }
         const int64_t band = f / (8 * g.tiles_n);
         const int64_t height = g.tiles_m - band * 8 < 8 ? g.tiles_m - band * 8 : 8;
         f -= band * 8 * g.tiles_n;
@@ -211,6 +292,9 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
         *i0 = (band * 8 + f % height) * (128 * CG) + rank * 128;
     };
 
+    // 384 threads of 168 registers: 128 keep 56 each, which leaves 224 for each of the other 256 (56 + 2 * 224 = 3 * 168)
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0) {
         // ---- loads ------------------------------------------------------------------------------
         if (lane == 0) {
@@ -298,9 +382,11 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
             mbar_wait(drain, 0u, abort_flag + 1);
         }
         __syncwarp();
+    }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         // ---- epilogue ---------------------------------------------------------------------------
-        const int ew = warp - 2;                                   // 0..7
+        const int ew = warp - 4;                                   // 0..7
         const uint32_t quarter = (uint32_t)(warp & 3);             // the 32 lanes of tensor memory this warp may read
         const int half = ew >> 2;                                  // which half of the columns
         constexpr int kCols = BN / 2;
@@ -316,13 +402,20 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
                 if (!__all_sync(0xffffffffu, mbar_wait(acc_full + acc, (item >> 1) & 1u, abort_flag))) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t taddr = tmem_base + acc * (uint32_t)BN + (uint32_t)(half * kCols) + ((quarter * 32u) << 16);
+                // 16 columns are added while the next 16 are on their way
+                uint32_t ra[16], rb[16];
+                tmem_ld16(taddr, ra);
+                tmem_ld_wait(ra);
 #pragma unroll
-                for (int q = 0; q < kCols / 16; ++q) {
-                    uint32_t r[16];
-                    tmem_ld16(taddr + q * 16u, r);
-                    tmem_ld_wait(r);
+                for (int q = 0; q < kCols / 16; q += 2) {
+                    tmem_ld16(taddr + (q + 1) * 16u, rb);
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) sum[q * 16 + x] = c == 0 ? __uint_as_float(r[x]) : sum[q * 16 + x] + __uint_as_float(r[x]);
+                    for (int x = 0; x < 16; ++x) sum[q * 16 + x] = c == 0 ? __uint_as_float(ra[x]) : sum[q * 16 + x] + __uint_as_float(ra[x]);
+                    tmem_ld_wait(rb);
+                    if (q + 2 < kCols / 16) tmem_ld16(taddr + (q + 2) * 16u, ra);
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) sum[q * 16 + 16 + x] = c == 0 ? __uint_as_float(rb[x]) : sum[q * 16 + 16 + x] + __uint_as_float(rb[x]);
+                    if (q + 2 < kCols / 16) tmem_ld_wait(ra);
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
@@ -338,7 +431,7 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
 #pragma unroll
                 for (int x = 0; x < 32; ++x) piece[lane * kSpStageCols + x] = sum[q * 32 + x];
                 __syncwarp();
-                if (row0 < g.m) out.piece(piece, lane, batch, row0, col0 + q * 32, g.m, g.n);
+                if (row0 < g.m) out.piece(piece, lane, batch, row0, col0 + q * 32, g.m, g.n, g.symmetric && i0 / (128 * CG) != j0 / BN);
                 __syncwarp();
             }
         }
@@ -395,7 +488,7 @@ static bool planes_map(CUtensorMap* map, const Planes& x, int planes, int box_ro
 }
 
 template <int P, int CG, int BN, typename Out>
-static int launch_shape(SplitKind kind, const Planes& a, const Planes& b, const Out& out, cudaStream_t st) {
+static int launch_shape(SplitKind kind, const Planes& a, const Planes& b, const Out& out, bool symmetric, cudaStream_t st) {
     using S = SplitShape<P, CG, BN>;
     SplitArgs g;
     memset(&g, 0, sizeof g);
@@ -403,7 +496,8 @@ static int launch_shape(SplitKind kind, const Planes& a, const Planes& b, const 
     g.kblocks = (int)((a.k + kSpKB - 1) / kSpKB);
     g.tiles_m = (a.rows + 128 * CG - 1) / (128 * CG);
     g.tiles_n = (b.rows + BN - 1) / BN;
-    g.n_tiles = g.tiles_m * g.tiles_n * a.batch;
+    g.symmetric = symmetric && BN == 128 * CG;
+    g.n_tiles = (g.symmetric ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n) * a.batch;
     g.a_k_major = a.k_major; g.b_k_major = b.k_major;
     const uint32_t fmt = kind == kSplitBf16x3 ? 1u : 0u;
     g.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((a.k_major ? 0u : 1u) << 15) | ((b.k_major ? 0u : 1u) << 16) | ((uint32_t)(BN >> 3) << 17) |
@@ -443,30 +537,32 @@ static int launch_shape(SplitKind kind, const Planes& a, const Planes& b, const 
     return 0;
 }
 
-// The tile is the one with the least rounds x (cycles per 16 of K and product): a 256 x 256 pair runs at the tensor cores'
-// 128 cycles, a 128 x 128 or 128 x 64 tile at what shared memory feeds (64 and 48), on twice as many slots.
+// The tile is the one with the least rounds x time per round, in cycles per 16 of K and product: measured at 4096^3, a
+// 256 x 256 pair takes the tensor cores' 128, a 128 x 128 tile 95 and a 128 x 64 tile 70 (bound by what L2 delivers), the
+// latter two on twice as many slots.
 template <int P, typename Out>
-static int launch_any(SplitKind kind, const Planes& a, const Planes& b, const Out& out, cudaStream_t st) {
-    if (a.k != b.k || a.batch != b.batch || a.k < 1) return (int)cudaErrorInvalidValue;
+static int launch_any(SplitKind kind, const Planes& a, const Planes& b, const Out& out, bool symmetric, cudaStream_t st) {
+    if (a.k != b.k || a.batch != b.batch || a.k < 1 || (symmetric && a.rows != b.rows)) return (int)cudaErrorInvalidValue;
     const int64_t sms = sm_count();
     auto rounds = [&](int64_t tm, int64_t tn, int64_t slots) {
-        const int64_t tiles = ((a.rows + tm - 1) / tm) * ((b.rows + tn - 1) / tn) * a.batch;
+        const int64_t across = (a.rows + tm - 1) / tm;
+        const int64_t tiles = (symmetric && tm == tn ? across * (across + 1) / 2 : across * ((b.rows + tn - 1) / tn)) * a.batch;
         return (tiles + slots - 1) / slots;
     };
-    const int64_t big = rounds(256, 256, sms / 2) * 128, mid = rounds(128, 128, sms) * 72, small = rounds(128, 64, sms) * 50;
-    if (big <= mid && big <= small) return launch_shape<P, 2, 256, Out>(kind, a, b, out, st);
-    if (mid <= small) return launch_shape<P, 1, 128, Out>(kind, a, b, out, st);
-    return launch_shape<P, 1, 64, Out>(kind, a, b, out, st);
+    const int64_t big = rounds(256, 256, sms / 2) * 128, mid = rounds(128, 128, sms) * 95, small = rounds(128, 64, sms) * 70;
+    if (big <= mid && big <= small) return launch_shape<P, 2, 256, Out>(kind, a, b, out, symmetric, st);
+    if (mid <= small) return launch_shape<P, 1, 128, Out>(kind, a, b, out, symmetric, st);
+    return launch_shape<P, 1, 64, Out>(kind, a, b, out, symmetric, st);
 }
 
 int launch_split_product(SplitKind kind, const Planes& a, const Planes& b, const Epilogue<float>& e, cudaStream_t st) {
     if (e.alpha != 1.0f || e.d) return (int)cudaErrorInvalidValue;
-    const FloatOut out = {e};
-    return kind == kSplitBf16x3 ? launch_any<3>(kind, a, b, out, st) : launch_any<2>(kind, a, b, out, st);
+    const FloatOut out = {e, e.ld % 4 == 0 && aligned16(e.y) && (!e.res || (e.res_col == 1 && e.res_row % 4 == 0 && aligned16(e.res)))};
+    return kind == kSplitBf16x3 ? launch_any<3>(kind, a, b, out, false, st) : launch_any<2>(kind, a, b, out, false, st);
 }
-int launch_split_product(const Planes& a, const Planes& b, const PlaneEpilogue& e, cudaStream_t st) {
+int launch_split_product(const Planes& a, const Planes& b, const PlaneEpilogue& e, bool symmetric, cudaStream_t st) {
     const PlaneOut out = {e};
-    return launch_any<2>(kSplitHalfx2, a, b, out, st);
+    return launch_any<2>(kSplitHalfx2, a, b, out, symmetric, st);
 }
 
 }  // namespace cb200
