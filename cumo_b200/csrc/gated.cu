@@ -15,8 +15,15 @@
 // composition are held in 64 bits, where it neither underflows in a way that could be seen in 32 bits nor loses digits.
 //
 // Three plans, all bound by memory traffic (3 s bytes per element forward, 5 s backward):
-//   walk    a thread per run, in order: many runs, or few steps
-#include "common.cuh"
+//   walk    a thread per run (or per 16-byte group of neighbouring runs), in order: many runs, or few steps
+//   strip   runs side by side in memory, too few of them to fill the GPU with a thread each: a CTA owns 32 lanes' runs, its
+//           warps take stretches of eight steps, and up to eight CTAs of a cluster take turns along the run, handing their
+//           stretches' (A, B) to one another through distributed shared memory
+//   rows    runs that are contiguous along the axis themselves: a warp, a CTA or a cluster per run, tiles turned through
+//           shared memory so that global accesses run along the axis while a thread owns consecutive steps
+#include <cooperative_groups.h>
+
+#include "linear.cuh"
 
 namespace cb200 {
 
@@ -59,44 +66,443 @@ __device__ __forceinline__ void gst(char* p, const GVec<T, V>& v) {
 __device__ __forceinline__ float gfma(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ double gfma(double a, double b, double c) { return fma(a, b, c); }
 
-// ---- walk: a thread per run ------------------------------------------------------------------------------------------
-constexpr int kWalkAhead = 8;
+// Gate modes of the packet kernels: the V runs of a lane have V neighbouring gates, or share one.
+enum GateMode { kGateOwn = 0, kGateShared = 1 };
 
-template <typename T, bool GRAD>
+// ---- walk: a thread per V neighbouring runs -----------------------------------------------------------------------------
+// Each thread keeps U steps of loads in flight; consecutive threads own consecutive runs, so that a step is one coalesced
+// access where the runs lie side by side.
+template <typename T, int V, int GM, bool GRAD>
 __global__ void __launch_bounds__(kBlock)
 gated_walk_kernel(const GatedRuns g) {
-    for (int64_t run = (int64_t)blockIdx.x * kBlock + threadIdx.x; run < g.runs; run += (int64_t)gridDim.x * kBlock) {
+    constexpr int U = V * sizeof(T) == 16 ? 4 : 8;
+    constexpr int GV = GM == kGateShared ? 1 : V;
+    const int64_t groups = g.runs / V;
+    for (int64_t group = (int64_t)blockIdx.x * kBlock + threadIdx.x; group < groups; group += (int64_t)gridDim.x * kBlock) {
+        int64_t off[7];
+        offsets_of<7>(group * V, g.nd, g.shape, g.step, off);
+        const char* u = g.u + off[0];
+        const char* a = g.a + off[1];
+        char* o = g.o + off[2];
+        const char* p = GRAD ? g.p + off[4] : nullptr;
+        char* q = GRAD ? g.q + off[5] : nullptr;
+        const int64_t i_step = g.nd > 0 ? g.step[3][g.nd - 1] : 0, d_step = g.nd > 0 ? g.step[6][g.nd - 1] : 0;
+        T init[V], h[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) init[v] = g.init ? *reinterpret_cast<const T*>(g.init + off[3] + v * i_step) : T(0);
+        const bool enters = !GRAD && g.init;              // a state enters at scan step 0
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = enters ? init[v] : T(0);
+        for (int64_t s0 = 0; s0 < g.n; s0 += U) {
+            GVec<T, V> uu[U], pp[U];
+            GVec<T, GV> aa[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int64_t s = s0 + i;
+                if (s >= g.n) break;
+                uu[i] = gld<T, V>(u + s * g.s_u);
+                if (s > 0 || enters) aa[i] = gld<T, GV>(a + s * g.s_a);
+                if (GRAD && s + 1 < g.n) pp[i] = gld<T, V>(p + s * g.s_p);
+            }
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int64_t s = s0 + i;
+                if (s >= g.n) break;
+                const bool first = !(s > 0 || enters), last = s + 1 >= g.n;
+                GVec<T, V> out, dg;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    h[v] = first ? uu[i].v[v] : gfma(aa[i].v[GM == kGateShared ? 0 : v], h[v], uu[i].v[v]);
+                    out.v[v] = h[v];
+                    if (GRAD) dg.v[v] = !last ? h[v] * pp[i].v[v] : g.init ? h[v] * init[v] : T(0);
+                }
+                gst<T, V>(o + s * g.s_o, out);
+                if (GRAD) gst<T, V>(q + s * g.s_q, dg);
+            }
+        }
+        if (GRAD && g.dinit) {
+            const GVec<T, GV> a0 = gld<T, GV>(a + g.n * g.s_a);
+#pragma unroll
+            for (int v = 0; v < V; ++v) *reinterpret_cast<T*>(g.dinit + off[6] + v * d_step) = a0.v[GM == kGateShared ? 0 : v] * h[v];
+        }
+    }
+}
+
+// ---- composing stretches --------------------------------------------------------------------------------------------
+// The state behind a stretch, A * h + B.  Pairs are held in 64 bits and rounded once, into the state they lead to.
+__device__ __forceinline__ double compose(double A, double B, double h) { return fma(A, h, B); }
+
+// A product of finite gates stays finite and a product of non-zero gates stays non-zero: where the recurrence would carry 0
+// past growing gates, or an infinity past shrinking ones, so does the pair.
+__device__ __forceinline__ double gates_times(double x, double y) {
+    double r = x * y;
+    if (isinf(r) && !isinf(x) && !isinf(y)) r = copysign(1.7976931348623157e308, r);
+    if (r == 0.0 && x != 0.0 && y != 0.0) r = copysign(4.9406564584124654e-324, r);
+    return r;
+}
+
+// ---- strip: 32 lanes x V runs, time cut over warps and over the CTAs of a cluster ----------------------------------------
+constexpr int kStripSteps = 8;                       // steps of a warp per round
+constexpr int kStripWarps = 8;
+
+template <typename T, int V, int GM, bool GRAD>
+__global__ void __launch_bounds__(kBlock, 2)
+gated_strip_kernel(const GatedRuns g, int cluster_size) {
+    namespace cg = cooperative_groups;
+    constexpr int L = kStripSteps, W = kStripWarps;
+    constexpr int GV = GM == kGateShared ? 1 : V;
+    __shared__ double warp_A[2][W][GV][32];           // two rounds' worth: one barrier per round is enough
+    __shared__ double warp_B[2][W][V][32];
+    __shared__ double cta_A[2][GV][32];               // this CTA's stretch, read by the others of the cluster
+    __shared__ double cta_B[2][V][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = cluster_size > 1 ? (int)cluster.block_rank() : 0;
+    const int64_t strip = blockIdx.x / cluster_size;
+    const int64_t group = strip * 32 + lane;
+    const bool live = group < g.runs / V;
+    int64_t off[7];
+    offsets_of<7>(live ? group * V : 0, g.nd, g.shape, g.step, off);
+    const char* u = g.u + off[0];
+    const char* a = g.a + off[1];
+    char* o = g.o + off[2];
+    const char* p = GRAD ? g.p + off[4] : nullptr;
+    char* q = GRAD ? g.q + off[5] : nullptr;
+    const int64_t i_step = g.nd > 0 ? g.step[3][g.nd - 1] : 0, d_step = g.nd > 0 ? g.step[6][g.nd - 1] : 0;
+    const bool enters = !GRAD && g.init;
+    double H[V];                                      // state in front of this round, the same in every warp and CTA of the cluster
+#pragma unroll
+    for (int v = 0; v < V; ++v) H[v] = enters && live ? (double)*reinterpret_cast<const T*>(g.init + off[3] + v * i_step) : 0.0;
+    const int64_t per_round = (int64_t)cluster_size * W * L;
+    const int64_t rounds = (g.n + per_round - 1) / per_round;
+    for (int64_t round = 0; round < rounds; ++round) {
+        const int64_t s0 = round * per_round + (int64_t)(rank * W + warp) * L;
+        const int buf = (int)(round & 1);
+        GVec<T, V> uu[L], pp[L];
+        GVec<T, GV> aa[L];
+        const int steps = !live || s0 >= g.n ? 0 : g.n - s0 < L ? (int)(g.n - s0) : L;
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            if (i >= steps) break;
+            const int64_t s = s0 + i;
+            uu[i] = gld<T, V>(u + s * g.s_u);
+            if (s > 0 || enters) aa[i] = gld<T, GV>(a + s * g.s_a);
+        }
+        if (GRAD) {
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                if (i >= steps) break;
+                if (s0 + i + 1 < g.n) pp[i] = gld<T, V>(p + (s0 + i) * g.s_p);
+            }
+        }
+        // this warp's stretch from a zero state; the very first step starts from nothing, whatever its gate is
+        double A[GV];
+        T B[V];
+#pragma unroll
+        for (int x = 0; x < GV; ++x) A[x] = 1.0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) B[v] = T(0);
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            if (i >= steps) break;
+            if (s0 + i == 0 && !enters) {
+#pragma unroll
+                for (int x = 0; x < GV; ++x) A[x] = 0.0;
+#pragma unroll
+                for (int v = 0; v < V; ++v) B[v] = uu[0].v[v];
+                continue;
+            }
+#pragma unroll
+            for (int x = 0; x < GV; ++x) A[x] *= (double)aa[i].v[x];
+#pragma unroll
+            for (int v = 0; v < V; ++v) B[v] = i == 0 ? uu[i].v[v] : gfma(aa[i].v[GM == kGateShared ? 0 : v], B[v], uu[i].v[v]);
+        }
+#pragma unroll
+        for (int x = 0; x < GV; ++x) {
+            if (isinf(A[x]) || A[x] == 0.0) {                    // by overflow or underflow, or by a gate that is infinite or 0 itself?
+                A[x] = 1.0;
+#pragma unroll
+                for (int i = 0; i < L; ++i)
+                    if (i < steps) A[x] = s0 + i > 0 || enters ? gates_times(A[x], (double)aa[i].v[x]) : 0.0;
+            }
+            warp_A[buf][warp][x][lane] = A[x];
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) warp_B[buf][warp][v][lane] = (double)B[v];
+        __syncthreads();
+        double before[V];
+        if (cluster_size > 1) {
+            if (warp < V) {                                      // warp v folds the CTA's stretches of run v of each lane
+                const int v = warp;
+                double fa = warp_A[buf][0][GM == kGateShared ? 0 : v][lane], fb = warp_B[buf][0][v][lane];
+#pragma unroll
+                for (int w = 1; w < W; ++w) {
+                    const double wa = warp_A[buf][w][GM == kGateShared ? 0 : v][lane];
+                    fb = compose(wa, warp_B[buf][w][v][lane], fb);
+                    fa = gates_times(fa, wa);
+                }
+                if (v < GV) cta_A[buf][v][lane] = fa;
+                cta_B[buf][v][lane] = fb;
+            }
+            cluster.sync();
+            for (int r = 0; r < cluster_size; ++r) {
+                const double* ra = cluster.map_shared_rank(&cta_A[buf][0][0], r);
+                const double* rb = cluster.map_shared_rank(&cta_B[buf][0][0], r);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    if (r == rank) before[v] = H[v];
+                    H[v] = compose(ra[(GM == kGateShared ? 0 : v) * 32 + lane], rb[v * 32 + lane], H[v]);
+                }
+            }
+            for (int w = 0; w < warp; ++w)
+#pragma unroll
+                for (int v = 0; v < V; ++v) before[v] = compose(warp_A[buf][w][GM == kGateShared ? 0 : v][lane], warp_B[buf][w][v][lane], before[v]);
+        } else {
+#pragma unroll
+            for (int w = 0; w < W; ++w)
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    if (w == warp) before[v] = H[v];
+                    H[v] = compose(warp_A[buf][w][GM == kGateShared ? 0 : v][lane], warp_B[buf][w][v][lane], H[v]);
+                }
+        }
+        T h[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = (T)before[v];
+        // again, from the state in front
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            if (i >= steps) break;
+            const int64_t s = s0 + i;
+            const bool last = s + 1 >= g.n;
+            GVec<T, V> out, dg;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                h[v] = s > 0 || enters ? gfma(aa[i].v[GM == kGateShared ? 0 : v], h[v], uu[i].v[v]) : uu[i].v[v];
+                out.v[v] = h[v];
+                if (GRAD) {
+                    T prior = T(0);
+                    if (!last) prior = pp[i].v[v];
+                    else if (g.init) prior = *reinterpret_cast<const T*>(g.init + off[3] + v * i_step);
+                    dg.v[v] = last && !g.init ? T(0) : h[v] * prior;
+                }
+            }
+            gst<T, V>(o + s * g.s_o, out);
+            if (GRAD) gst<T, V>(q + s * g.s_q, dg);
+            if (GRAD && last && g.dinit) {
+                const GVec<T, GV> a0 = gld<T, GV>(a + g.n * g.s_a);
+#pragma unroll
+                for (int v = 0; v < V; ++v) *reinterpret_cast<T*>(g.dinit + off[6] + v * d_step) = a0.v[GM == kGateShared ? 0 : v] * h[v];
+            }
+        }
+    }
+    if (cluster_size > 1) cluster.sync();                        // nobody leaves while its pairs may still be read
+}
+
+// ---- rows: runs contiguous along the axis -----------------------------------------------------------------------------------
+// G threads per run (a warp, or the CTA, or the CTAs of a cluster in turns), kRowItems consecutive steps per thread.  A tile
+// is copied into shared memory along the axis, padded so that threads reading their own steps hit different banks, and the
+// results go back the same way.
+constexpr int kRowItems = 8;
+
+template <typename T>
+__device__ __forceinline__ int row_slot(int i) { return i + i / kRowItems; }       // one element of padding per thread
+
+template <typename T, int G, bool GRAD>
+__global__ void __launch_bounds__(kBlock)
+gated_rows_kernel(const GatedRuns g, int cluster_size) {
+    namespace cg = cooperative_groups;
+    constexpr int I = kRowItems, TILE = G * I, SLOTS = TILE + G, PER_CTA = kBlock / G;
+    extern __shared__ __align__(16) char smem[];
+    __shared__ double warp_A[kWarpsPerBlock], warp_B[kWarpsPerBlock];
+    __shared__ double cta_A[2], cta_B[2];
+    int buf = 0;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int me = threadIdx.x % G, slot = threadIdx.x / G;
+    T* su = reinterpret_cast<T*>(smem) + (size_t)slot * SLOTS * (GRAD ? 3 : 2);
+    T* sa = su + SLOTS;
+    T* sp = sa + SLOTS;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = cluster_size > 1 ? (int)cluster.block_rank() : 0;
+    const int64_t first = (int64_t)(blockIdx.x / cluster_size) * PER_CTA, stride = (int64_t)(gridDim.x / cluster_size) * PER_CTA;
+    auto sync = [&]() { if (G > 32) __syncthreads(); else __syncwarp(); };
+    for (int64_t base = first; base < g.runs; base += stride) {
+        const int64_t run = base + slot;
+        if (G <= 32 && run >= g.runs) break;                     // (a whole warp leaves; the CTA form has one run per CTA)
         int64_t off[7];
         offsets_of<7>(run, g.nd, g.shape, g.step, off);
         const char* u = g.u + off[0];
         const char* a = g.a + off[1];
         char* o = g.o + off[2];
-        const T init = g.init ? *reinterpret_cast<const T*>(g.init + off[3]) : T(0);
         const char* p = GRAD ? g.p + off[4] : nullptr;
         char* q = GRAD ? g.q + off[5] : nullptr;
-        const bool enters = !GRAD && g.init;              // a state enters at scan step 0
-        T h = enters ? init : T(0);
-        for (int64_t s0 = 0; s0 < g.n; s0 += kWalkAhead) {
-            T uu[kWalkAhead], aa[kWalkAhead], pp[kWalkAhead];
+        const T init = g.init ? *reinterpret_cast<const T*>(g.init + off[3]) : T(0);
+        const bool enters = !GRAD && g.init;
+        double H = enters ? (double)init : 0.0;
+        const int64_t per_round = (int64_t)cluster_size * TILE, rounds = (g.n + per_round - 1) / per_round;
+        for (int64_t round = 0; round < rounds; ++round) {
+            const int64_t s0 = round * per_round + (int64_t)rank * TILE;
+            const int count = s0 >= g.n ? 0 : g.n - s0 < TILE ? (int)(g.n - s0) : TILE;
+            T lu[I], la[I], lp[I];
 #pragma unroll
-            for (int i = 0; i < kWalkAhead; ++i) {
-                const int64_t s = s0 + i;
-                if (s >= g.n) break;
-                uu[i] = *reinterpret_cast<const T*>(u + s * g.s_u);
-                aa[i] = s > 0 || enters ? *reinterpret_cast<const T*>(a + s * g.s_a) : T(0);
-                if (GRAD) pp[i] = s + 1 < g.n ? *reinterpret_cast<const T*>(p + s * g.s_p) : init;
+            for (int i = 0; i < I; ++i) {
+                const int e = i * G + me;
+                const int64_t s = s0 + e;
+                lu[i] = e < count ? ld_one<T>(u + s * g.s_u) : T(0);
+                la[i] = e < count && (s > 0 || enters) ? ld_one<T>(a + s * g.s_a) : T(1);
+                if (GRAD) lp[i] = e >= count ? T(0) : s + 1 < g.n ? ld_one<T>(p + s * g.s_p) : init;
             }
 #pragma unroll
-            for (int i = 0; i < kWalkAhead; ++i) {
-                const int64_t s = s0 + i;
-                if (s >= g.n) break;
-                h = s > 0 || enters ? gfma(aa[i], h, uu[i]) : uu[i];
-                *reinterpret_cast<T*>(o + s * g.s_o) = h;
-                if (GRAD) *reinterpret_cast<T*>(q + s * g.s_q) = s + 1 < g.n || g.init ? h * pp[i] : T(0);
+            for (int i = 0; i < I; ++i) {
+                const int e = row_slot<T>(i * G + me);
+                su[e] = lu[i]; sa[e] = la[i];
+                if (GRAD) sp[e] = lp[i];
             }
+            sync();
+            // this thread's steps from a zero state
+            T x[I], c[I];
+            const int mine = me * (I + 1);
+            double A = 1.0;
+            T b = T(0);
+#pragma unroll
+            for (int i = 0; i < I; ++i) {
+                x[i] = su[mine + i]; c[i] = sa[mine + i];
+                A *= (double)c[i];
+                b = i == 0 ? x[0] : gfma(c[i], b, x[i]);
+            }
+            if (isinf(A) || A == 0.0) {
+                A = 1.0;
+#pragma unroll
+                for (int i = 0; i < I; ++i) A = gates_times(A, (double)c[i]);
+            }
+            const bool starts = s0 + me * I == 0 && !enters;     // the first step of all starts from nothing
+            if (starts) A = 0.0;
+            double B = (double)b;
+            // pairs of this and all threads before it, within the warp
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const double pa = __shfl_up_sync(0xffffffffu, A, d), pb = __shfl_up_sync(0xffffffffu, B, d);
+                if (lane >= d) { B = compose(A, B, pb); A = gates_times(A, pa); }
+            }
+            double before = H;
+            if (G > 32) {
+                if (lane == 31) { warp_A[warp] = A; warp_B[warp] = B; }
+                __syncthreads();
+                if (cluster_size > 1) {
+                    if (threadIdx.x == 0) {
+                        double fa = warp_A[0], fb = warp_B[0];
+#pragma unroll
+                        for (int w = 1; w < kWarpsPerBlock; ++w) { fb = compose(warp_A[w], warp_B[w], fb); fa = gates_times(fa, warp_A[w]); }
+                        cta_A[buf] = fa; cta_B[buf] = fb;
+                    }
+                    cluster.sync();
+                    for (int r = 0; r < cluster_size; ++r) {
+                        if (r == rank) before = H;
+                        H = compose(*cluster.map_shared_rank(&cta_A[buf], r), *cluster.map_shared_rank(&cta_B[buf], r), H);
+                    }
+                    buf ^= 1;                                    // (across runs too: the others may still read this one)
+                    for (int w = 0; w < warp; ++w) before = compose(warp_A[w], warp_B[w], before);
+                } else {
+#pragma unroll
+                    for (int w = 0; w < kWarpsPerBlock; ++w) {
+                        if (w == warp) before = H;
+                        H = compose(warp_A[w], warp_B[w], H);
+                    }
+                }
+            } else {
+                H = compose(__shfl_sync(0xffffffffu, A, 31), __shfl_sync(0xffffffffu, B, 31), H);
+            }
+            const double ea = __shfl_up_sync(0xffffffffu, A, 1), eb = __shfl_up_sync(0xffffffffu, B, 1);
+            T h = (T)(lane > 0 ? compose(ea, eb, before) : before);
+#pragma unroll
+            for (int i = 0; i < I; ++i) {
+                h = i == 0 && starts ? x[0] : gfma(c[i], h, x[i]);
+                if (GRAD) {
+                    const int64_t s = s0 + me * I + i;
+                    const bool last = s + 1 == g.n;
+                    sa[mine + i] = last && !g.init ? T(0) : h * sp[mine + i];
+                    if (last && g.dinit) *reinterpret_cast<T*>(g.dinit + off[6]) = *reinterpret_cast<const T*>(a + g.n * g.s_a) * h;
+                }
+                su[mine + i] = h;
+            }
+            sync();
+#pragma unroll
+            for (int i = 0; i < I; ++i) {
+                const int e = i * G + me;
+                if (e < count) {
+                    st_one<T>(o + (s0 + e) * g.s_o, su[row_slot<T>(e)]);
+                    if (GRAD) st_one<T>(q + (s0 + e) * g.s_q, sa[row_slot<T>(e)]);
+                }
+            }
+            sync();
         }
-        if (GRAD && g.dinit) *reinterpret_cast<T*>(g.dinit + off[6]) = *reinterpret_cast<const T*>(a + g.n * g.s_a) * h;
     }
+    if (cluster_size > 1) cluster.sync();
+}
+
+// ---- choice of plan -------------------------------------------------------------------------------------------------------
+template <typename K>
+static int launch_cluster(K kernel, const GatedRuns& g, unsigned ctas, int cluster, size_t smem) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kBlock);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = current_stream();
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t rc = cudaLaunchKernelEx(&cfg, kernel, g, cluster);
+    if (rc != cudaSuccess) { cudaGetLastError(); return (int)rc; }
+    count_launch();
+    return 0;
+}
+
+// CTAs of a cluster per strip (or row): enough that the GPU has about two resident CTAs per SM's worth, no more than the steps feed.
+static int cluster_for(int64_t ctas, int64_t steps, int64_t steps_per_cta) {
+    int c = 1;
+    while (c < 8 && ctas * c < (int64_t)sm_count() * 2 && steps > steps_per_cta * c) c *= 2;
+    return c;
+}
+
+template <typename T, int V, int GM, bool GRAD>
+static int launch_side_by_side(const GatedRuns& g) {
+    const int64_t groups = g.runs / V;
+    // a thread per group when that alone keeps enough loads in flight (16 bytes x 4 steps x 2 operands each, about 44 KiB per
+    // SM wanted), or when there is little to cut
+    if (groups >= (int64_t)sm_count() * 512 || g.n <= 2 * kStripSteps) {
+        gated_walk_kernel<T, V, GM, GRAD><<<grid_for((groups + kBlock - 1) / kBlock, 8), kBlock, 0, current_stream()>>>(g);
+        count_launch();
+        return (int)cudaGetLastError();
+    }
+    const int64_t strips = (groups + 31) / 32;
+    const int cluster = cluster_for(strips, g.n, kStripSteps * kStripWarps);
+    if (strips * cluster > 0x7fffffff) return (int)cudaErrorInvalidValue;
+    return launch_cluster(gated_strip_kernel<T, V, GM, GRAD>, g, (unsigned)(strips * cluster), cluster, 0);
+}
+
+template <typename T, bool GRAD>
+static int launch_rows(const GatedRuns& g) {
+    const int64_t tile = (int64_t)kBlock * kRowItems;
+    constexpr int arrays = GRAD ? 3 : 2;
+    constexpr size_t smem = (size_t)arrays * (kBlock * kRowItems + kBlock) * sizeof(T);
+    if (g.n <= 32 * kRowItems * 2 || g.runs >= (int64_t)sm_count() * 32) {
+        const unsigned grid = grid_for((g.runs + kWarpsPerBlock - 1) / kWarpsPerBlock, 6);
+        if (smem > 48 * 1024) {
+            const cudaError_t rc = cudaFuncSetAttribute(gated_rows_kernel<T, 32, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            if (rc != cudaSuccess) return (int)rc;
+        }
+        return launch_cluster(gated_rows_kernel<T, 32, GRAD>, g, grid, 1, smem);
+    }
+    if (smem > 48 * 1024) {
+        const cudaError_t rc = cudaFuncSetAttribute(gated_rows_kernel<T, kBlock, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (rc != cudaSuccess) return (int)rc;
+    }
+    const int64_t most = (int64_t)sm_count() * 6;
+    const int cluster = cluster_for(g.runs, g.n, tile);
+    const int64_t rows = g.runs < most ? g.runs : most;
+    return launch_cluster(gated_rows_kernel<T, kBlock, GRAD>, g, (unsigned)(rows * cluster), cluster, smem);
 }
 
 template <typename T, bool GRAD>
@@ -118,10 +524,23 @@ static int gated_launch(GatedRuns& g) {
         }
     }
     g.nd = nd;
-    const unsigned grid = grid_for((g.runs + kBlock - 1) / kBlock, 8);
-    gated_walk_kernel<T, GRAD><<<grid, kBlock, 0, current_stream()>>>(g);
-    count_launch();
-    return (int)cudaGetLastError();
+    // Which dimension runs along memory?  Whole packets of neighbouring runs need every per-run operand contiguous and aligned
+    // there (the gate may also be one for all of them).
+    constexpr int ES = sizeof(T), V = 16 / ES;
+    const int in = nd - 1;
+    const bool side = nd > 0 && g.step[0][in] == ES && g.step[2][in] == ES && (!GRAD || (g.step[4][in] == ES && g.step[5][in] == ES));
+    const bool shared_gate = nd > 0 && g.step[1][in] == 0;
+    auto even = [&](const char* p, int k, int64_t s) {
+        bool ok = aligned16(p) && mult16(s);
+        for (int d = 0; d < in && ok; ++d) ok = mult16(g.step[k][d]);
+        return ok;
+    };
+    if (side && (shared_gate || g.step[1][in] == ES) && g.shape[in] % V == 0 && even(g.u, 0, g.s_u) && even(g.o, 2, g.s_o) &&
+        (shared_gate || even(g.a, 1, g.s_a)) && (!GRAD || (even(g.p, 4, g.s_p) && even(g.q, 5, g.s_q))))
+        return shared_gate ? launch_side_by_side<T, V, kGateShared, GRAD>(g) : launch_side_by_side<T, V, kGateOwn, GRAD>(g);
+    const bool along = (g.s_o == ES || g.s_o == -ES) && g.n > 1;
+    if (along && !side && g.n > 32) return launch_rows<T, GRAD>(g);
+    return launch_side_by_side<T, 1, kGateOwn, GRAD>(g);
 }
 
 // common part of the two entry points: outer dimensions
