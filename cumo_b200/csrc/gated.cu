@@ -43,6 +43,7 @@ struct GatedRuns {
     const char* p;
     char* q;
     char* dinit;                     // may be null
+    int head;                        // lanes whose gate gradients are added up before they leave (0: none are)
 };
 
 template <typename T, int V> struct alignas(sizeof(T) * V) GVec { T v[V]; };
@@ -69,6 +70,16 @@ __device__ __forceinline__ double gfma(double a, double b, double c) { return fm
 // Gate modes of the packet kernels: the V runs of a lane have V neighbouring gates, or share one.
 enum GateMode { kGateOwn = 0, kGateShared = 1 };
 
+// The gradient of a gate that `head` neighbouring lanes of V runs share, in the first lane of each such group.
+template <typename T, int V>
+__device__ __forceinline__ T shared_sum(const GVec<T, V>& d, int head) {
+    T s = d.v[0];
+#pragma unroll
+    for (int v = 1; v < V; ++v) s += d.v[v];
+    for (int w = head >> 1; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+    return s;
+}
+
 // ---- walk: a thread per V neighbouring runs -----------------------------------------------------------------------------
 // Each thread keeps U steps of loads in flight; consecutive threads own consecutive runs, so that a step is one coalesced
 // access where the runs lie side by side.
@@ -77,10 +88,11 @@ __global__ void __launch_bounds__(kBlock)
 gated_walk_kernel(const GatedRuns g) {
     constexpr int U = V * sizeof(T) == 16 ? 4 : 8;
     constexpr int GV = GM == kGateShared ? 1 : V;
-    const int64_t groups = g.runs / V;
-    for (int64_t group = (int64_t)blockIdx.x * kBlock + threadIdx.x; group < groups; group += (int64_t)gridDim.x * kBlock) {
+    const int64_t groups = g.runs / V, padded = (groups + 31) / 32 * 32;          // whole warps: they add up heads together
+    for (int64_t group = (int64_t)blockIdx.x * kBlock + threadIdx.x; group < padded; group += (int64_t)gridDim.x * kBlock) {
+        const bool live = group < groups;
         int64_t off[7];
-        offsets_of<7>(group * V, g.nd, g.shape, g.step, off);
+        offsets_of<7>(live ? group * V : 0, g.nd, g.shape, g.step, off);
         const char* u = g.u + off[0];
         const char* a = g.a + off[1];
         char* o = g.o + off[2];
@@ -116,11 +128,18 @@ gated_walk_kernel(const GatedRuns g) {
                     out.v[v] = h[v];
                     if (GRAD) dg.v[v] = !last ? h[v] * pp[i].v[v] : g.init ? h[v] * init[v] : T(0);
                 }
-                gst<T, V>(o + s * g.s_o, out);
-                if (GRAD) gst<T, V>(q + s * g.s_q, dg);
+                if (live) gst<T, V>(o + s * g.s_o, out);
+                if (GRAD) {
+                    if (GM == kGateShared && g.head) {
+                        const T sum = shared_sum(dg, g.head);
+                        if (live && (threadIdx.x & (g.head - 1)) == 0) *reinterpret_cast<T*>(q + s * g.s_q) = sum;
+                    } else if (live) {
+                        gst<T, V>(q + s * g.s_q, dg);
+                    }
+                }
             }
         }
-        if (GRAD && g.dinit) {
+        if (GRAD && g.dinit && live) {
             const GVec<T, GV> a0 = gld<T, GV>(a + g.n * g.s_a);
 #pragma unroll
             for (int v = 0; v < V; ++v) *reinterpret_cast<T*>(g.dinit + off[6] + v * d_step) = a0.v[GM == kGateShared ? 0 : v] * h[v];
@@ -142,24 +161,24 @@ __device__ __forceinline__ double gates_times(double x, double y) {
 }
 
 // ---- strip: 32 lanes x V runs, time cut over warps and over the CTAs of a cluster ----------------------------------------
-constexpr int kStripSteps = 8;                       // steps of a warp per round
+// A round is kStripWarps x L steps of each CTA.  Every warp loads its L steps and folds them from a zero state; warp v then
+// folds the eight stretches of the lanes' run v, exchanges the CTA's pair with the cluster, and leaves each warp the state in
+// front of its stretch.  Two CTAs per SM keep loads in flight while one of them exchanges.
 constexpr int kStripWarps = 8;
 
-template <typename T, int V, int GM, bool GRAD>
+template <typename T, int V, int L, int GM, bool GRAD>
 __global__ void __launch_bounds__(kBlock, 2)
 gated_strip_kernel(const GatedRuns g, int cluster_size) {
     namespace cg = cooperative_groups;
-    constexpr int L = kStripSteps, W = kStripWarps;
+    constexpr int W = kStripWarps;
     constexpr int GV = GM == kGateShared ? 1 : V;
-    __shared__ double warp_A[2][W][GV][32];           // two rounds' worth: one barrier per round is enough
-    __shared__ double warp_B[2][W][V][32];
-    __shared__ double cta_A[2][GV][32];               // this CTA's stretch, read by the others of the cluster
-    __shared__ double cta_B[2][V][32];
+    __shared__ double warp_A[W][GV][32];
+    __shared__ double warp_B[W][V][32];               // a stretch's B; then the state in front of it
+    __shared__ double cta_A[2][V][32], cta_B[2][V][32];   // this CTA's pair, read by the others of the cluster; two rounds' worth
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = cluster_size > 1 ? (int)cluster.block_rank() : 0;
-    const int64_t strip = blockIdx.x / cluster_size;
-    const int64_t group = strip * 32 + lane;
+    const int64_t group = (int64_t)(blockIdx.x / cluster_size) * 32 + lane;
     const bool live = group < g.runs / V;
     int64_t off[7];
     offsets_of<7>(live ? group * V : 0, g.nd, g.shape, g.step, off);
@@ -170,115 +189,114 @@ gated_strip_kernel(const GatedRuns g, int cluster_size) {
     char* q = GRAD ? g.q + off[5] : nullptr;
     const int64_t i_step = g.nd > 0 ? g.step[3][g.nd - 1] : 0, d_step = g.nd > 0 ? g.step[6][g.nd - 1] : 0;
     const bool enters = !GRAD && g.init;
-    double H[V];                                      // state in front of this round, the same in every warp and CTA of the cluster
-#pragma unroll
-    for (int v = 0; v < V; ++v) H[v] = enters && live ? (double)*reinterpret_cast<const T*>(g.init + off[3] + v * i_step) : 0.0;
+    double H = 0.0;                                   // warp v < V: the state of run v in front of this round (the same in every CTA)
+    if (enters && warp < V) H = (double)*reinterpret_cast<const T*>(g.init + off[3] + warp * i_step);
     const int64_t per_round = (int64_t)cluster_size * W * L;
     const int64_t rounds = (g.n + per_round - 1) / per_round;
     for (int64_t round = 0; round < rounds; ++round) {
         const int64_t s0 = round * per_round + (int64_t)(rank * W + warp) * L;
-        const int buf = (int)(round & 1);
         GVec<T, V> uu[L], pp[L];
         GVec<T, GV> aa[L];
-        const int steps = !live || s0 >= g.n ? 0 : g.n - s0 < L ? (int)(g.n - s0) : L;
-#pragma unroll
-        for (int i = 0; i < L; ++i) {
-            if (i >= steps) break;
-            const int64_t s = s0 + i;
-            uu[i] = gld<T, V>(u + s * g.s_u);
-            if (s > 0 || enters) aa[i] = gld<T, GV>(a + s * g.s_a);
-        }
-        if (GRAD) {
+        const int steps = s0 >= g.n ? 0 : g.n - s0 < L ? (int)(g.n - s0) : L;
+        {
+            const char* ul = u + s0 * g.s_u;
+            const char* al = a + s0 * g.s_a;
+            const char* pl = GRAD ? p + s0 * g.s_p : nullptr;
 #pragma unroll
             for (int i = 0; i < L; ++i) {
                 if (i >= steps) break;
-                if (s0 + i + 1 < g.n) pp[i] = gld<T, V>(p + (s0 + i) * g.s_p);
+                uu[i] = gld<T, V>(ul + i * g.s_u);
+                if (s0 + i > 0 || enters) aa[i] = gld<T, GV>(al + i * g.s_a);
+                if (GRAD && s0 + i + 1 < g.n) pp[i] = gld<T, V>(pl + i * g.s_p);
             }
         }
         // this warp's stretch from a zero state; the very first step starts from nothing, whatever its gate is
-        double A[GV];
-        T B[V];
+        T A[GV], B[V];
 #pragma unroll
-        for (int x = 0; x < GV; ++x) A[x] = 1.0;
+        for (int x = 0; x < GV; ++x) A[x] = T(1);
 #pragma unroll
         for (int v = 0; v < V; ++v) B[v] = T(0);
+        const bool starts = s0 == 0 && !enters;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
             if (i >= steps) break;
-            if (s0 + i == 0 && !enters) {
-#pragma unroll
-                for (int x = 0; x < GV; ++x) A[x] = 0.0;
+            if (i == 0 && starts) {
 #pragma unroll
                 for (int v = 0; v < V; ++v) B[v] = uu[0].v[v];
                 continue;
             }
 #pragma unroll
-            for (int x = 0; x < GV; ++x) A[x] *= (double)aa[i].v[x];
+            for (int x = 0; x < GV; ++x) A[x] *= aa[i].v[x];
 #pragma unroll
             for (int v = 0; v < V; ++v) B[v] = i == 0 ? uu[i].v[v] : gfma(aa[i].v[GM == kGateShared ? 0 : v], B[v], uu[i].v[v]);
         }
 #pragma unroll
         for (int x = 0; x < GV; ++x) {
-            if (isinf(A[x]) || A[x] == 0.0) {                    // by overflow or underflow, or by a gate that is infinite or 0 itself?
-                A[x] = 1.0;
+            double wide = (double)A[x];
+            if (!(fabs(wide) > 1e-30 && fabs(wide) < 1e30)) {    // (near) the end of what the product of the gates can hold: once more in 64 bits
+                wide = 1.0;
 #pragma unroll
                 for (int i = 0; i < L; ++i)
-                    if (i < steps) A[x] = s0 + i > 0 || enters ? gates_times(A[x], (double)aa[i].v[x]) : 0.0;
+                    if (i < steps && !(i == 0 && starts)) wide = gates_times(wide, (double)aa[i].v[x]);
             }
-            warp_A[buf][warp][x][lane] = A[x];
+            warp_A[warp][x][lane] = starts ? 0.0 : wide;
         }
 #pragma unroll
-        for (int v = 0; v < V; ++v) warp_B[buf][warp][v][lane] = (double)B[v];
+        for (int v = 0; v < V; ++v) warp_B[warp][v][lane] = (double)B[v];
         __syncthreads();
-        double before[V];
+        const int buf = (int)(round & 1);
         if (cluster_size > 1) {
-            if (warp < V) {                                      // warp v folds the CTA's stretches of run v of each lane
-                const int v = warp;
-                double fa = warp_A[buf][0][GM == kGateShared ? 0 : v][lane], fb = warp_B[buf][0][v][lane];
+            if (warp < V) {
+                const int x = GM == kGateShared ? 0 : warp;
+                double fa = warp_A[0][x][lane], fb = warp_B[0][warp][lane];
 #pragma unroll
                 for (int w = 1; w < W; ++w) {
-                    const double wa = warp_A[buf][w][GM == kGateShared ? 0 : v][lane];
-                    fb = compose(wa, warp_B[buf][w][v][lane], fb);
+                    const double wa = warp_A[w][x][lane];
+                    fb = compose(wa, warp_B[w][warp][lane], fb);
                     fa = gates_times(fa, wa);
                 }
-                if (v < GV) cta_A[buf][v][lane] = fa;
-                cta_B[buf][v][lane] = fb;
+                cta_A[buf][warp][lane] = fa;
+                cta_B[buf][warp][lane] = fb;
             }
             cluster.sync();
-            for (int r = 0; r < cluster_size; ++r) {
-                const double* ra = cluster.map_shared_rank(&cta_A[buf][0][0], r);
-                const double* rb = cluster.map_shared_rank(&cta_B[buf][0][0], r);
+        }
+        if (warp < V) {
+            const int x = GM == kGateShared ? 0 : warp;
+            double before = H;
+            if (cluster_size > 1) {
+                double ra[8], rb[8];
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    if (r == rank) before[v] = H[v];
-                    H[v] = compose(ra[(GM == kGateShared ? 0 : v) * 32 + lane], rb[v * 32 + lane], H[v]);
+                for (int r = 0; r < 8; ++r)
+                    if (r < cluster_size) { ra[r] = *cluster.map_shared_rank(&cta_A[buf][warp][lane], r); rb[r] = *cluster.map_shared_rank(&cta_B[buf][warp][lane], r); }
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    if (r == rank) before = H;
+                    if (r < cluster_size) H = compose(ra[r], rb[r], H);
                 }
             }
-            for (int w = 0; w < warp; ++w)
 #pragma unroll
-                for (int v = 0; v < V; ++v) before[v] = compose(warp_A[buf][w][GM == kGateShared ? 0 : v][lane], warp_B[buf][w][v][lane], before[v]);
-        } else {
-#pragma unroll
-            for (int w = 0; w < W; ++w)
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    if (w == warp) before[v] = H[v];
-                    H[v] = compose(warp_A[buf][w][GM == kGateShared ? 0 : v][lane], warp_B[buf][w][v][lane], H[v]);
-                }
+            for (int w = 0; w < W; ++w) {
+                const double next = compose(warp_A[w][x][lane], warp_B[w][warp][lane], before);
+                warp_B[w][warp][lane] = before;
+                before = next;
+            }
+            if (cluster_size == 1) H = before;
         }
+        __syncthreads();
         T h[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = (T)before[v];
+        for (int v = 0; v < V; ++v) h[v] = (T)warp_B[warp][v][lane];
         // again, from the state in front
+        char* ol = o + s0 * g.s_o;
+        char* ql = GRAD ? q + s0 * g.s_q : nullptr;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
             if (i >= steps) break;
-            const int64_t s = s0 + i;
-            const bool last = s + 1 >= g.n;
+            const bool last = s0 + i + 1 >= g.n;
             GVec<T, V> out, dg;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                h[v] = s > 0 || enters ? gfma(aa[i].v[GM == kGateShared ? 0 : v], h[v], uu[i].v[v]) : uu[i].v[v];
+                h[v] = i == 0 && starts ? uu[i].v[v] : gfma(aa[i].v[GM == kGateShared ? 0 : v], h[v], uu[i].v[v]);
                 out.v[v] = h[v];
                 if (GRAD) {
                     T prior = T(0);
@@ -287,14 +305,22 @@ gated_strip_kernel(const GatedRuns g, int cluster_size) {
                     dg.v[v] = last && !g.init ? T(0) : h[v] * prior;
                 }
             }
-            gst<T, V>(o + s * g.s_o, out);
-            if (GRAD) gst<T, V>(q + s * g.s_q, dg);
-            if (GRAD && last && g.dinit) {
-                const GVec<T, GV> a0 = gld<T, GV>(a + g.n * g.s_a);
+            if (live) gst<T, V>(ol + i * g.s_o, out);
+            if (GRAD) {
+                if (GM == kGateShared && g.head) {
+                    const T sum = shared_sum(dg, g.head);
+                    if (live && (lane & (g.head - 1)) == 0) *reinterpret_cast<T*>(ql + i * g.s_q) = sum;
+                } else if (live) {
+                    gst<T, V>(ql + i * g.s_q, dg);
+                }
+                if (last && g.dinit && live) {
+                    const GVec<T, GV> a0 = gld<T, GV>(a + g.n * g.s_a);
 #pragma unroll
-                for (int v = 0; v < V; ++v) *reinterpret_cast<T*>(g.dinit + off[6] + v * d_step) = a0.v[GM == kGateShared ? 0 : v] * h[v];
+                    for (int v = 0; v < V; ++v) *reinterpret_cast<T*>(g.dinit + off[6] + v * d_step) = a0.v[GM == kGateShared ? 0 : v] * h[v];
+                }
             }
         }
+        __syncthreads();                                         // before the next round's pairs go where these states are
     }
     if (cluster_size > 1) cluster.sync();                        // nobody leaves while its pairs may still be read
 }
@@ -466,20 +492,52 @@ static int cluster_for(int64_t ctas, int64_t steps, int64_t steps_per_cta) {
     return c;
 }
 
-template <typename T, int V, int GM, bool GRAD>
-static int launch_side_by_side(const GatedRuns& g) {
+template <typename T, int V, int L, int GM, bool GRAD>
+static int launch_strip(const GatedRuns& g) {
+    const int64_t strips = (g.runs / V + 31) / 32;
+    const int cluster = cluster_for(strips, g.n, L * kStripWarps);
+    if (strips * cluster > 0x7fffffff) return (int)cudaErrorInvalidValue;
+    return launch_cluster(gated_strip_kernel<T, V, L, GM, GRAD>, g, (unsigned)(strips * cluster), cluster, 0);
+}
+
+// `packet`: runs per 16 bytes that may be taken together (1: element by element)
+template <typename T, int GM, bool GRAD>
+static int launch_side_by_side(GatedRuns& g, int packet, int64_t shared_runs) {
+    constexpr int V = 16 / sizeof(T);
+    // gates shared by a whole power-of-two number of lanes: their gradients are added up in the warp
+    auto heads = [&](int v) {
+        const int64_t lanes = shared_runs / v;
+        g.head = GRAD && shared_runs && shared_runs % v == 0 && lanes <= 32 && (lanes & (lanes - 1)) == 0 ? (int)lanes : 0;
+        return !shared_runs || g.head;
+    };
+    if constexpr (GM == kGateOwn) {
+        if (packet == 1) {
+            if (shared_runs) return (int)cudaErrorNotSupported;
+            if (g.runs >= (int64_t)sm_count() * 1024 || g.n <= 16) {
+                gated_walk_kernel<T, 1, GM, GRAD><<<grid_for((g.runs + kBlock - 1) / kBlock, 8), kBlock, 0, current_stream()>>>(g);
+                count_launch();
+                return (int)cudaGetLastError();
+            }
+            return launch_strip<T, 1, 16, GM, GRAD>(g);
+        }
+    }
     const int64_t groups = g.runs / V;
     // a thread per group when that alone keeps enough loads in flight (16 bytes x 4 steps x 2 operands each, about 44 KiB per
     // SM wanted), or when there is little to cut
-    if (groups >= (int64_t)sm_count() * 512 || g.n <= 2 * kStripSteps) {
+    if (groups >= (int64_t)sm_count() * 512 || g.n <= 16) {
+        if (!heads(V)) return (int)cudaErrorNotSupported;
         gated_walk_kernel<T, V, GM, GRAD><<<grid_for((groups + kBlock - 1) / kBlock, 8), kBlock, 0, current_stream()>>>(g);
         count_launch();
         return (int)cudaGetLastError();
     }
-    const int64_t strips = (groups + 31) / 32;
-    const int cluster = cluster_for(strips, g.n, kStripSteps * kStripWarps);
-    if (strips * cluster > 0x7fffffff) return (int)cudaErrorInvalidValue;
-    return launch_cluster(gated_strip_kernel<T, V, GM, GRAD>, g, (unsigned)(strips * cluster), cluster, 0);
+    // strips as wide as leaves two CTAs per SM with at most eight to a cluster; the gradients hold a third operand in registers
+    // and take half as many steps at a time
+    if (sizeof(T) == 8 || (groups + 31) / 32 * 8 >= (int64_t)sm_count() * 2) {
+        if (!heads(V)) return (int)cudaErrorNotSupported;
+        return launch_strip<T, V, GRAD ? 4 : 8, GM, GRAD>(g);
+    }
+    if (!heads(V / 2)) return (int)cudaErrorNotSupported;
+    return launch_strip<T, V / 2, GRAD ? 8 : 16, GM, GRAD>(g);
 }
 
 template <typename T, bool GRAD>
@@ -528,19 +586,22 @@ static int gated_launch(GatedRuns& g) {
     // there (the gate may also be one for all of them).
     constexpr int ES = sizeof(T), V = 16 / ES;
     const int in = nd - 1;
-    const bool side = nd > 0 && g.step[0][in] == ES && g.step[2][in] == ES && (!GRAD || (g.step[4][in] == ES && g.step[5][in] == ES));
     const bool shared_gate = nd > 0 && g.step[1][in] == 0;
+    const int64_t shared_runs = GRAD && shared_gate && g.step[5][in] == 0 ? g.shape[in] : 0;
+    for (int d = 0; GRAD && d < nd; ++d)
+        if (g.step[5][d] == 0 && g.shape[d] > 1 && (d < in || !shared_runs)) return (int)cudaErrorNotSupported;     // a sum over other dimensions
+    const bool side = nd > 0 && g.step[0][in] == ES && g.step[2][in] == ES && (!GRAD || (g.step[4][in] == ES && (g.step[5][in] == ES || shared_runs)));
     auto even = [&](const char* p, int k, int64_t s) {
         bool ok = aligned16(p) && mult16(s);
         for (int d = 0; d < in && ok; ++d) ok = mult16(g.step[k][d]);
         return ok;
     };
     if (side && (shared_gate || g.step[1][in] == ES) && g.shape[in] % V == 0 && even(g.u, 0, g.s_u) && even(g.o, 2, g.s_o) &&
-        (shared_gate || even(g.a, 1, g.s_a)) && (!GRAD || (even(g.p, 4, g.s_p) && even(g.q, 5, g.s_q))))
-        return shared_gate ? launch_side_by_side<T, V, kGateShared, GRAD>(g) : launch_side_by_side<T, V, kGateOwn, GRAD>(g);
+        (shared_gate || even(g.a, 1, g.s_a)) && (!GRAD || (even(g.p, 4, g.s_p) && (shared_runs || even(g.q, 5, g.s_q)))))
+        return shared_gate ? launch_side_by_side<T, kGateShared, GRAD>(g, V, shared_runs) : launch_side_by_side<T, kGateOwn, GRAD>(g, V, 0);
     const bool along = (g.s_o == ES || g.s_o == -ES) && g.n > 1;
-    if (along && !side && g.n > 32) return launch_rows<T, GRAD>(g);
-    return launch_side_by_side<T, 1, kGateOwn, GRAD>(g);
+    if (along && !side && g.n > 32) return shared_runs ? (int)cudaErrorNotSupported : launch_rows<T, GRAD>(g);
+    return launch_side_by_side<T, kGateOwn, GRAD>(g, 1, shared_runs);
 }
 
 // common part of the two entry points: outer dimensions

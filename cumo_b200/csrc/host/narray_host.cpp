@@ -1112,27 +1112,47 @@ int cb200_na_gated_cumsum_grad(cb200_na_t* grad, cb200_na_t* gate, cb200_na_t* h
     for (int d = 0; same && d < h->ndim; ++d) same = h->shape[d] == grad->shape[d];
     if (!same) { fail(h->dtype == grad->dtype ? "ShapeError" : "TypeError", "h must have the type and shape of grad"); return 1; }
     repeated_steps(h, grad->ndim, grad->shape, "h", hstep);
+    // A gate repeated along the last of the other dimensions alone: the kernels can add its gradients up themselves.
+    int64_t gshape[kMaxD];
+    int repeated = 0, last_other = -1;
+    for (int d = 0; d < grad->ndim; ++d) {
+        const bool rep = gstep[d] == 0 && grad->shape[d] != 1;
+        gshape[d] = rep ? 1 : grad->shape[d];
+        repeated += rep;
+        if (d != axis) last_other = d;
+    }
+    const bool fold = repeated == 1 && last_other >= 0 && gshape[last_other] != grad->shape[last_other];
     cb200_na* dx = make(grad->dtype, grad->ndim, grad->shape, false);
-    cb200_na* dgate = dx ? make(grad->dtype, grad->ndim, grad->shape, false) : nullptr;
+    cb200_na* dgate = dx ? make(grad->dtype, grad->ndim, fold ? gshape : grad->shape, size_of(grad) == 0) : nullptr;
     cb200_na* dinit = dgate && initial ? make(grad->dtype, grad->ndim - 1, state, size_of(grad) == 0) : nullptr;
     auto give_up = [&]() { cb200_na_release(dx); cb200_na_release(dgate); cb200_na_release(dinit); return 1; };
     if (!dx || !dgate || (initial && !dinit)) return give_up();
     if (size_of(grad) != 0) {
         size_t oshape[kMaxD];
         ssize_t o1[kMaxD], o2[kMaxD], o3[kMaxD], o4[kMaxD], o5[kMaxD], o6[kMaxD], o7[kMaxD];
-        int k = 0;
-        for (int d = 0; d < grad->ndim; ++d) {
-            if (d == axis) continue;
-            oshape[k] = (size_t)grad->shape[d];
-            o1[k] = (ssize_t)grad->step[d]; o2[k] = (ssize_t)gstep[d]; o3[k] = (ssize_t)h->step[d]; o5[k] = (ssize_t)dx->step[d]; o6[k] = (ssize_t)dgate->step[d];
-            o4[k] = initial ? (ssize_t)istep[k] : 0;
-            o7[k] = dinit ? (ssize_t)dinit->step[k] : 0;
-            ++k;
+        auto launch = [&]() {
+            int k = 0;
+            for (int d = 0; d < grad->ndim; ++d) {
+                if (d == axis) continue;
+                oshape[k] = (size_t)grad->shape[d];
+                o1[k] = (ssize_t)grad->step[d]; o2[k] = (ssize_t)gstep[d]; o3[k] = (ssize_t)h->step[d]; o5[k] = (ssize_t)dx->step[d];
+                o6[k] = dgate->shape[d] == grad->shape[d] ? (ssize_t)dgate->step[d] : 0;
+                o4[k] = initial ? (ssize_t)istep[k] : 0;
+                o7[k] = dinit ? (ssize_t)dinit->step[k] : 0;
+                ++k;
+            }
+            auto f = grad->dtype == CB200_SFLOAT ? cb200_sfloat_gated_cumsum_grad_runs_kernel_launch : cb200_dfloat_gated_cumsum_grad_runs_kernel_launch;
+            return f(data_ptr(grad), data_ptr(gate), data_ptr(h), initial ? data_ptr(initial) : nullptr, data_ptr(dx), data_ptr(dgate),
+                     dinit ? data_ptr(dinit) : nullptr, (ssize_t)grad->step[axis], (ssize_t)gstep[axis], (ssize_t)h->step[axis], (ssize_t)dx->step[axis],
+                     (ssize_t)dgate->step[axis], (uint64_t)grad->shape[axis], k, oshape, o1, o2, o3, o4, o5, o6, o7);
+        };
+        int status = launch();
+        if (status == (int)cudaErrorNotSupported && fold) {       // not that many of them: every product, summed below
+            cb200_na_release(dgate);
+            dgate = make(grad->dtype, grad->ndim, grad->shape, false);
+            if (!dgate) return give_up();
+            status = launch();
         }
-        auto f = grad->dtype == CB200_SFLOAT ? cb200_sfloat_gated_cumsum_grad_runs_kernel_launch : cb200_dfloat_gated_cumsum_grad_runs_kernel_launch;
-        const int status = f(data_ptr(grad), data_ptr(gate), data_ptr(h), initial ? data_ptr(initial) : nullptr, data_ptr(dx), data_ptr(dgate),
-                             dinit ? data_ptr(dinit) : nullptr, (ssize_t)grad->step[axis], (ssize_t)gstep[axis], (ssize_t)h->step[axis], (ssize_t)dx->step[axis],
-                             (ssize_t)dgate->step[axis], (uint64_t)grad->shape[axis], k, oshape, o1, o2, o3, o4, o5, o6, o7);
         if (status) { fail("CudaError", "gated_cumsum_grad: %s", cudaGetErrorString((cudaError_t)status)); return give_up(); }
         if (!launch_ok()) return give_up();
     }

@@ -603,7 +603,10 @@ int cb200_sfloat_sum_noalloc_kernel_launch(cumo_na_reduction_arg_t* arg, char* e
  * other dimensions (host arrays; a step of 0 repeats).  `initial` (may be NULL) is h[-1] per run; without it h[0] = x[0] and
  * gate[0] is not read.  The second function writes the gradients for grad = dL/dh, given the h of the first:
  * dx[t] = grad[t] + gate[t+1] * dx[t+1], dgate[t] = dx[t] * h[t-1] (0 at t = 0 without an initial state) and, where
- * dinitial is not NULL, gate[0] * dx[0].  Outputs may not overlap inputs and their steps may not be 0.  Both return a cudaError_t. */
+ * dinitial is not NULL, gate[0] * dx[0].  Outputs may not overlap inputs and their steps may not be 0, except that dgate's step
+ * along the last outer dimension may be, where gate's is: dgate then receives the sum over that dimension, or the call returns
+ * cudaErrorNotSupported with nothing launched (the kernels do it for power-of-two extents that a warp covers).  Both return a
+ * cudaError_t. */
 #define CB200_DECL_GATED(T) \
     int cb200_##T##_gated_cumsum_runs_kernel_launch(char* x, char* gate, char* initial, char* h, ssize_t s_x, ssize_t s_gate, ssize_t s_h, uint64_t n, int n_outer, \
         const size_t* shape, const ssize_t* x_step, const ssize_t* gate_step, const ssize_t* initial_step, const ssize_t* h_step); \
