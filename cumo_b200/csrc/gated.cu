@@ -155,16 +155,29 @@ __device__ __forceinline__ double compose(double A, double B, double h) { return
 // past growing gates, or an infinity past shrinking ones, so does the pair.
 __device__ __forceinline__ double gates_times(double x, double y) {
     double r = x * y;
-    if (isinf(r) && !isinf(x) && !isinf(y)) r = copysign(1.7976931348623157e308, r);
-    if (r == 0.0 && x != 0.0 && y != 0.0) r = copysign(4.9406564584124654e-324, r);
+    const int e = __double2hiint(r) & 0x7ff00000;                // 0 or subnormal; infinite or NaN: look closer
+    if (e == 0 || e == 0x7ff00000) {
+        if (isinf(r) && !isinf(x) && !isinf(y)) r = copysign(1.7976931348623157e308, r);
+        if (r == 0.0 && x != 0.0 && y != 0.0) r = copysign(4.9406564584124654e-324, r);
+    }
     return r;
 }
 
 // ---- strip: 32 lanes x V runs, time cut over warps and over the CTAs of a cluster ----------------------------------------
 // A round is kStripWarps x L steps of each CTA.  Every warp loads its L steps and folds them from a zero state; warp v then
 // folds the eight stretches of the lanes' run v, exchanges the CTA's pair with the cluster, and leaves each warp the state in
-// front of its stretch.  Two CTAs per SM keep loads in flight while one of them exchanges.
+// front of its stretch.  Each thread's next steps are on their way (asynchronous copies into slots of shared memory that only it
+// reads) while all this happens, and two CTAs per SM cover each other's exchanges.
 constexpr int kStripWarps = 8;
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const char* src) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+
+template <typename T, int V, int L, int GM, bool GRAD>
+constexpr size_t strip_bytes() { return (size_t)kBlock * L * ((GRAD ? 2 : 1) * V + (GM == kGateShared ? 1 : V)) * sizeof(T); }
 
 template <typename T, int V, int L, int GM, bool GRAD>
 __global__ void __launch_bounds__(kBlock, 2)
@@ -193,22 +206,38 @@ gated_strip_kernel(const GatedRuns g, int cluster_size) {
     if (enters && warp < V) H = (double)*reinterpret_cast<const T*>(g.init + off[3] + warp * i_step);
     const int64_t per_round = (int64_t)cluster_size * W * L;
     const int64_t rounds = (g.n + per_round - 1) / per_round;
+    // slots [step][thread] of u, then p, then the gate
+    extern __shared__ __align__(16) char slots[];
+    const GVec<T, V>* mine_u = reinterpret_cast<const GVec<T, V>*>(slots) + threadIdx.x;
+    const GVec<T, V>* mine_p = mine_u + L * kBlock;
+    const GVec<T, GV>* mine_a = reinterpret_cast<const GVec<T, GV>*>(slots + (size_t)kBlock * L * (GRAD ? 2 : 1) * sizeof(GVec<T, V>)) + threadIdx.x;
+    const uint32_t at_u = (uint32_t)__cvta_generic_to_shared(mine_u), at_p = (uint32_t)__cvta_generic_to_shared(mine_p), at_a = (uint32_t)__cvta_generic_to_shared(mine_a);
+    auto fetch = [&](int64_t s0) {
+        const int steps = s0 >= g.n ? 0 : g.n - s0 < L ? (int)(g.n - s0) : L;
+        const char* ul = u + s0 * g.s_u;
+        const char* al = a + s0 * g.s_a;
+        const char* pl = GRAD ? p + s0 * g.s_p : nullptr;
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            if (i >= steps) break;
+            copy_async<sizeof(T) * V>(at_u + i * kBlock * sizeof(GVec<T, V>), ul + i * g.s_u);
+            if (s0 + i > 0 || enters) copy_async<sizeof(T) * GV>(at_a + i * kBlock * sizeof(GVec<T, GV>), al + i * g.s_a);
+            if (GRAD && s0 + i + 1 < g.n) copy_async<sizeof(T) * V>(at_p + i * kBlock * sizeof(GVec<T, V>), pl + i * g.s_p);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    fetch((int64_t)(rank * W + warp) * L);
     for (int64_t round = 0; round < rounds; ++round) {
         const int64_t s0 = round * per_round + (int64_t)(rank * W + warp) * L;
         GVec<T, V> uu[L], pp[L];
         GVec<T, GV> aa[L];
         const int steps = s0 >= g.n ? 0 : g.n - s0 < L ? (int)(g.n - s0) : L;
-        {
-            const char* ul = u + s0 * g.s_u;
-            const char* al = a + s0 * g.s_a;
-            const char* pl = GRAD ? p + s0 * g.s_p : nullptr;
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
-            for (int i = 0; i < L; ++i) {
-                if (i >= steps) break;
-                uu[i] = gld<T, V>(ul + i * g.s_u);
-                if (s0 + i > 0 || enters) aa[i] = gld<T, GV>(al + i * g.s_a);
-                if (GRAD && s0 + i + 1 < g.n) pp[i] = gld<T, V>(pl + i * g.s_p);
-            }
+        for (int i = 0; i < L; ++i) {
+            uu[i] = mine_u[i * kBlock];
+            aa[i] = mine_a[i * kBlock];
+            if (GRAD) pp[i] = mine_p[i * kBlock];
         }
         // this warp's stretch from a zero state; the very first step starts from nothing, whatever its gate is
         T A[GV], B[V];
@@ -243,7 +272,8 @@ gated_strip_kernel(const GatedRuns g, int cluster_size) {
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) warp_B[warp][v][lane] = (double)B[v];
-        __syncthreads();
+        __syncthreads();                                         // (the slots have been read)
+        if (round + 1 < rounds) fetch(s0 + per_round);
         const int buf = (int)(round & 1);
         if (cluster_size > 1) {
             if (warp < V) {
@@ -329,16 +359,16 @@ gated_strip_kernel(const GatedRuns g, int cluster_size) {
 // G threads per run (a warp, or the CTA, or the CTAs of a cluster in turns), kRowItems consecutive steps per thread.  A tile
 // is copied into shared memory along the axis, padded so that threads reading their own steps hit different banks, and the
 // results go back the same way.
-constexpr int kRowItems = 8;
+constexpr int kRowItems = 8;                         // (4 where a warp's run has at most 128 steps)
 
-template <typename T>
-__device__ __forceinline__ int row_slot(int i) { return i + i / kRowItems; }       // one element of padding per thread
+template <int I>
+__device__ __forceinline__ int row_slot(int i) { return i + i / I; }       // one element of padding per thread
 
-template <typename T, int G, bool GRAD>
-__global__ void __launch_bounds__(kBlock)
+template <typename T, int G, int I, bool GRAD>
+__global__ void __launch_bounds__(kBlock, 2)
 gated_rows_kernel(const GatedRuns g, int cluster_size) {
     namespace cg = cooperative_groups;
-    constexpr int I = kRowItems, TILE = G * I, SLOTS = TILE + G, PER_CTA = kBlock / G;
+    constexpr int TILE = G * I, SLOTS = TILE + G, PER_CTA = kBlock / G;
     extern __shared__ __align__(16) char smem[];
     __shared__ double warp_A[kWarpsPerBlock], warp_B[kWarpsPerBlock];
     __shared__ double cta_A[2], cta_B[2];
@@ -351,39 +381,48 @@ gated_rows_kernel(const GatedRuns g, int cluster_size) {
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = cluster_size > 1 ? (int)cluster.block_rank() : 0;
     const int64_t first = (int64_t)(blockIdx.x / cluster_size) * PER_CTA, stride = (int64_t)(gridDim.x / cluster_size) * PER_CTA;
+    const bool enters = !GRAD && g.init;
+    const int64_t per_round = (int64_t)cluster_size * TILE, rounds = (g.n + per_round - 1) / per_round;
     auto sync = [&]() { if (G > 32) __syncthreads(); else __syncwarp(); };
+    T lu[I], la[I], lp[I];
+    // the tile of a run and round, into registers: requested while the tile before it is worked on
+    auto fetch = [&](int64_t run, int64_t round) {
+        int64_t off[7];
+        offsets_of<7>(run, g.nd, g.shape, g.step, off);
+        const int64_t s0 = round * per_round + (int64_t)rank * TILE;
+        const int count = s0 >= g.n ? 0 : g.n - s0 < TILE ? (int)(g.n - s0) : TILE;
+        const char* u = g.u + off[0] + (s0 + me) * g.s_u;
+        const char* a = g.a + off[1] + (s0 + me) * g.s_a;
+        const char* p = GRAD ? g.p + off[4] + (s0 + me) * g.s_p : nullptr;
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            const int e = i * G + me;
+            lu[i] = e < count ? ld_one<T>(u + i * G * g.s_u) : T(0);
+            la[i] = e < count && (s0 + e > 0 || enters) ? ld_one<T>(a + i * G * g.s_a) : T(1);
+            if (GRAD) lp[i] = e < count && s0 + e + 1 < g.n ? ld_one<T>(p + i * G * g.s_p) : T(0);
+        }
+    };
+    if (first + slot < g.runs) fetch(first + slot, 0);
     for (int64_t base = first; base < g.runs; base += stride) {
         const int64_t run = base + slot;
         if (G <= 32 && run >= g.runs) break;                     // (a whole warp leaves; the CTA form has one run per CTA)
         int64_t off[7];
         offsets_of<7>(run, g.nd, g.shape, g.step, off);
-        const char* u = g.u + off[0];
-        const char* a = g.a + off[1];
         char* o = g.o + off[2];
-        const char* p = GRAD ? g.p + off[4] : nullptr;
         char* q = GRAD ? g.q + off[5] : nullptr;
         const T init = g.init ? *reinterpret_cast<const T*>(g.init + off[3]) : T(0);
-        const bool enters = !GRAD && g.init;
         double H = enters ? (double)init : 0.0;
-        const int64_t per_round = (int64_t)cluster_size * TILE, rounds = (g.n + per_round - 1) / per_round;
         for (int64_t round = 0; round < rounds; ++round) {
             const int64_t s0 = round * per_round + (int64_t)rank * TILE;
             const int count = s0 >= g.n ? 0 : g.n - s0 < TILE ? (int)(g.n - s0) : TILE;
-            T lu[I], la[I], lp[I];
 #pragma unroll
             for (int i = 0; i < I; ++i) {
-                const int e = i * G + me;
-                const int64_t s = s0 + e;
-                lu[i] = e < count ? ld_one<T>(u + s * g.s_u) : T(0);
-                la[i] = e < count && (s > 0 || enters) ? ld_one<T>(a + s * g.s_a) : T(1);
-                if (GRAD) lp[i] = e >= count ? T(0) : s + 1 < g.n ? ld_one<T>(p + s * g.s_p) : init;
-            }
-#pragma unroll
-            for (int i = 0; i < I; ++i) {
-                const int e = row_slot<T>(i * G + me);
+                const int e = row_slot<I>(i * G + me);
                 su[e] = lu[i]; sa[e] = la[i];
-                if (GRAD) sp[e] = lp[i];
+                if (GRAD) sp[e] = s0 + i * G + me + 1 == g.n ? init : lp[i];
             }
+            if (round + 1 < rounds) fetch(run, round + 1);
+            else if (run + stride < g.runs) fetch(run + stride, 0);
             sync();
             // this thread's steps from a zero state
             T x[I], c[I];
@@ -447,7 +486,7 @@ gated_rows_kernel(const GatedRuns g, int cluster_size) {
                     const int64_t s = s0 + me * I + i;
                     const bool last = s + 1 == g.n;
                     sa[mine + i] = last && !g.init ? T(0) : h * sp[mine + i];
-                    if (last && g.dinit) *reinterpret_cast<T*>(g.dinit + off[6]) = *reinterpret_cast<const T*>(a + g.n * g.s_a) * h;
+                    if (last && g.dinit) *reinterpret_cast<T*>(g.dinit + off[6]) = *reinterpret_cast<const T*>(g.a + off[1] + g.n * g.s_a) * h;
                 }
                 su[mine + i] = h;
             }
@@ -456,8 +495,8 @@ gated_rows_kernel(const GatedRuns g, int cluster_size) {
             for (int i = 0; i < I; ++i) {
                 const int e = i * G + me;
                 if (e < count) {
-                    st_one<T>(o + (s0 + e) * g.s_o, su[row_slot<T>(e)]);
-                    if (GRAD) st_one<T>(q + (s0 + e) * g.s_q, sa[row_slot<T>(e)]);
+                    st_one<T>(o + (s0 + e) * g.s_o, su[row_slot<I>(e)]);
+                    if (GRAD) st_one<T>(q + (s0 + e) * g.s_q, sa[row_slot<I>(e)]);
                 }
             }
             sync();
@@ -497,7 +536,13 @@ static int launch_strip(const GatedRuns& g) {
     const int64_t strips = (g.runs / V + 31) / 32;
     const int cluster = cluster_for(strips, g.n, L * kStripWarps);
     if (strips * cluster > 0x7fffffff) return (int)cudaErrorInvalidValue;
-    return launch_cluster(gated_strip_kernel<T, V, L, GM, GRAD>, g, (unsigned)(strips * cluster), cluster, 0);
+    constexpr size_t smem = strip_bytes<T, V, L, GM, GRAD>();
+    auto kernel = gated_strip_kernel<T, V, L, GM, GRAD>;
+    if (smem > 24 * 1024) {
+        const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (rc != cudaSuccess) { cudaGetLastError(); return (int)rc; }
+    }
+    return launch_cluster(kernel, g, (unsigned)(strips * cluster), cluster, smem);
 }
 
 // `packet`: runs per 16 bytes that may be taken together (1: element by element)
@@ -540,27 +585,26 @@ static int launch_side_by_side(GatedRuns& g, int packet, int64_t shared_runs) {
     return launch_strip<T, V / 2, GRAD ? 8 : 16, GM, GRAD>(g);
 }
 
+template <typename T, int G, int I, bool GRAD>
+static int launch_rows_of(const GatedRuns& g, int64_t rows, int cluster) {
+    constexpr size_t smem = (size_t)(GRAD ? 3 : 2) * (kBlock * I + kBlock) * sizeof(T);
+    auto kernel = gated_rows_kernel<T, G, I, GRAD>;
+    if (smem > 48 * 1024 - 512) {
+        const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (rc != cudaSuccess) { cudaGetLastError(); return (int)rc; }
+    }
+    return launch_cluster(kernel, g, (unsigned)(rows * cluster), cluster, smem);
+}
+
 template <typename T, bool GRAD>
 static int launch_rows(const GatedRuns& g) {
-    const int64_t tile = (int64_t)kBlock * kRowItems;
-    constexpr int arrays = GRAD ? 3 : 2;
-    constexpr size_t smem = (size_t)arrays * (kBlock * kRowItems + kBlock) * sizeof(T);
-    if (g.n <= 32 * kRowItems * 2 || g.runs >= (int64_t)sm_count() * 32) {
-        const unsigned grid = grid_for((g.runs + kWarpsPerBlock - 1) / kWarpsPerBlock, 6);
-        if (smem > 48 * 1024) {
-            const cudaError_t rc = cudaFuncSetAttribute(gated_rows_kernel<T, 32, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-            if (rc != cudaSuccess) return (int)rc;
-        }
-        return launch_cluster(gated_rows_kernel<T, 32, GRAD>, g, grid, 1, smem);
-    }
-    if (smem > 48 * 1024) {
-        const cudaError_t rc = cudaFuncSetAttribute(gated_rows_kernel<T, kBlock, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (rc != cudaSuccess) return (int)rc;
-    }
-    const int64_t most = (int64_t)sm_count() * 6;
-    const int cluster = cluster_for(g.runs, g.n, tile);
-    const int64_t rows = g.runs < most ? g.runs : most;
-    return launch_cluster(gated_rows_kernel<T, kBlock, GRAD>, g, (unsigned)(rows * cluster), cluster, smem);
+    // a warp per run where there are enough of them or a warp's tile holds most of one
+    const unsigned warps = grid_for((g.runs + kWarpsPerBlock - 1) / kWarpsPerBlock, 2);
+    if (g.n <= 128) return launch_rows_of<T, 32, 4, GRAD>(g, warps, 1);
+    if (g.n <= 32 * kRowItems * 2 || g.runs >= (int64_t)sm_count() * 32) return launch_rows_of<T, 32, kRowItems, GRAD>(g, warps, 1);
+    const int cluster = cluster_for(g.runs, g.n, (int64_t)kBlock * kRowItems);
+    const int64_t most = (int64_t)sm_count() * 2;
+    return launch_rows_of<T, kBlock, kRowItems, GRAD>(g, g.runs < most ? g.runs : most, cluster);
 }
 
 template <typename T, bool GRAD>
