@@ -23,7 +23,8 @@
 //           shared memory so that global accesses run along the axis while a thread owns consecutive steps
 #include <cooperative_groups.h>
 
-#include "linear.cuh"
+#include "split_product.cuh"
+#include "tc_common.cuh"
 
 namespace cb200 {
 
@@ -43,6 +44,7 @@ struct GatedRuns {
     const char* p;
     char* q;
     char* dinit;                     // may be null
+    int* gave_up;                    // set when a bounded wait ran out
     int head;                        // lanes whose gate gradients are added up before they leave (0: none are)
 };
 
@@ -165,8 +167,9 @@ __device__ __forceinline__ double gates_times(double x, double y) {
 
 // ---- strip: 32 lanes x V runs, time cut over warps and over the CTAs of a cluster ----------------------------------------
 // A round is kStripWarps x L steps of each CTA.  Every warp loads its L steps and folds them from a zero state; warp v then
-// folds the eight stretches of the lanes' run v, exchanges the CTA's pair with the cluster, and leaves each warp the state in
-// front of its stretch.  Each thread's next steps are on their way (asynchronous copies into slots of shared memory that only it
+// folds the eight stretches of the lanes' run v, stores the CTA's pair into every CTA of the cluster (asynchronous stores that
+// count themselves in at the receiver's mbarrier: a cluster barrier would also wait for the outputs' way to memory), and leaves
+// each warp the state in front of its stretch.  The wait for the pairs is bounded.  Each thread's next steps are on their way (asynchronous copies into slots of shared memory that only it
 // reads) while all this happens, and two CTAs per SM cover each other's exchanges.
 constexpr int kStripWarps = 8;
 
@@ -187,7 +190,10 @@ gated_strip_kernel(const GatedRuns g, int cluster_size) {
     constexpr int GV = GM == kGateShared ? 1 : V;
     __shared__ double warp_A[W][GV][32];
     __shared__ double warp_B[W][V][32];               // a stretch's B; then the state in front of it
-    __shared__ double cta_A[2][V][32], cta_B[2][V][32];   // this CTA's pair, read by the others of the cluster; two rounds' worth
+    extern __shared__ __align__(16) char slots[];
+    using Pairs = double2[8][V][32];                  // (A, B) of every CTA of the cluster, two rounds' worth, behind the slots
+    Pairs* pairs = reinterpret_cast<Pairs*>(slots + strip_bytes<T, V, L, GM, GRAD>());
+    __shared__ __align__(8) uint64_t arrived[2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = cluster_size > 1 ? (int)cluster.block_rank() : 0;
@@ -202,12 +208,12 @@ gated_strip_kernel(const GatedRuns g, int cluster_size) {
     char* q = GRAD ? g.q + off[5] : nullptr;
     const int64_t i_step = g.nd > 0 ? g.step[3][g.nd - 1] : 0, d_step = g.nd > 0 ? g.step[6][g.nd - 1] : 0;
     const bool enters = !GRAD && g.init;
+    bool gave_up = false;
     double H = 0.0;                                   // warp v < V: the state of run v in front of this round (the same in every CTA)
     if (enters && warp < V) H = (double)*reinterpret_cast<const T*>(g.init + off[3] + warp * i_step);
     const int64_t per_round = (int64_t)cluster_size * W * L;
     const int64_t rounds = (g.n + per_round - 1) / per_round;
     // slots [step][thread] of u, then p, then the gate
-    extern __shared__ __align__(16) char slots[];
     const GVec<T, V>* mine_u = reinterpret_cast<const GVec<T, V>*>(slots) + threadIdx.x;
     const GVec<T, V>* mine_p = mine_u + L * kBlock;
     const GVec<T, GV>* mine_a = reinterpret_cast<const GVec<T, GV>*>(slots + (size_t)kBlock * L * (GRAD ? 2 : 1) * sizeof(GVec<T, V>)) + threadIdx.x;
@@ -227,6 +233,14 @@ gated_strip_kernel(const GatedRuns g, int cluster_size) {
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     fetch((int64_t)(rank * W + warp) * L);
+    if (cluster_size > 1) {
+        if (threadIdx.x == 0) {
+            mbar_init(&arrived[0], V);
+            mbar_init(&arrived[1], V);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        cluster.sync();
+    }
     for (int64_t round = 0; round < rounds; ++round) {
         const int64_t s0 = round * per_round + (int64_t)(rank * W + warp) * L;
         GVec<T, V> uu[L], pp[L];
@@ -275,40 +289,46 @@ gated_strip_kernel(const GatedRuns g, int cluster_size) {
         __syncthreads();                                         // (the slots have been read)
         if (round + 1 < rounds) fetch(s0 + per_round);
         const int buf = (int)(round & 1);
-        if (cluster_size > 1) {
-            if (warp < V) {
-                const int x = GM == kGateShared ? 0 : warp;
-                double fa = warp_A[0][x][lane], fb = warp_B[0][warp][lane];
-#pragma unroll
-                for (int w = 1; w < W; ++w) {
-                    const double wa = warp_A[w][x][lane];
-                    fb = compose(wa, warp_B[w][warp][lane], fb);
-                    fa = gates_times(fa, wa);
-                }
-                cta_A[buf][warp][lane] = fa;
-                cta_B[buf][warp][lane] = fb;
-            }
-            cluster.sync();
-        }
         if (warp < V) {
             const int x = GM == kGateShared ? 0 : warp;
-            double before = H;
-            if (cluster_size > 1) {
-                double ra[8], rb[8];
+            double wa[W], wb[W], before = H;
 #pragma unroll
-                for (int r = 0; r < 8; ++r)
-                    if (r < cluster_size) { ra[r] = *cluster.map_shared_rank(&cta_A[buf][warp][lane], r); rb[r] = *cluster.map_shared_rank(&cta_B[buf][warp][lane], r); }
+            for (int w = 0; w < W; ++w) { wa[w] = warp_A[w][x][lane]; wb[w] = warp_B[w][warp][lane]; }
+            if (cluster_size > 1) {
+                double fa = wa[0], fb = wb[0];
+#pragma unroll
+                for (int w = 1; w < W; ++w) { fb = compose(wa[w], wb[w], fb); fa = gates_times(fa, wa[w]); }
+                const uint32_t to = smem_u32(&pairs[buf][rank][warp][lane]), bar = smem_u32(&arrived[buf]);
+                if (lane == 0)
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((uint32_t)(cluster_size * 32 * sizeof(double2))) : "memory");
+                for (int r = 0; r < cluster_size; ++r) {
+                    uint32_t there, bar_there;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(to), "r"(r));
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar_there) : "r"(bar), "r"(r));
+                    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];"
+                                 ::"r"(there), "l"(__double_as_longlong(fa)), "l"(__double_as_longlong(fb)), "r"(bar_there) : "memory");
+                }
+                const uint32_t parity = (uint32_t)(round >> 1) & 1u;
+                bool came = false;
+                for (uint32_t spin = 0; spin < kSpinLimit && !came && !gave_up; ++spin) {
+                    uint32_t done;
+                    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+                    came = done;
+                    if (!came && spin > 64) __nanosleep(32);
+                }
+                if (!came) gave_up = true;                       // (never seen: a cluster's CTAs run together)
+                __syncwarp();
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
                     if (r == rank) before = H;
-                    if (r < cluster_size) H = compose(ra[r], rb[r], H);
+                    if (r < cluster_size) { const double2 ab = pairs[buf][r][warp][lane]; H = compose(ab.x, ab.y, H); }
                 }
             }
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                const double next = compose(warp_A[w][x][lane], warp_B[w][warp][lane], before);
                 warp_B[w][warp][lane] = before;
-                before = next;
+                before = compose(wa[w], wb[w], before);
             }
             if (cluster_size == 1) H = before;
         }
@@ -352,7 +372,8 @@ gated_strip_kernel(const GatedRuns g, int cluster_size) {
         }
         __syncthreads();                                         // before the next round's pairs go where these states are
     }
-    if (cluster_size > 1) cluster.sync();                        // nobody leaves while its pairs may still be read
+    if (gave_up) *reinterpret_cast<volatile int*>(g.gave_up) = 1;
+    if (cluster_size > 1) cluster.sync();                        // nobody leaves while a pair may still be on its way
 }
 
 // ---- rows: runs contiguous along the axis -----------------------------------------------------------------------------------
@@ -532,11 +553,16 @@ static int cluster_for(int64_t ctas, int64_t steps, int64_t steps_per_cta) {
 }
 
 template <typename T, int V, int L, int GM, bool GRAD>
-static int launch_strip(const GatedRuns& g) {
+static int launch_strip(GatedRuns& g) {
     const int64_t strips = (g.runs / V + 31) / 32;
     const int cluster = cluster_for(strips, g.n, L * kStripWarps);
     if (strips * cluster > 0x7fffffff) return (int)cudaErrorInvalidValue;
-    constexpr size_t smem = strip_bytes<T, V, L, GM, GRAD>();
+    if (cluster > 1) {
+        const int late = product_gave_up();
+        if (late) return late;
+        if (!gave_up_word(&g.gave_up)) return (int)cudaErrorMemoryAllocation;
+    }
+    constexpr size_t smem = strip_bytes<T, V, L, GM, GRAD>() + 2 * 8 * V * 32 * sizeof(double2);
     auto kernel = gated_strip_kernel<T, V, L, GM, GRAD>;
     if (smem > 24 * 1024) {
         const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);

@@ -451,22 +451,29 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
 // One word of mapped host memory per process that a kernel sets when a bounded wait ran out; read without synchronising.
-static int* gave_up_word(int** dev) {
+int* gave_up_word(int** dev) {
     static std::mutex mu;
     static int* host = nullptr;
+    static int* on_device[64] = {};
+    int d = 0;
+    if (dev && cudaGetDevice(&d) != cudaSuccess) return nullptr;
+    if (d < 0 || d >= 64) return nullptr;
     std::lock_guard<std::mutex> lock(mu);
-    if (!host) {
+    if (host && !dev) return host;
+    if (!host || !on_device[d]) {
         cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;       // the first call may come during a capture
         cudaThreadExchangeStreamCaptureMode(&mode);
-        void* p = nullptr;
-        const cudaError_t rc = cudaHostAlloc(&p, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+        void* p = host;
+        cudaError_t rc = cudaSuccess;
+        if (!host) rc = cudaHostAlloc(&p, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+        if (rc == cudaSuccess && !host) { host = static_cast<int*>(p); *host = 0; }
+        void* q = nullptr;
+        if (rc == cudaSuccess && dev) rc = cudaHostGetDevicePointer(&q, host, 0);
         cudaThreadExchangeStreamCaptureMode(&mode);
         if (rc != cudaSuccess) { cudaGetLastError(); return nullptr; }
-        host = static_cast<int*>(p);
-        *host = 0;
+        if (dev) on_device[d] = static_cast<int*>(q);
     }
-    void* d = nullptr;
-    if (dev) { if (cudaHostGetDevicePointer(&d, host, 0) != cudaSuccess) { cudaGetLastError(); return nullptr; } *dev = static_cast<int*>(d); }
+    if (dev) *dev = on_device[d];
     return host;
 }
 

@@ -67,5 +67,7 @@ int launch_fix_marked(int64_t m, int64_t n, int64_t k, const SplitSource& a, boo
 
 // 0, or cudaErrorLaunchTimeout once a bounded wait inside a product has run out on this device (see cb200_product_status).
 int product_gave_up();
+// The word behind it, and its address on the current device; null when it cannot be had.
+int* gave_up_word(int** dev);
 
 }  // namespace cb200
