@@ -218,17 +218,28 @@ gated_strip_kernel(const GatedRuns g, int cluster_size) {
     const GVec<T, V>* mine_p = mine_u + L * kBlock;
     const GVec<T, GV>* mine_a = reinterpret_cast<const GVec<T, GV>*>(slots + (size_t)kBlock * L * (GRAD ? 2 : 1) * sizeof(GVec<T, V>)) + threadIdx.x;
     const uint32_t at_u = (uint32_t)__cvta_generic_to_shared(mine_u), at_p = (uint32_t)__cvta_generic_to_shared(mine_p), at_a = (uint32_t)__cvta_generic_to_shared(mine_a);
+    // Stretches inside the run take the short form of each loop: no step of theirs is the first, the last or missing.
+    auto inside = [&](int64_t s0) { return (s0 > 0 || enters) && s0 + L < g.n; };
     auto fetch = [&](int64_t s0) {
-        const int steps = s0 >= g.n ? 0 : g.n - s0 < L ? (int)(g.n - s0) : L;
         const char* ul = u + s0 * g.s_u;
         const char* al = a + s0 * g.s_a;
         const char* pl = GRAD ? p + s0 * g.s_p : nullptr;
+        if (inside(s0)) {
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-            if (i >= steps) break;
-            copy_async<sizeof(T) * V>(at_u + i * kBlock * sizeof(GVec<T, V>), ul + i * g.s_u);
-            if (s0 + i > 0 || enters) copy_async<sizeof(T) * GV>(at_a + i * kBlock * sizeof(GVec<T, GV>), al + i * g.s_a);
-            if (GRAD && s0 + i + 1 < g.n) copy_async<sizeof(T) * V>(at_p + i * kBlock * sizeof(GVec<T, V>), pl + i * g.s_p);
+            for (int i = 0; i < L; ++i) {
+                copy_async<sizeof(T) * V>(at_u + i * kBlock * sizeof(GVec<T, V>), ul);
+                copy_async<sizeof(T) * GV>(at_a + i * kBlock * sizeof(GVec<T, GV>), al);
+                ul += g.s_u; al += g.s_a;
+                if (GRAD) { copy_async<sizeof(T) * V>(at_p + i * kBlock * sizeof(GVec<T, V>), pl); pl += g.s_p; }
+            }
+        } else {
+            const int steps = s0 >= g.n ? 0 : g.n - s0 < L ? (int)(g.n - s0) : L;
+#pragma unroll 1
+            for (int i = 0; i < steps; ++i) {
+                copy_async<sizeof(T) * V>(at_u + i * kBlock * sizeof(GVec<T, V>), ul + i * g.s_u);
+                if (s0 + i > 0 || enters) copy_async<sizeof(T) * GV>(at_a + i * kBlock * sizeof(GVec<T, GV>), al + i * g.s_a);
+                if (GRAD && s0 + i + 1 < g.n) copy_async<sizeof(T) * V>(at_p + i * kBlock * sizeof(GVec<T, V>), pl + i * g.s_p);
+            }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -259,19 +270,29 @@ gated_strip_kernel(const GatedRuns g, int cluster_size) {
         for (int x = 0; x < GV; ++x) A[x] = T(1);
 #pragma unroll
         for (int v = 0; v < V; ++v) B[v] = T(0);
-        const bool starts = s0 == 0 && !enters;
+        const bool starts = s0 == 0 && !enters, whole = inside(s0);
+        if (whole) {
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-            if (i >= steps) break;
-            if (i == 0 && starts) {
+            for (int i = 0; i < L; ++i) {
 #pragma unroll
-                for (int v = 0; v < V; ++v) B[v] = uu[0].v[v];
-                continue;
+                for (int x = 0; x < GV; ++x) A[x] *= aa[i].v[x];
+#pragma unroll
+                for (int v = 0; v < V; ++v) B[v] = i == 0 ? uu[i].v[v] : gfma(aa[i].v[GM == kGateShared ? 0 : v], B[v], uu[i].v[v]);
             }
+        } else {
 #pragma unroll
-            for (int x = 0; x < GV; ++x) A[x] *= aa[i].v[x];
+            for (int i = 0; i < L; ++i) {
+                if (i >= steps) break;
+                if (i == 0 && starts) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) B[v] = i == 0 ? uu[i].v[v] : gfma(aa[i].v[GM == kGateShared ? 0 : v], B[v], uu[i].v[v]);
+                    for (int v = 0; v < V; ++v) B[v] = uu[0].v[v];
+                    continue;
+                }
+#pragma unroll
+                for (int x = 0; x < GV; ++x) A[x] *= aa[i].v[x];
+#pragma unroll
+                for (int v = 0; v < V; ++v) B[v] = i == 0 ? uu[i].v[v] : gfma(aa[i].v[GM == kGateShared ? 0 : v], B[v], uu[i].v[v]);
+            }
         }
 #pragma unroll
         for (int x = 0; x < GV; ++x) {
@@ -339,6 +360,29 @@ gated_strip_kernel(const GatedRuns g, int cluster_size) {
         // again, from the state in front
         char* ol = o + s0 * g.s_o;
         char* ql = GRAD ? q + s0 * g.s_q : nullptr;
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                GVec<T, V> out, dg;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    h[v] = gfma(aa[i].v[GM == kGateShared ? 0 : v], h[v], uu[i].v[v]);
+                    out.v[v] = h[v];
+                    if (GRAD) dg.v[v] = h[v] * pp[i].v[v];
+                }
+                if (live) gst<T, V>(ol, out);
+                ol += g.s_o;
+                if (GRAD) {
+                    if (GM == kGateShared && g.head) {
+                        const T sum = shared_sum(dg, g.head);
+                        if (live && (lane & (g.head - 1)) == 0) *reinterpret_cast<T*>(ql) = sum;
+                    } else if (live) {
+                        gst<T, V>(ql, dg);
+                    }
+                    ql += g.s_q;
+                }
+            }
+        } else
 #pragma unroll
         for (int i = 0; i < L; ++i) {
             if (i >= steps) break;
