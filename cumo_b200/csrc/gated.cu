@@ -589,10 +589,10 @@ static int launch_cluster(K kernel, const GatedRuns& g, unsigned ctas, int clust
     return 0;
 }
 
-// CTAs of a cluster per strip (or row): enough that the GPU has about two resident CTAs per SM's worth, no more than the steps feed.
+// CTAs of a cluster per strip (or row): as many as stay within two per SM, no more than the steps feed.
 static int cluster_for(int64_t ctas, int64_t steps, int64_t steps_per_cta) {
     int c = 1;
-    while (c < 8 && ctas * c < (int64_t)sm_count() * 2 && steps > steps_per_cta * c) c *= 2;
+    while (c < 8 && ctas * c * 2 <= (int64_t)sm_count() * 2 && steps > steps_per_cta * c) c *= 2;
     return c;
 }
 
@@ -647,7 +647,7 @@ static int launch_side_by_side(GatedRuns& g, int packet, int64_t shared_runs) {
     }
     // strips as wide as leaves two CTAs per SM with at most eight to a cluster; the gradients hold a third operand in registers
     // and take half as many steps at a time
-    if (sizeof(T) == 8 || (groups + 31) / 32 * 8 >= (int64_t)sm_count() * 2) {
+    if (sizeof(T) == 8 || (groups + 31) / 32 * 8 >= (int64_t)sm_count()) {
         if (!heads(V)) return (int)cudaErrorNotSupported;
         return launch_strip<T, V, GRAD ? 4 : 8, GM, GRAD>(g);
     }

@@ -215,6 +215,15 @@ struct SplitSet {
 
 static bool worth_splitting(int64_t m, int64_t n, int64_t k) { return m >= 32 && n >= 32 && k >= 32 && m * n * k >= (1LL << 22); }
 
+// The product on the CUDA cores: few rows of A, few rows of B (the same with the sides exchanged is not offered by the
+// epilogue's row-major output, so those take the tiles), or tiles.
+template <typename T>
+static int product(int64_t m, int64_t n, int64_t k, const Operand<T>& a, const Operand<T>& b, const Epilogue<T>& e, cudaStream_t st) {
+    static const int most = getenv("CB_R") ? atoi(getenv("CB_R")) : 32;
+    if (m <= most && k >= 16) return launch_product_rows<T>(m, n, k, a, b, e, st);
+    return launch_product_cc<T>(m, n, k, 1, a, b, e, st);
+}
+
 // ---- entry points ------------------------------------------------------------------------------------------------------
 template <typename T>
 static int linear(int64_t m, int64_t n, int64_t k, const T* x, ssize_t x_row, ssize_t x_col, const T* w, ssize_t w_row, ssize_t w_col,
@@ -231,7 +240,8 @@ static int linear(int64_t m, int64_t n, int64_t k, const T* x, ssize_t x_row, ss
     e.res = residual; e.res_row = r_row / es; e.res_col = r_col / es;
     e.y = y; e.ld = n; e.pre = pre;
     if constexpr (sizeof(T) == 4) {
-        if (worth_splitting(m, n, k)) {
+        static const int most = getenv("CB_R") ? atoi(getenv("CB_R")) : 32;
+        if (m > most && worth_splitting(m, n, k)) {
             const int late = product_gave_up();
             if (late) return late;
             Scratch scratch(current_stream());
@@ -243,7 +253,7 @@ static int linear(int64_t m, int64_t n, int64_t k, const T* x, ssize_t x_row, ss
         }
     }
     const Operand<T> a = {x, x_row / es, x_col / es, 0}, b = {w, w_col / es, w_row / es, 0};
-    return launch_product_cc<T>(m, n, k, 1, a, b, e, current_stream());
+    return product<T>(m, n, k, a, b, e, current_stream());
 }
 
 template <typename T>
@@ -299,13 +309,13 @@ static int linear_grad(int64_t m, int64_t n, int64_t k, const T* grad, ssize_t g
     if (dx) {                                    // dx[i][c] = sum_j dz[i][j] * w[c][j]
         e.y = dx; e.ld = k;
         const Operand<T> b = {w, w_row / es, w_col / es, 0};
-        const int rc = launch_product_cc<T>(m, k, n, 1, dz, b, e, st);
+        const int rc = product<T>(m, k, n, dz, b, e, st);
         if (rc) return rc;
     }
     if (dw) {                                    // dw[c][j] = sum_i x[i][c] * dz[i][j]
         e.y = dw; e.ld = n;
         const Operand<T> a = {x, x_col / es, x_row / es, 0}, b = {dz.p, dz.k, dz.row, 0};
-        const int rc = launch_product_cc<T>(k, n, m, 1, a, b, e, st);
+        const int rc = product<T>(k, n, m, a, b, e, st);
         if (rc) return rc;
     }
     return 0;
