@@ -86,6 +86,8 @@ def _declare(lib: ctypes.CDLL) -> None:
         "cb200_na_minmax": (c_int, [H, c_uint32, c_int, c_int, POINTER(H), POINTER(H)]),
         "cb200_na_bincount": (H, [H, H, c_int64]),
         "cb200_na_cum": (H, [c_char_p, H, c_int, c_int]),
+        "cb200_na_linear": (H, [H, H, H, c_int, H, POINTER(H)]),
+        "cb200_na_linear_grad": (c_int, [H, H, H, c_int, H, POINTER(H), POINTER(H), POINTER(H)]),
         "cb200_na_gated_cumsum": (H, [H, H, H, c_int]),
         "cb200_na_gated_cumsum_grad": (c_int, [H, H, H, H, c_int, POINTER(H), POINTER(H), POINTER(H)]),
         "cb200_na_where": (H, [H, c_int]),

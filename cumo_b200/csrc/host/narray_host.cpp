@@ -12,7 +12,9 @@
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <initializer_list>
 #include <string>
+#include <type_traits>
 #include <vector>
 
 namespace {
@@ -1163,6 +1165,120 @@ int cb200_na_gated_cumsum_grad(cb200_na_t* grad, cb200_na_t* gate, cb200_na_t* h
         if (!dinit) return give_up();
     }
     *dx_out = dx; *dgate_out = dgate; *dinitial_out = dinit;
+    return 0;
+}
+
+// ---- linear layer ----------------------------------------------------------------------------
+// An operand (..., width) as a matrix of evenly spaced rows: the array itself, or a contiguous copy where its leading
+// dimensions do not run evenly.
+struct Rows {
+    cb200_na* copy = nullptr;
+    char* p = nullptr;
+    ssize_t row = 0, col = 0;
+    ~Rows() { if (copy) cb200_na_release(copy); }
+    bool of(const cb200_na* x, int nd, const int64_t* shape, const int64_t* step) {
+        p = data_ptr(x);
+        col = shape[nd - 1] != 1 ? (ssize_t)step[nd - 1] : 0;
+        bool even = true;
+        int last = -1;
+        for (int d = nd - 2; d >= 0 && even; --d) {
+            if (shape[d] == 1) continue;
+            if (last < 0) row = (ssize_t)step[d];
+            else even = step[d] == step[last] * shape[last];
+            last = d;
+        }
+        if (even) return true;
+        cb200_na view = *x;
+        view.ndim = nd;
+        for (int d = 0; d < nd; ++d) { view.shape[d] = shape[d]; view.step[d] = step[d]; }
+        copy = cast_to(&view, x->dtype);
+        if (!copy) return false;
+        p = data_ptr(copy);
+        col = (ssize_t)copy->step[nd - 1];
+        row = (ssize_t)copy->step[nd - 2];
+        return true;
+    }
+};
+
+static bool linear_types(const char* what, const cb200_na* a, std::initializer_list<const cb200_na*> others) {
+    bool ok = is_float_type(a->dtype);
+    for (const cb200_na* x : others) ok = ok && (!x || x->dtype == a->dtype);
+    if (!ok) fail("TypeError", "%s needs operands that are all SFloat or all DFloat", what);
+    return ok;
+}
+
+cb200_na_t* cb200_na_linear(cb200_na_t* x, cb200_na_t* w, cb200_na_t* bias, int activation, cb200_na_t* residual, cb200_na_t** pre_out) {
+    if (pre_out) *pre_out = nullptr;
+    if (!linear_types("linear", x, {w, bias, residual})) return nullptr;
+    if (w->ndim != 2) return (cb200_na*)fail("ShapeError", "w needs two dimensions");
+    const int64_t k = w->shape[0], n = w->shape[1];
+    if (k == 0) return (cb200_na*)fail("ShapeError", "linear over an empty axis");
+    if (x->ndim < 1 || x->shape[x->ndim - 1] != k) return (cb200_na*)fail("ShapeError", "the last axis of x should be %lld", (long long)k);
+    if (bias && (bias->ndim != 1 || bias->shape[0] != n)) return (cb200_na*)fail("ShapeError", "bias should have the shape (%lld)", (long long)n);
+    int64_t shape[kMaxD], rstep[kMaxD], m = 1;
+    for (int d = 0; d + 1 < x->ndim; ++d) { shape[d] = x->shape[d]; m *= shape[d]; }
+    shape[x->ndim - 1] = n;
+    if (residual && !repeated_steps(residual, x->ndim, shape, "residual", rstep)) return nullptr;
+    Rows rx, rr;
+    if (m * n && !rx.of(x, x->ndim, x->shape, x->step)) return nullptr;
+    if (m * n && residual && !rr.of(residual, x->ndim, shape, rstep)) return nullptr;
+    cb200_na* y = make(x->dtype, x->ndim, shape, false);
+    cb200_na* pre = y && pre_out ? make(x->dtype, x->ndim, shape, false) : nullptr;
+    if (!y || (pre_out && !pre)) { cb200_na_release(y); return nullptr; }
+    int status = 0;
+    if (m * n) {
+        auto run = [&](auto f, auto* type) {
+            using T = std::remove_pointer_t<decltype(type)>;
+            return f(m, n, k, (const T*)rx.p, rx.row, rx.col, (const T*)data_ptr(w), (ssize_t)w->step[0], (ssize_t)w->step[1], bias ? (const T*)data_ptr(bias) : nullptr,
+                     bias ? (ssize_t)bias->step[0] : 0, (const T*)rr.p, rr.row, rr.col, activation, (T*)data_ptr(y), pre ? (T*)data_ptr(pre) : nullptr);
+        };
+        status = x->dtype == CB200_SFLOAT ? run(cb200_sfloat_linear_kernel_launch, (float*)nullptr) : run(cb200_dfloat_linear_kernel_launch, (double*)nullptr);
+    }
+    if (status) fail("CudaError", "linear: %s", cudaGetErrorString((cudaError_t)status));
+    if (status || !launch_ok()) { cb200_na_release(y); cb200_na_release(pre); return nullptr; }
+    if (pre_out) *pre_out = pre;
+    return y;
+}
+
+int cb200_na_linear_grad(cb200_na_t* grad, cb200_na_t* x, cb200_na_t* w, int activation, cb200_na_t* pre, cb200_na_t** dx_out, cb200_na_t** dw_out,
+                         cb200_na_t** dbias_out) {
+    if (dx_out) *dx_out = nullptr;
+    if (dw_out) *dw_out = nullptr;
+    if (dbias_out) *dbias_out = nullptr;
+    if (!linear_types("linear_grad", grad, {x, w, pre})) return 1;
+    if (w->ndim != 2) { fail("ShapeError", "w needs two dimensions"); return 1; }
+    const int64_t k = w->shape[0], n = w->shape[1];
+    if (k == 0) { fail("ShapeError", "linear_grad over an empty axis"); return 1; }
+    bool fits = x->ndim >= 1 && grad->ndim == x->ndim && x->shape[x->ndim - 1] == k && grad->shape[x->ndim - 1] == n;
+    int64_t m = 1;
+    for (int d = 0; fits && d + 1 < x->ndim; ++d) { fits = x->shape[d] == grad->shape[d]; m *= x->shape[d]; }
+    if (!fits) { fail("ShapeError", "x should be (.., %lld) and grad (.., %lld) with the same leading dimensions", (long long)k, (long long)n); return 1; }
+    if (activation) {
+        bool same = pre && pre->ndim == grad->ndim;
+        for (int d = 0; same && d < pre->ndim; ++d) same = pre->shape[d] == grad->shape[d];
+        if (!same) { fail(pre ? "ShapeError" : "ValueError", "with an activation, pre is needed in the shape of grad"); return 1; }
+    }
+    Rows rg, rx, rp;
+    if (m * n && (!rg.of(grad, grad->ndim, grad->shape, grad->step) || !rx.of(x, x->ndim, x->shape, x->step) ||
+                  (activation && !rp.of(pre, pre->ndim, pre->shape, pre->step)))) return 1;
+    cb200_na* dx = dx_out ? make(grad->dtype, x->ndim, x->shape, false) : nullptr;
+    cb200_na* dw = dw_out && (dx || !dx_out) ? make(grad->dtype, 2, w->shape, false) : nullptr;
+    cb200_na* db = dbias_out && (dw || !dw_out) ? make(grad->dtype, 1, &w->shape[1], false) : nullptr;
+    bool ok = (dx || !dx_out) && (dw || !dw_out) && (db || !dbias_out);
+    if (ok) {
+        auto run = [&](auto f, auto* type) {
+            using T = std::remove_pointer_t<decltype(type)>;
+            return f(m, n, k, (const T*)rg.p, rg.row, rg.col, (const T*)rx.p, rx.row, rx.col, (const T*)data_ptr(w), (ssize_t)w->step[0], (ssize_t)w->step[1],
+                     (const T*)rp.p, rp.row, rp.col, activation, dx ? (T*)data_ptr(dx) : nullptr, dw ? (T*)data_ptr(dw) : nullptr, db ? (T*)data_ptr(db) : nullptr);
+        };
+        const int status = grad->dtype == CB200_SFLOAT ? run(cb200_sfloat_linear_grad_kernel_launch, (float*)nullptr) : run(cb200_dfloat_linear_grad_kernel_launch, (double*)nullptr);
+        if (status) fail("CudaError", "linear_grad: %s", cudaGetErrorString((cudaError_t)status));
+        ok = !status && launch_ok();
+    }
+    if (!ok) { cb200_na_release(dx); cb200_na_release(dw); cb200_na_release(db); return 1; }
+    if (dx_out) *dx_out = dx;
+    if (dw_out) *dw_out = dw;
+    if (dbias_out) *dbias_out = db;
     return 0;
 }
 

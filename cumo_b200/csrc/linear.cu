@@ -204,9 +204,9 @@ struct SplitSet {
         }
         return rc;
     }
-    int product(int a, bool a_over_columns, int b, bool b_over_columns, const Epilogue<float>& e, cudaStream_t st) const {
+    int product(int a, bool a_over_columns, int b, bool b_over_columns, const Epilogue<float>& e, Scratch& scratch, cudaStream_t st) const {
         const Planes pa = x[a].operand(a_over_columns), pb = x[b].operand(b_over_columns);
-        int rc = launch_split_product(kSplitBf16x3, pa, pb, e, st);
+        int rc = launch_split_product(kSplitBf16x3, pa, pb, e, scratch, st);
         if (rc) return rc;
         return launch_fix_marked(pa.rows, pb.rows, pa.k, x[a].src, x[a].turned(a_over_columns), x[a].marks_of(a_over_columns), x[b].src,
                                  x[b].turned(b_over_columns), x[b].marks_of(b_over_columns), x[a].marks.any, e, st);
@@ -249,7 +249,7 @@ static int linear(int64_t m, int64_t n, int64_t k, const T* x, ssize_t x_row, ss
             const int ix = set.add(SplitSource{x, x_row / es, x_col / es, nullptr, 0, 0, kActNone}, m, k);
             const int iw = set.add(SplitSource{w, w_row / es, w_col / es, nullptr, 0, 0, kActNone}, k, n);
             int rc = set.split(scratch, current_stream());
-            return rc ? rc : set.product(ix, true, iw, false, e, current_stream());
+            return rc ? rc : set.product(ix, true, iw, false, e, scratch, current_stream());
         }
     }
     const Operand<T> a = {x, x_row / es, x_col / es, 0}, b = {w, w_col / es, w_row / es, 0};
@@ -288,9 +288,9 @@ static int linear_grad(int64_t m, int64_t n, int64_t k, const T* grad, ssize_t g
             Epilogue<float> e = {};
             e.alpha = 1.f;
             e.y = dx; e.ld = k;
-            if (rc == 0 && dx) rc = set.product(iz, true, iw, true, e, st);
+            if (rc == 0 && dx) rc = set.product(iz, true, iw, true, e, scratch, st);
             e.y = dw; e.ld = n;
-            if (rc == 0 && dw) rc = set.product(ix, false, iz, false, e, st);
+            if (rc == 0 && dw) rc = set.product(ix, false, iz, false, e, scratch, st);
             return rc;
         }
     }

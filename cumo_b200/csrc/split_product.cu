@@ -47,6 +47,7 @@ struct SplitArgs {
     int64_t tiles_m, tiles_n, n_tiles;          // n_tiles counts all batch entries
     int64_t batch;
     int a_k_major, b_k_major;
+    int splits, per_split;                      // K cut into so many pieces of so many K-blocks, each to an output of its own
     int symmetric;                              // square tiles on and above the diagonal; what lies above is written to both sides
     uint32_t idesc;
     int* gave_up;
@@ -270,10 +271,11 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
 
     const int64_t cluster = blockIdx.x / CG, clusters = gridDim.x / CG;
     const int64_t my_tiles = misplaced || cluster >= g.n_tiles ? 0 : (g.n_tiles - cluster + clusters - 1) / clusters;
-    const uint32_t chunks = (uint32_t)((g.kblocks + S::kChunkBlocks - 1) / S::kChunkBlocks);
     // bands of eight tile rows, walked column by column: the tiles in flight share rows of A and columns of B in L2
-    auto tile_of = [&](int64_t t, int64_t* batch, int64_t* i0, int64_t* j0) {
+    auto tile_of = [&](int64_t t, int64_t* batch, int64_t* i0, int64_t* j0, int* piece) {
         int64_t f = cluster + t * clusters;
+        *piece = (int)(f % g.splits);
+        f /= g.splits;
         const int64_t per = g.symmetric ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
         *batch = f / per;
         f -= *batch * per;
@@ -302,9 +304,11 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
             bool ok = true;
             for (int64_t t = 0; t < my_tiles && ok; ++t) {
                 int64_t batch, i0, j0;
-                tile_of(t, &batch, &i0, &j0);
+                int piece;
+                tile_of(t, &batch, &i0, &j0, &piece);
                 j0 += rank * S::kBRows;
-                for (int kb = 0; kb < g.kblocks; ++kb, ++it) {
+                const int end = (piece + 1) * g.per_split < g.kblocks ? (piece + 1) * g.per_split : g.kblocks;
+                for (int kb = piece * g.per_split; kb < end; ++kb, ++it) {
                     const uint32_t slot = it % S::kStages;
                     if (!mbar_wait(empty + slot, ((it / S::kStages) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
                     if (rank == 0) mbar_expect_tx(full + slot, (uint32_t)(S::kStageBytes * CG));
@@ -340,12 +344,14 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
             bool ok = true;
             const uint32_t a_step = g.a_k_major ? 32u : 2048u, b_step = g.b_k_major ? 32u : 2048u;     // bytes per 16 of K
             for (int64_t t = 0; t < my_tiles && ok; ++t) {
-                for (int kb0 = 0; kb0 < g.kblocks && ok; kb0 += S::kChunkBlocks, ++item) {
+                const int piece = (int)((cluster + t * clusters) % g.splits);
+                const int end = (piece + 1) * g.per_split < g.kblocks ? (piece + 1) * g.per_split : g.kblocks;
+                for (int kb0 = piece * g.per_split; kb0 < end && ok; kb0 += S::kChunkBlocks, ++item) {
                     const uint32_t acc = item & 1u;
                     if (!mbar_wait_pair(acc_empty + acc, ((item >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t d_tmem = tmem_base + acc * (uint32_t)BN;
-                    const int kb1 = kb0 + S::kChunkBlocks < g.kblocks ? kb0 + S::kChunkBlocks : g.kblocks;
+                    const int kb1 = kb0 + S::kChunkBlocks < end ? kb0 + S::kChunkBlocks : end;
                     for (int kb = kb0; kb < kb1; ++kb, ++it) {
                         const uint32_t slot = it % S::kStages;
                         if (!mbar_wait(full + slot, (it / S::kStages) & 1u, abort_flag)) { ok = false; break; }
@@ -396,7 +402,10 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
         bool ok = true;
         for (int64_t t = 0; t < my_tiles && ok; ++t) {
             int64_t batch, i0, j0;
-            tile_of(t, &batch, &i0, &j0);
+            int part;
+            tile_of(t, &batch, &i0, &j0, &part);
+            const int blocks = (part + 1) * g.per_split < g.kblocks ? g.per_split : g.kblocks - part * g.per_split;
+            const uint32_t chunks = (uint32_t)((blocks + S::kChunkBlocks - 1) / S::kChunkBlocks);
             for (uint32_t c = 0; c < chunks; ++c, ++item) {
                 const uint32_t acc = item & 1u;
                 if (!__all_sync(0xffffffffu, mbar_wait(acc_full + acc, (item >> 1) & 1u, abort_flag))) { ok = false; break; }
@@ -431,7 +440,7 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
 #pragma unroll
                 for (int x = 0; x < 32; ++x) piece[lane * kSpStageCols + x] = sum[q * 32 + x];
                 __syncwarp();
-                if (row0 < g.m) out.piece(piece, lane, batch, row0, col0 + q * 32, g.m, g.n, g.symmetric && i0 / (128 * CG) != j0 / BN);
+                if (row0 < g.m) out.piece(piece, lane, g.splits > 1 ? part : batch, row0, col0 + q * 32, g.m, g.n, g.symmetric && i0 / (128 * CG) != j0 / BN);
                 __syncwarp();
             }
         }
@@ -495,7 +504,7 @@ static bool planes_map(CUtensorMap* map, const Planes& x, int planes, int box_ro
 }
 
 template <int P, int CG, int BN, typename Out>
-static int launch_shape(SplitKind kind, const Planes& a, const Planes& b, const Out& out, bool symmetric, cudaStream_t st) {
+static int launch_shape(SplitKind kind, const Planes& a, const Planes& b, const Out& out, bool symmetric, int splits, cudaStream_t st) {
     using S = SplitShape<P, CG, BN>;
     SplitArgs g;
     memset(&g, 0, sizeof g);
@@ -504,7 +513,9 @@ static int launch_shape(SplitKind kind, const Planes& a, const Planes& b, const 
     g.tiles_m = (a.rows + 128 * CG - 1) / (128 * CG);
     g.tiles_n = (b.rows + BN - 1) / BN;
     g.symmetric = symmetric && BN == 128 * CG;
-    g.n_tiles = (g.symmetric ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n) * a.batch;
+    g.per_split = (g.kblocks + splits - 1) / splits;
+    g.splits = (g.kblocks + g.per_split - 1) / g.per_split;             // no piece is empty
+    g.n_tiles = g.splits * (g.symmetric ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n) * a.batch;
     g.a_k_major = a.k_major; g.b_k_major = b.k_major;
     const uint32_t fmt = kind == kSplitBf16x3 ? 1u : 0u;
     g.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((a.k_major ? 0u : 1u) << 15) | ((b.k_major ? 0u : 1u) << 16) | ((uint32_t)(BN >> 3) << 17) |
@@ -528,6 +539,11 @@ static int launch_shape(SplitKind kind, const Planes& a, const Planes& b, const 
     }
     const int64_t slots = sm_count() / CG;
     const unsigned grid = (unsigned)((g.n_tiles < slots ? g.n_tiles : slots) * CG);
+    if (CG == 1) {
+        kernel<<<grid, kSpThreads, S::kSmem, st>>>(g, ma, mb, out);
+        count_launch();
+        return (int)cudaGetLastError();
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kSpThreads);
@@ -544,32 +560,78 @@ static int launch_shape(SplitKind kind, const Planes& a, const Planes& b, const 
     return 0;
 }
 
-// The tile is the one with the least rounds x time per round, in cycles per 16 of K and product: measured at 4096^3, a
-// 256 x 256 pair takes the tensor cores' 128, a 128 x 128 tile 95 and a 128 x 64 tile 70 (bound by what L2 delivers), the
-// latter two on twice as many slots.
-template <int P, typename Out>
-static int launch_any(SplitKind kind, const Planes& a, const Planes& b, const Out& out, bool symmetric, cudaStream_t st) {
-    if (a.k != b.k || a.batch != b.batch || a.k < 1 || (symmetric && a.rows != b.rows)) return (int)cudaErrorInvalidValue;
-    const int64_t sms = sm_count();
-    auto rounds = [&](int64_t tm, int64_t tn, int64_t slots) {
-        const int64_t across = (a.rows + tm - 1) / tm;
-        const int64_t tiles = (symmetric && tm == tn ? across * (across + 1) / 2 : across * ((b.rows + tn - 1) / tn)) * a.batch;
-        return (tiles + slots - 1) / slots;
-    };
-    const int64_t big = rounds(256, 256, sms / 2) * 128, mid = rounds(128, 128, sms) * 95, small = rounds(128, 64, sms) * 70;
-    if (big <= mid && big <= small) return launch_shape<P, 2, 256, Out>(kind, a, b, out, symmetric, st);
-    if (mid <= small) return launch_shape<P, 1, 128, Out>(kind, a, b, out, symmetric, st);
-    return launch_shape<P, 1, 64, Out>(kind, a, b, out, symmetric, st);
+// The tile and the number of pieces K is cut into are those with the least estimated cycles: rounds over the SMs x K-blocks of
+// a piece x instructions x cycles per instruction -- measured at 4096^3, a 256 x 256 pair takes the tensor cores' 128, a
+// 128 x 128 tile 95 and a 128 x 64 tile 70 (bound by what L2 delivers), the latter two on twice as many slots -- plus, with
+// pieces, writing and adding up their results (about 2500 bytes per cycle) and one more launch.
+struct Shape { int tile, splits; };
+
+static Shape choose_shape(int terms, const Planes& a, const Planes& b, bool symmetric, int most_splits) {
+    const int64_t sms = sm_count(), kblocks = (a.k + kSpKB - 1) / kSpKB;
+    const int64_t tm[3] = {256, 128, 128}, tn[3] = {256, 128, 64}, cycles[3] = {128, 95, 70}, slots[3] = {sms / 2, sms, sms};
+    Shape best = {0, 1};
+    int64_t least = INT64_MAX;
+    for (int t = 0; t < 3; ++t) {
+        const int64_t across = (a.rows + tm[t] - 1) / tm[t];
+        const int64_t tiles = (symmetric && tm[t] == tn[t] ? across * (across + 1) / 2 : across * ((b.rows + tn[t] - 1) / tn[t])) * a.batch;
+        for (int s = 1; s <= most_splits && (s == 1 || kblocks / s >= 2); ++s) {
+            const int64_t rounds = (tiles * s + slots[t] - 1) / slots[t];
+            int64_t cost = rounds * ((kblocks + s - 1) / s * 4 * terms * cycles[t] + 3000);
+            if (s > 1) cost += 6000 + (int64_t)(s + 1) * a.rows * b.rows * 4 / 2500;
+            if (cost < least) { least = cost; best = {t, s}; }
+        }
+    }
+    return best;
 }
 
-int launch_split_product(SplitKind kind, const Planes& a, const Planes& b, const Epilogue<float>& e, cudaStream_t st) {
-    if (e.alpha != 1.0f || e.d) return (int)cudaErrorInvalidValue;
-    const FloatOut out = {e, e.ld % 4 == 0 && aligned16(e.y) && (!e.res || (e.res_col == 1 && e.res_row % 4 == 0 && aligned16(e.res)))};
-    return kind == kSplitBf16x3 ? launch_any<3>(kind, a, b, out, false, st) : launch_any<2>(kind, a, b, out, false, st);
+template <int P, typename Out>
+static int launch_any(SplitKind kind, const Planes& a, const Planes& b, const Out& out, bool symmetric, Shape shape, cudaStream_t st) {
+    if (a.k != b.k || a.batch != b.batch || a.k < 1 || (symmetric && a.rows != b.rows)) return (int)cudaErrorInvalidValue;
+    if (shape.tile == 0) return launch_shape<P, 2, 256, Out>(kind, a, b, out, symmetric, shape.splits, st);
+    if (shape.tile == 1) return launch_shape<P, 1, 128, Out>(kind, a, b, out, symmetric, shape.splits, st);
+    return launch_shape<P, 1, 64, Out>(kind, a, b, out, symmetric, shape.splits, st);
+}
+
+// The pieces' results added in order, and the epilogue.
+__global__ void __launch_bounds__(kBlock)
+join_pieces_kernel(int64_t m, int64_t n, int splits, const float* pieces, const Epilogue<float> e) {
+    const int64_t total = m * n;
+    for (int64_t f = (int64_t)blockIdx.x * kBlock + threadIdx.x; f < total; f += (int64_t)gridDim.x * kBlock) {
+        float part[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) if (s < splits) part[s] = pieces[s * total + f];
+        float z = part[0];
+#pragma unroll
+        for (int s = 1; s < 8; ++s) if (s < splits) z += part[s];
+        const int64_t i = f / n;
+        finish(e, 0, i, f - i * n, z);
+    }
+}
+
+int launch_split_product(SplitKind kind, const Planes& a, const Planes& b, const Epilogue<float>& e, Scratch& scratch, cudaStream_t st) {
+    if (e.alpha != 1.0f || e.d || a.batch != 1) return (int)cudaErrorInvalidValue;
+    Shape shape = choose_shape(kind == kSplitBf16x3 ? 6 : 3, a, b, false, 8);
+    Epilogue<float> way = e;
+    float* pieces = nullptr;
+    if (shape.splits > 1) {
+        const int64_t kblocks = (a.k + kSpKB - 1) / kSpKB, per = (kblocks + shape.splits - 1) / shape.splits;
+        shape.splits = (int)((kblocks + per - 1) / per);
+        pieces = reinterpret_cast<float*>(scratch.take((size_t)shape.splits * a.rows * b.rows * sizeof(float)));
+        if (!pieces) return (int)cudaErrorMemoryAllocation;
+        way = Epilogue<float>{};
+        way.alpha = 1.f; way.y = pieces; way.ld = b.rows; way.y_batch = a.rows * b.rows;
+    }
+    const FloatOut out = {way, way.ld % 4 == 0 && aligned16(way.y) && way.y_batch % 4 == 0 &&
+                                   (!way.res || (way.res_col == 1 && way.res_row % 4 == 0 && aligned16(way.res)))};
+    int rc = kind == kSplitBf16x3 ? launch_any<3>(kind, a, b, out, false, shape, st) : launch_any<2>(kind, a, b, out, false, shape, st);
+    if (rc || shape.splits == 1) return rc;
+    join_pieces_kernel<<<grid_for((a.rows * b.rows + kBlock - 1) / kBlock, 8), kBlock, 0, st>>>(a.rows, b.rows, shape.splits, pieces, e);
+    count_launch();
+    return (int)cudaGetLastError();
 }
 int launch_split_product(const Planes& a, const Planes& b, const PlaneEpilogue& e, bool symmetric, cudaStream_t st) {
     const PlaneOut out = {e};
-    return launch_any<2>(kSplitHalfx2, a, b, out, symmetric, st);
+    return launch_any<2>(kSplitHalfx2, a, b, out, symmetric, choose_shape(3, a, b, symmetric, 1), st);
 }
 
 }  // namespace cb200

@@ -39,7 +39,7 @@ struct PlaneEpilogue {
 
 // C = A . B^T (per batch entry), contraction over k; the result leaves through `e` (float) or `pe` (planes).  Returns a
 // cudaError_t; cudaErrorNotSupported when tensor maps cannot be had, in which case nothing was launched.
-int launch_split_product(SplitKind kind, const Planes& a, const Planes& b, const Epilogue<float>& e, cudaStream_t st);
+int launch_split_product(SplitKind kind, const Planes& a, const Planes& b, const Epilogue<float>& e, Scratch& scratch, cudaStream_t st);
 // `symmetric` says that the result is (A = B, or A and B symmetric and equal, and d symmetric): about half the tiles are computed.
 int launch_split_product(const Planes& a, const Planes& b, const PlaneEpilogue& e, bool symmetric, cudaStream_t st);
 

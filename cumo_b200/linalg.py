@@ -7,10 +7,10 @@ every operand into two TF32 numbers and wants both operands with K contiguous.
 """
 from __future__ import annotations
 
-from ctypes import c_char_p, c_double, c_int, c_int64, c_size_t, c_ssize_t, c_void_p, create_string_buffer
+from ctypes import byref, c_char_p, c_double, c_int, c_int64, c_size_t, c_ssize_t, c_void_p, create_string_buffer
 
 from . import _lib
-from .narray import CudaError, CumoError, DFloat, SFloat, ShapeError
+from .narray import CudaError, CumoError, DFloat, SFloat, ShapeError, _raise_last
 
 
 def gemm_nt(a: SFloat, bt: SFloat) -> SFloat:
@@ -38,7 +38,7 @@ def gemm(a, b, alpha=1.0, beta=0.0, c=None):
     matrices, leading axes are batches; either operand may be a transposed view; an operand that holds one matrix is
     used for every batch of the other): alpha * a . b + beta * c.
     It hands cuBLAS's column-major bookkeeping to the library exactly as gemm.c does: c^T = b^T . a^T."""
-    from ctypes import byref, c_float, c_longlong
+    from ctypes import c_float, c_longlong
 
     T = type(a)
     if T not in (SFloat, DFloat) or type(b) is not T or a.ndim < 2 or b.ndim < 2:
@@ -106,25 +106,6 @@ def _activation(name):
     return ACTIVATIONS.index(name)
 
 
-def _rows(x, width, what):
-    """`x` (..., width) as a matrix of rows; a view of it where its leading axes are evenly spaced, else of a copy."""
-    if x.ndim < 1 or x.shape[-1] != width:
-        raise ShapeError(f"{what} has shape {x.shape}, its last axis should be {width}")
-    if x.ndim == 2:
-        return x
-    if x.ndim == 1:
-        return x[None, ...]
-    shp, st = x.shape, x.steps
-    lead = [(n, s) for n, s in zip(shp[:-1], st[:-1]) if n != 1]
-    even = all(a[1] == b[0] * b[1] for a, b in zip(lead, lead[1:]))
-    if not even or x.size == 0:
-        return x.reshape(x.size // width if width else 0, width)
-    rows = 1
-    for n, _ in lead:
-        rows *= n
-    return x._view([rows, width], [lead[-1][1] if lead else 0, st[-1]], 0)
-
-
 def _ptr(x):
     return c_void_p(x.data_ptr if x is not None else None)
 
@@ -147,64 +128,39 @@ def _status(rc, what):
         raise CudaError(f"{what} failed with CUDA status {rc}")
 
 
+def _handle(x):
+    return None if x is None else x._h
+
+
 def linear(x, w, bias=None, activation=None, residual=None, keep=False):
     """act(x . w + bias) + residual in one pass: x (..., K), w (K, N) -> (..., N), all SFloat or all DFloat, every operand
     an array or any view of one (a transposed `w` is not copied).  `bias` (N,) and `residual` (repeated to the result's
     shape) may be left out; `activation` is None, "relu", "silu", "gelu", "gelu_tanh", "sigmoid" or "tanh".  With `keep`
     also returns the value in front of the activation, which linear_grad needs."""
-    T = type(x)
-    _check_types(T, w=w, bias=bias, residual=residual)
+    _check_types(type(x), w=w, bias=bias, residual=residual)
+    if w is None:
+        raise TypeError("linear needs w")
     act = _activation(activation)
-    if w.ndim != 2:
-        raise ShapeError(f"w has shape {w.shape}, two axes are needed")
-    k, n = w.shape
-    if k == 0:
-        raise ShapeError("linear over an empty axis")
-    x2 = _rows(x, k, "x")
-    m = x2.shape[0]
-    shape = x.shape[:-1] + (n,)
-    if bias is not None and tuple(bias.shape) != (n,):
-        raise ShapeError(f"bias has shape {bias.shape}, not {(n,)}")
-    r2 = None if residual is None else _rows(residual if residual.shape == shape else residual._repeated_to(shape), n, "residual")
-    y = T(*shape)
-    pre = T(*shape) if keep else None
-    fn = getattr(_lib.load(), f"cb200_{y._tname}_linear_kernel_launch")
-    fn.restype, fn.argtypes = c_int, None
-    _status(fn(c_int64(m), c_int64(n), c_int64(k), _ptr(x2), _step(x2, 0), _step(x2, 1), _ptr(w), _step(w, 0), _step(w, 1), _ptr(bias), _step(bias, 0),
-               _ptr(r2), _step(r2, 0), _step(r2, 1), c_int(act), _ptr(y), _ptr(pre)), "linear")
-    return (y, pre) if keep else y
+    pre = c_void_p()
+    y = type(x)._from_handle(_lib.load().cb200_na_linear(x._h, w._h, _handle(bias), act, _handle(residual), byref(pre) if keep else None))
+    return (y, type(x)._from_handle(pre.value)) if keep else y
 
 
 def linear_grad(grad, x, w, activation=None, pre=None, want=("x", "w", "bias")):
     """The gradients of `y, pre = linear(x, w, bias, activation, residual, keep=True)` for grad = dL/dy (..., N): a tuple of
     those that `want` names, in its order -- "x" in x's shape, "w" in w's, "bias" (N,).  (The residual's gradient is grad.)
     `pre` may be left out when there is no activation.  Sums run in a fixed order: the same operands give the same bits."""
-    T = type(grad)
-    _check_types(T, x=x, w=w, pre=pre)
+    _check_types(type(grad), x=x, w=w, pre=pre)
+    if x is None or w is None:
+        raise TypeError("linear_grad needs x and w")
     act = _activation(activation)
     want = (want,) if isinstance(want, str) else tuple(want)
     if not want or len(set(want)) != len(want) or not set(want) <= {"x", "w", "bias"}:
         raise ValueError('want names some of "x", "w" and "bias", each once')
-    if act and pre is None:
-        raise ValueError("pre is needed with an activation")
-    if w.ndim != 2:
-        raise ShapeError(f"w has shape {w.shape}, two axes are needed")
-    k, n = w.shape
-    if k == 0:
-        raise ShapeError("linear_grad over an empty axis")
-    x2, g2 = _rows(x, k, "x"), _rows(grad, n, "grad")
-    if grad.shape[:-1] != x.shape[:-1]:
-        raise ShapeError(f"grad has shape {grad.shape}, x {x.shape}")
-    if act and pre.shape != grad.shape:
-        raise ShapeError(f"pre has shape {pre.shape}, grad {grad.shape}")
-    p2 = _rows(pre, n, "pre") if act else None
-    out = {"x": T(*x.shape) if "x" in want else None, "w": T(k, n) if "w" in want else None, "bias": T(n) if "bias" in want else None}
-    fn = getattr(_lib.load(), f"cb200_{grad._tname}_linear_grad_kernel_launch")
-    fn.restype, fn.argtypes = c_int, None
-    _status(fn(c_int64(x2.shape[0]), c_int64(n), c_int64(k), _ptr(g2), _step(g2, 0), _step(g2, 1), _ptr(x2), _step(x2, 0), _step(x2, 1),
-               _ptr(w), _step(w, 0), _step(w, 1), _ptr(p2), _step(p2, 0), _step(p2, 1), c_int(act), _ptr(out["x"]), _ptr(out["w"]), _ptr(out["bias"])),
-            "linear_grad")
-    return tuple(out[name] for name in want)
+    out = {name: c_void_p() for name in want}
+    if _lib.load().cb200_na_linear_grad(grad._h, x._h, w._h, act, _handle(pre), *(byref(out[name]) if name in out else None for name in ("x", "w", "bias"))):
+        _raise_last()
+    return tuple(type(grad)._from_handle(out[name].value) for name in want)
 
 
 def orthogonalize(g, steps=5, coefs=(3.4445, -4.7750, 2.0315), eps=1e-7):

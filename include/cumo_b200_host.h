@@ -100,6 +100,12 @@ cb200_na_t* cb200_na_where(cb200_na_t* bits, int want_zeros);
 /* cumsum / cumprod (narray/gen/tmpl/cum.c:41-70): axis < 0 runs over all elements in row-major order, else along
  * that axis; the result has the operand's shape and type.  nan: the NaN-skipping operator (float types). */
 cb200_na_t* cb200_na_cum(const char* op, cb200_na_t* a, int axis, int nan);
+/* act(x . w + bias) + residual for x (.., k), w (k, n); bias (n), residual (repeated to the result's shape) and pre (receives
+ * the value in front of the activation) may be NULL.  Activations are numbered as in cb200_<T>_linear_kernel_launch. */
+cb200_na_t* cb200_na_linear(cb200_na_t* x, cb200_na_t* w, cb200_na_t* bias, int activation, cb200_na_t* residual, cb200_na_t** pre);
+/* Its gradients for grad (.., n); each output may be NULL, pre too without an activation.  Returns 0, or 1 with cb200_host_error() set. */
+int cb200_na_linear_grad(cb200_na_t* grad, cb200_na_t* x, cb200_na_t* w, int activation, cb200_na_t* pre, cb200_na_t** dx, cb200_na_t** dw,
+                         cb200_na_t** dbias);
 /* h[t] = gate[t] * h[t-1] + x[t] along `axis`, in x's shape; gate is repeated to x's shape, initial (may be NULL: h[0] = x[0])
  * to the shape without the axis.  All SFloat or all DFloat. */
 cb200_na_t* cb200_na_gated_cumsum(cb200_na_t* x, cb200_na_t* gate, cb200_na_t* initial, int axis);
