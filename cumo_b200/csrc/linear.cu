@@ -185,31 +185,39 @@ struct SplitSet {
         a.ld = planes_ld(a.C);
         return count++;
     }
-    // scratch for all of them, marks cleared by one memset, then the splits
+    // scratch for all of them, marks cleared by one memset, then one launch that splits them
     int split(Scratch& scratch, cudaStream_t st) {
         size_t marks = 16;
         for (int i = 0; i < count; ++i) marks += (size_t)(x[i].R + x[i].C);
         char* mk = scratch.take(marks);
         if (!mk) return (int)cudaErrorMemoryAllocation;
-        int rc = (int)cudaMemsetAsync(mk, 0, marks, st);
+        const int rc = (int)cudaMemsetAsync(mk, 0, marks, st);
+        if (rc) return rc;
         int* any = reinterpret_cast<int*>(mk);
         mk += 16;
-        for (int i = 0; i < count && rc == 0; ++i) {
+        SplitJobs jobs = {};
+        jobs.count = count;
+        for (int i = 0; i < count; ++i) {
             SplitMatrix& a = x[i];
             a.planes = reinterpret_cast<uint16_t*>(scratch.take((size_t)3 * a.R * a.ld * 2));
             if (!a.planes) return (int)cudaErrorMemoryAllocation;
             a.marks = {reinterpret_cast<uint8_t*>(mk), reinterpret_cast<uint8_t*>(mk) + a.R, any};
             mk += a.R + a.C;
-            rc = launch_split(a.src, a.R, a.C, a.planes, a.ld, a.marks, st);
+            jobs.job[i] = {a.src, a.R, a.C, a.ld, a.planes, a.marks};
         }
-        return rc;
+        return launch_split(jobs, st);
     }
-    int product(int a, bool a_over_columns, int b, bool b_over_columns, const Epilogue<float>& e, Scratch& scratch, cudaStream_t st) const {
+    FixJobs fixes = {};
+    int product(int a, bool a_over_columns, int b, bool b_over_columns, const Epilogue<float>& e, Scratch& scratch, cudaStream_t st) {
         const Planes pa = x[a].operand(a_over_columns), pb = x[b].operand(b_over_columns);
-        int rc = launch_split_product(kSplitBf16x3, pa, pb, e, scratch, st);
-        if (rc) return rc;
-        return launch_fix_marked(pa.rows, pb.rows, pa.k, x[a].src, x[a].turned(a_over_columns), x[a].marks_of(a_over_columns), x[b].src,
-                                 x[b].turned(b_over_columns), x[b].marks_of(b_over_columns), x[a].marks.any, e, st);
+        fixes.job[fixes.count++] = {pa.rows, pb.rows, pa.k, x[a].src, x[b].src, x[a].turned(a_over_columns), x[b].turned(b_over_columns),
+                                    x[a].marks_of(a_over_columns), x[b].marks_of(b_over_columns), e};
+        return launch_split_product(kSplitBf16x3, pa, pb, e, scratch, st);
+    }
+    // what the marks ask for, once all products are queued
+    int fix(cudaStream_t st) {
+        fixes.any = x[0].marks.any;
+        return launch_fix_marked(fixes, st);
     }
 };
 
@@ -249,7 +257,8 @@ static int linear(int64_t m, int64_t n, int64_t k, const T* x, ssize_t x_row, ss
             const int ix = set.add(SplitSource{x, x_row / es, x_col / es, nullptr, 0, 0, kActNone}, m, k);
             const int iw = set.add(SplitSource{w, w_row / es, w_col / es, nullptr, 0, 0, kActNone}, k, n);
             int rc = set.split(scratch, current_stream());
-            return rc ? rc : set.product(ix, true, iw, false, e, scratch, current_stream());
+            if (rc == 0) rc = set.product(ix, true, iw, false, e, scratch, current_stream());
+            return rc ? rc : set.fix(current_stream());
         }
     }
     const Operand<T> a = {x, x_row / es, x_col / es, 0}, b = {w, w_col / es, w_row / es, 0};
@@ -291,7 +300,7 @@ static int linear_grad(int64_t m, int64_t n, int64_t k, const T* grad, ssize_t g
             if (rc == 0 && dx) rc = set.product(iz, true, iw, true, e, scratch, st);
             e.y = dw; e.ld = n;
             if (rc == 0 && dw) rc = set.product(ix, false, iz, false, e, scratch, st);
-            return rc;
+            return rc ? rc : set.fix(st);
         }
     }
     if (activation != kActNone || dbias) {

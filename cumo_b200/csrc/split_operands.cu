@@ -27,15 +27,18 @@ __device__ __forceinline__ float source_at(const SplitSource& s, int64_t i, int6
 
 // A thread takes eight neighbouring columns: two 16-byte loads where the source allows it, one 16-byte store per plane.
 // Bound by memory: 4 bytes read and 6 written per element (8 read with an activation's slope).
-template <bool VEC>
 __global__ void __launch_bounds__(kBlock)
-split_kernel(const SplitSource s, int64_t R, int64_t C, uint16_t* planes, int64_t ld, const Marks marks) {
-    const int64_t groups = ld / 8, total = R * groups;
-    const int64_t plane = R * ld;
+split_kernel(const SplitJobs jobs) {
+    const SplitJob& job = jobs.job[blockIdx.y];
+    const SplitSource& s = job.s;
+    const int64_t C = job.C, ld = job.ld, groups = ld / 8, total = job.R * groups, plane = job.R * ld;
+    uint16_t* planes = job.planes;
+    const bool vec = s.col == 1 && (reinterpret_cast<uintptr_t>(s.p) & 15) == 0 && s.row % 4 == 0 &&
+                     (s.act == kActNone || (s.pre_col == 1 && (reinterpret_cast<uintptr_t>(s.pre) & 15) == 0 && s.pre_row % 4 == 0));
     for (int64_t f = (int64_t)blockIdx.x * kBlock + threadIdx.x; f < total; f += (int64_t)gridDim.x * kBlock) {
-        const int64_t i = f / groups, j = (f - i * groups) * 8;
+        const int64_t i = total < 0x7fffffff ? (int64_t)((uint32_t)f / (uint32_t)groups) : f / groups, j = (f - i * groups) * 8;
         float v[8];
-        if (VEC && j + 8 <= C) {
+        if (vec && j + 8 <= C) {
             const float4* p = reinterpret_cast<const float4*>(s.p + i * s.row + j);
             const float4 x = __ldg(p), y = __ldg(p + 1);
             v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
@@ -62,41 +65,41 @@ split_kernel(const SplitSource s, int64_t R, int64_t C, uint16_t* planes, int64_
 #pragma unroll
         for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4*>(planes + p * plane + i * ld + j) = make_uint4(out[p][0], out[p][1], out[p][2], out[p][3]);
         if (!fine) {
-            *marks.any = 1;
-            marks.row[i] = 1;
+            *job.marks.any = 1;
+            job.marks.row[i] = 1;
             for (int e = 0; e < 8; ++e)
-                if (j + e < C && (__float_as_uint(v[e]) & 0x7fffffffu) >= 0x7f7f8000u) marks.col[j + e] = 1;
+                if (j + e < C && (__float_as_uint(v[e]) & 0x7fffffffu) >= 0x7f7f8000u) job.marks.col[j + e] = 1;
         }
     }
 }
 
-int launch_split(const SplitSource& s, int64_t R, int64_t C, uint16_t* planes, int64_t ld, const Marks& marks, cudaStream_t st) {
-    const bool vec = s.col == 1 && aligned16(s.p) && s.row % 4 == 0 &&
-                     (s.act == kActNone || (s.pre_col == 1 && aligned16(s.pre) && s.pre_row % 4 == 0));
-    const unsigned grid = grid_for((R * (ld / 8) + kBlock - 1) / kBlock, 16);
-    if (vec) split_kernel<true><<<grid, kBlock, 0, st>>>(s, R, C, planes, ld, marks);
-    else split_kernel<false><<<grid, kBlock, 0, st>>>(s, R, C, planes, ld, marks);
+int launch_split(const SplitJobs& jobs, cudaStream_t st) {
+    int64_t most = 0;
+    for (int i = 0; i < jobs.count; ++i) { const int64_t t = jobs.job[i].R * (jobs.job[i].ld / 8); most = t > most ? t : most; }
+    split_kernel<<<dim3(grid_for((most + kBlock - 1) / kBlock, 16), (unsigned)jobs.count), kBlock, 0, st>>>(jobs);
     count_launch();
     return (int)cudaGetLastError();
 }
 
 __global__ void __launch_bounds__(kBlock)
-fix_marked_kernel(int64_t m, int64_t n, int64_t k, const SplitSource a, bool a_turned, const uint8_t* a_marks, const SplitSource b, bool b_turned,
-                  const uint8_t* b_marks, const int* any, const Epilogue<float> e) {
-    if (*any == 0) return;
-    const int64_t total = m * n;
+fix_marked_kernel(const FixJobs jobs) {
+    if (*jobs.any == 0) return;
+    const FixJob& x = jobs.job[blockIdx.y];
+    const int64_t total = x.m * x.n;
     for (int64_t f = (int64_t)blockIdx.x * kBlock + threadIdx.x; f < total; f += (int64_t)gridDim.x * kBlock) {
-        const int64_t i = f / n, j = f - i * n;
-        if (!a_marks[i] && !b_marks[j]) continue;
+        const int64_t i = f / x.n, j = f - i * x.n;
+        if (!x.a_marks[i] && !x.b_marks[j]) continue;
         float acc = 0.f;
-        for (int64_t c = 0; c < k; ++c) acc = fmaf(a_turned ? source_at(a, c, i) : source_at(a, i, c), b_turned ? source_at(b, c, j) : source_at(b, j, c), acc);
-        finish(e, 0, i, j, acc);
+        for (int64_t c = 0; c < x.k; ++c)
+            acc = fmaf(x.a_turned ? source_at(x.a, c, i) : source_at(x.a, i, c), x.b_turned ? source_at(x.b, c, j) : source_at(x.b, j, c), acc);
+        finish(x.e, 0, i, j, acc);
     }
 }
 
-int launch_fix_marked(int64_t m, int64_t n, int64_t k, const SplitSource& a, bool a_turned, const uint8_t* a_marks, const SplitSource& b, bool b_turned,
-                      const uint8_t* b_marks, const int* any, const Epilogue<float>& e, cudaStream_t st) {
-    fix_marked_kernel<<<grid_for((m * n + kBlock - 1) / kBlock, 4), kBlock, 0, st>>>(m, n, k, a, a_turned, a_marks, b, b_turned, b_marks, any, e);
+int launch_fix_marked(const FixJobs& jobs, cudaStream_t st) {
+    int64_t most = 0;
+    for (int i = 0; i < jobs.count; ++i) { const int64_t t = jobs.job[i].m * jobs.job[i].n; most = t > most ? t : most; }
+    fix_marked_kernel<<<dim3(grid_for((most + kBlock - 1) / kBlock, 2), (unsigned)jobs.count), kBlock, 0, st>>>(jobs);
     count_launch();
     return (int)cudaGetLastError();
 }

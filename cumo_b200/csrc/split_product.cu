@@ -6,8 +6,7 @@
 //               128-byte-swizzled stages
 //   warp 1      allocates tensor memory; one thread issues the tcgen05.mma's: smallest products first
 //   warps 2, 3  idle; this warpgroup gives most of its registers to the others
-//   warps 4..11 epilogue: every 24 instructions' worth of products (a chunk) they add the accumulator from tensor memory
-//               to registers, two accumulators taking turns so that the MMAs never wait; at the end of a tile the sums pass
+//   warps 4..11 epilogue: after every K-block they add the accumulator from tensor memory to registers, two accumulators taking turns so that the MMAs never wait; at the end of a tile the sums pass
 //               through a small shared-memory tile per warp, so that global memory is read and written along rows
 // With CG = 2 two CTAs of a cluster share a 256 x 256 tile: each loads its 128 rows of A and its half of B, the first CTA
 // issues the instructions for both.  Shared memory feeds 64 bytes per cycle to the tensor cores then, instead of the 128 of
@@ -36,14 +35,13 @@ struct SplitShape {
     static constexpr int kStageBytes = P * (kABytes + kBBytes);
     static constexpr int kEpilogueBytes = 8 * 32 * kSpStageCols * 4;
     static constexpr int kStages = (232448 - 1024 - kEpilogueBytes) / kStageBytes < 4 ? (232448 - 1024 - kEpilogueBytes) / kStageBytes : 4;
-    static constexpr int kChunkBlocks = P == 3 ? 1 : 2;                  // K-blocks per accumulator: 24 instructions
     static constexpr size_t kSmem = (size_t)kStages * kStageBytes + kEpilogueBytes + 256;
     static_assert(kStages >= 2, "two stages at least");
 };
 
 struct SplitArgs {
     int64_t m, n;
-    int kblocks;
+    int kblocks, chunk;                         // K-blocks; how many of them the large products' accumulator takes
     int64_t tiles_m, tiles_n, n_tiles;          // n_tiles counts all batch entries
     int64_t batch;
     int a_k_major, b_k_major;
@@ -83,16 +81,22 @@ __device__ __forceinline__ void split_commit(uint64_t* bar) {
                      ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
 }
 
-// mbar_wait for barriers that the other CTA of the pair arrives at
-__device__ __forceinline__ bool mbar_wait_pair(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+// Bounded waits that let the hardware hold the thread until the phase ends (at most 2 microseconds a try: half a second in all):
+// an accumulator's turn is under a microsecond, and the sleeping poll of tc_common.cuh wakes too late for it.
+constexpr uint32_t kTries = 1u << 18;
+template <bool PAIR>
+__device__ __forceinline__ bool split_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
     const uint32_t addr = smem_u32(bar);
-    for (uint32_t spin = 0; spin < kSpinLimit; ++spin) {
+    for (uint32_t t = 0; t < kTries; ++t) {
         uint32_t done;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(done) : "r"(addr), "r"(parity) : "memory");
+        if constexpr (PAIR)                                      // barriers that the other CTA of the pair arrives at
+            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                         : "=r"(done) : "r"(addr), "r"(parity), "r"(2000u) : "memory");
+        else
+            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                         : "=r"(done) : "r"(addr), "r"(parity), "r"(2000u) : "memory");
         if (done) return true;
-        if (spin > 16) __nanosleep(32);
-        if ((spin & 255u) == 255u && *abort_flag) return false;
+        if ((t & 63u) == 63u && *abort_flag) return false;
     }
     *abort_flag = 1;
     return false;
@@ -236,8 +240,10 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
     uint64_t* bars = reinterpret_cast<uint64_t*>(base + S::kStages * S::kStageBytes + S::kEpilogueBytes);
     uint64_t* full = bars;                          // [4] TMA -> MMA
     uint64_t* empty = bars + 4;                     // [4] MMA -> TMA
-    uint64_t* acc_full = bars + 8;                  // [2] MMA -> epilogue
-    uint64_t* acc_empty = bars + 10;                // [2] epilogue -> MMA, 8 warps of each CTA
+    uint64_t* main_full = bars + 8;                 // MMA -> epilogue
+    uint64_t* main_empty = bars + 9;                // epilogue -> MMA, 8 warps of each CTA
+    uint64_t* cross_full = bars + 10;
+    uint64_t* cross_empty = bars + 11;
     uint64_t* drain = bars + 12;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -247,7 +253,8 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
     const bool misplaced = (smem_u32(base) & 1023u) != 0;       // the same in every CTA; nothing is launched into it then
     if (tid == 0) {
         for (int i = 0; i < 4; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(acc_full + i, 1); mbar_init(acc_empty + i, 8 * CG); }
+        mbar_init(main_full, 1); mbar_init(cross_full, 1);
+        mbar_init(main_empty, 8 * CG); mbar_init(cross_empty, 8 * CG);
         mbar_init(drain, 1);
         abort_flag[0] = misplaced ? 1 : 0;
         abort_flag[1] = 0;                                       // never set: what the last waits poll
@@ -310,7 +317,7 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
                 const int end = (piece + 1) * g.per_split < g.kblocks ? (piece + 1) * g.per_split : g.kblocks;
                 for (int kb = piece * g.per_split; kb < end; ++kb, ++it) {
                     const uint32_t slot = it % S::kStages;
-                    if (!mbar_wait(empty + slot, ((it / S::kStages) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                    if (!split_wait<false>(empty + slot, ((it / S::kStages) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
                     if (rank == 0) mbar_expect_tx(full + slot, (uint32_t)(S::kStageBytes * CG));
                     const uint32_t bar = CG == 2 ? in_cta(smem_u32(full + slot), 0) : smem_u32(full + slot);
                     uint32_t dst = smem_u32(base + slot * S::kStageBytes);
@@ -343,49 +350,59 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
             uint32_t it = 0, item = 0;
             bool ok = true;
             const uint32_t a_step = g.a_k_major ? 32u : 2048u, b_step = g.b_k_major ? 32u : 2048u;     // bytes per 16 of K
+            constexpr int kTerms = P == 3 ? 6 : 3;
+            constexpr int ta[6] = {P == 3 ? 2 : 1, 0, P == 3 ? 1 : 0, 1, 0, 0};
+            constexpr int tb[6] = {0, P == 3 ? 2 : 1, P == 3 ? 1 : 0, 0, 1, 0};
+            // terms [t0, t1) of a stage; `fresh`: the first instruction starts the accumulator anew
+            auto issue = [&](uint32_t sa, uint32_t sb, uint32_t d_tmem, int t0, int t1, bool fresh) {
+#pragma unroll
+                for (int term = 0; term < kTerms; ++term) {
+                    if (term < t0 || term >= t1) continue;
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) {
+                        const uint32_t aa = sa + ta[term] * S::kABytes + ks * a_step, bb = sb + tb[term] * S::kBBytes + ks * b_step;
+                        const uint64_t da = g.a_k_major ? umma_desc(aa) : umma_desc_mn(aa);
+                        const uint64_t db = g.b_k_major ? umma_desc(bb) : umma_desc_mn(bb);
+                        const uint32_t accumulate = fresh && term == t0 && ks == 0 ? 0u : 1u;
+                        if constexpr (CG == 1)
+                            asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                                         ::"r"(d_tmem), "l"(da), "l"(db), "r"(g.idesc), "r"(accumulate) : "memory");
+                        else
+                            asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                                         ::"r"(d_tmem), "l"(da), "l"(db), "r"(g.idesc), "r"(accumulate) : "memory");
+                    }
+                }
+            };
             for (int64_t t = 0; t < my_tiles && ok; ++t) {
                 const int piece = (int)((cluster + t * clusters) % g.splits);
-                const int end = (piece + 1) * g.per_split < g.kblocks ? (piece + 1) * g.per_split : g.kblocks;
-                for (int kb0 = piece * g.per_split; kb0 < end && ok; kb0 += S::kChunkBlocks, ++item) {
-                    const uint32_t acc = item & 1u;
-                    if (!mbar_wait_pair(acc_empty + acc, ((item >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                const int begin = piece * g.per_split, end = (piece + 1) * g.per_split < g.kblocks ? (piece + 1) * g.per_split : g.kblocks;
+                int in_chunk = 0;
+                for (int kb = begin; kb < end; ++kb, ++it) {
+                    const uint32_t slot = it % S::kStages;
+                    if (!split_wait<false>(full + slot, (it / S::kStages) & 1u, abort_flag)) { ok = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t d_tmem = tmem_base + acc * (uint32_t)BN;
-                    const int kb1 = kb0 + S::kChunkBlocks < end ? kb0 + S::kChunkBlocks : end;
-                    for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                        const uint32_t slot = it % S::kStages;
-                        if (!mbar_wait(full + slot, (it / S::kStages) & 1u, abort_flag)) { ok = false; break; }
+                    const uint32_t sa = smem_u32(base + slot * S::kStageBytes), sb = sa + P * S::kABytes;
+                    // a tile's first block starts with the large products, whose accumulator the epilogue hands back first
+                    if (kb > begin) issue(sa, sb, tmem_base + BN, 0, kTerms - 1, false);
+                    if (in_chunk == 0) {
+                        if (!split_wait<CG == 2>(main_empty, (item & 1u) ^ 1u, abort_flag)) { ok = false; break; }
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint32_t sa = smem_u32(base + slot * S::kStageBytes), sb = sa + P * S::kABytes;
-                        constexpr int kTerms = P == 3 ? 6 : 3;
-                        constexpr int ta[6] = {P == 3 ? 2 : 1, 0, P == 3 ? 1 : 0, 1, 0, 0};
-                        constexpr int tb[6] = {0, P == 3 ? 2 : 1, P == 3 ? 1 : 0, 0, 1, 0};
-#pragma unroll
-                        for (int term = 0; term < kTerms; ++term) {
-#pragma unroll
-                            for (int ks = 0; ks < 4; ++ks) {
-                                const uint32_t aa = sa + ta[term] * S::kABytes + ks * a_step, bb = sb + tb[term] * S::kBBytes + ks * b_step;
-                                const uint64_t da = g.a_k_major ? umma_desc(aa) : umma_desc_mn(aa);
-                                const uint64_t db = g.b_k_major ? umma_desc(bb) : umma_desc_mn(bb);
-                                const uint32_t accumulate = (uint32_t)((kb - kb0) | term | ks) != 0;
-                                if constexpr (CG == 1)
-                                    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                                                 ::"r"(d_tmem), "l"(da), "l"(db), "r"(g.idesc), "r"(accumulate) : "memory");
-                                else
-                                    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                                                 ::"r"(d_tmem), "l"(da), "l"(db), "r"(g.idesc), "r"(accumulate) : "memory");
-                            }
-                        }
-                        split_commit<CG>(empty + slot);
                     }
-                    if (!ok) break;
-                    split_commit<CG>(acc_full + acc);
+                    issue(sa, sb, tmem_base, kTerms - 1, kTerms, in_chunk == 0);
+                    if (kb == begin) {
+                        if (!split_wait<CG == 2>(cross_empty, ((uint32_t)t & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        issue(sa, sb, tmem_base + BN, 0, kTerms - 1, true);
+                    }
+                    split_commit<CG>(empty + slot);
+                    if (++in_chunk == g.chunk || kb + 1 == end) { split_commit<CG>(main_full); in_chunk = 0; ++item; }
                 }
+                if (ok) split_commit<CG>(cross_full);
             }
             // what was issued finishes before tensor memory is freed, whatever happened above
             if constexpr (CG == 1) asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(drain)) : "memory");
             else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(drain)) : "memory");
-            mbar_wait(drain, 0u, abort_flag + 1);
+            split_wait<false>(drain, 0u, abort_flag + 1);
         }
         __syncwarp();
     }
@@ -405,12 +422,17 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
             int part;
             tile_of(t, &batch, &i0, &j0, &part);
             const int blocks = (part + 1) * g.per_split < g.kblocks ? g.per_split : g.kblocks - part * g.per_split;
-            const uint32_t chunks = (uint32_t)((blocks + S::kChunkBlocks - 1) / S::kChunkBlocks);
-            for (uint32_t c = 0; c < chunks; ++c, ++item) {
-                const uint32_t acc = item & 1u;
-                if (!__all_sync(0xffffffffu, mbar_wait(acc_full + acc, (item >> 1) & 1u, abort_flag))) { ok = false; break; }
+            const uint32_t chunks = (uint32_t)((blocks + g.chunk - 1) / g.chunk);
+#pragma unroll
+            for (int x = 0; x < kCols; ++x) sum[x] = 0.f;
+            // the chunks of large products, then the small ones
+#pragma unroll 1
+            for (uint32_t c = 0; c <= chunks; ++c) {
+                const bool cross = c == chunks;
+                uint64_t* bar = cross ? cross_full : main_full;
+                if (!__all_sync(0xffffffffu, split_wait<false>(bar, (cross ? (uint32_t)t : item) & 1u, abort_flag))) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t taddr = tmem_base + acc * (uint32_t)BN + (uint32_t)(half * kCols) + ((quarter * 32u) << 16);
+                const uint32_t taddr = tmem_base + (cross ? (uint32_t)BN : 0u) + (uint32_t)(half * kCols) + ((quarter * 32u) << 16);
                 // 16 columns are added while the next 16 are on their way
                 uint32_t ra[16], rb[16];
                 tmem_ld16(taddr, ra);
@@ -419,19 +441,21 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
                 for (int q = 0; q < kCols / 16; q += 2) {
                     tmem_ld16(taddr + (q + 1) * 16u, rb);
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) sum[q * 16 + x] = c == 0 ? __uint_as_float(ra[x]) : sum[q * 16 + x] + __uint_as_float(ra[x]);
+                    for (int x = 0; x < 16; ++x) sum[q * 16 + x] += __uint_as_float(ra[x]);
                     tmem_ld_wait(rb);
                     if (q + 2 < kCols / 16) tmem_ld16(taddr + (q + 2) * 16u, ra);
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) sum[q * 16 + 16 + x] = c == 0 ? __uint_as_float(rb[x]) : sum[q * 16 + 16 + x] + __uint_as_float(rb[x]);
+                    for (int x = 0; x < 16; ++x) sum[q * 16 + 16 + x] += __uint_as_float(rb[x]);
                     if (q + 2 < kCols / 16) tmem_ld_wait(ra);
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
-                    if constexpr (CG == 1) mbar_arrive(acc_empty + acc);
-                    else asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_cta(smem_u32(acc_empty + acc), 0)) : "memory");
+                    uint64_t* back = cross ? cross_empty : main_empty;
+                    if constexpr (CG == 1) mbar_arrive(back);
+                    else asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_cta(smem_u32(back), 0)) : "memory");
                 }
+                if (!cross) ++item;
             }
             if (!ok) break;
             const int64_t row0 = i0 + (int64_t)quarter * 32, col0 = j0 + half * kCols;
@@ -512,6 +536,9 @@ static int launch_shape(SplitKind kind, const Planes& a, const Planes& b, const 
     g.kblocks = (int)((a.k + kSpKB - 1) / kSpKB);
     g.tiles_m = (a.rows + 128 * CG - 1) / (128 * CG);
     g.tiles_n = (b.rows + BN - 1) / BN;
+    // Half pairs feed products whose errors add up over an iteration: short sums, whose own rounding is small, take the finest
+    // chunks (four truncating additions); longer ones, and the three-part products of a single layer, sixteen.
+    g.chunk = kind == kSplitHalfx2 && g.kblocks <= 16 ? 1 : 4;
     g.symmetric = symmetric && BN == 128 * CG;
     g.per_split = (g.kblocks + splits - 1) / splits;
     g.splits = (g.kblocks + g.per_split - 1) / g.per_split;             // no piece is empty

@@ -5,8 +5,9 @@
 //     a b = a1 b1 + (a1 b2 + a2 b1) + (a2 b2 + a1 b3 + a3 b1) + terms of 2^-24 a b and below,
 // six bfloat16 products; with two half-precision parts a1 b1 + (a1 b2 + a2 b1), three products.  Products of two 16-bit
 // numbers are exact in the tensor core; what it adds them into is 32 bits wide but truncates, an error that leans one way and
-// grows with the number of additions (2e-8 of the accumulator each, measured), so an accumulator takes 24 instructions'
-// worth of them at most and is then added into registers with ordinary rounded additions.
+// grows with the number of additions (2e-8 of the accumulator each, measured).  So the large products a1 b1 have an
+// accumulator of their own, which takes at most 256 of K -- sixteen additions -- before it is added into registers with
+// ordinary rounded additions; what truncation does to the accumulator of the small products is 2^-8 of that and less.
 #pragma once
 
 #include "linear.cuh"
@@ -57,13 +58,28 @@ struct SplitSource {
     int act;
 };
 
-// The R x C source as three bfloat16 planes, [plane][R][ld].
-int launch_split(const SplitSource& s, int64_t R, int64_t C, uint16_t* planes, int64_t ld, const Marks& marks, cudaStream_t st);
+// R x C sources as three bfloat16 planes each, [plane][R][ld]; up to three in one launch.
+struct SplitJob {
+    SplitSource s;
+    int64_t R, C, ld;
+    uint16_t* planes;
+    Marks marks;
+};
+struct SplitJobs { SplitJob job[3]; int count; };
+int launch_split(const SplitJobs& jobs, cudaStream_t st);
 
 // Outputs i, j with a[i] or b[j] marked, in float from the operands: element (row, k) of A at (row, k) of `a`, or (k, row)
-// if a_turned; B alike.  Returns at once on the device when nothing was marked.
-int launch_fix_marked(int64_t m, int64_t n, int64_t k, const SplitSource& a, bool a_turned, const uint8_t* a_marks, const SplitSource& b, bool b_turned,
-                      const uint8_t* b_marks, const int* any, const Epilogue<float>& e, cudaStream_t st);
+// if a_turned; B alike.  Returns at once on the device when nothing was marked.  Up to two products in one launch.
+struct FixJob {
+    int64_t m, n, k;
+    SplitSource a, b;
+    bool a_turned, b_turned;
+    const uint8_t* a_marks;
+    const uint8_t* b_marks;
+    Epilogue<float> e;
+};
+struct FixJobs { FixJob job[2]; int count; const int* any; };
+int launch_fix_marked(const FixJobs& jobs, cudaStream_t st);
 
 // 0, or cudaErrorLaunchTimeout once a bounded wait inside a product has run out on this device (see cb200_product_status).
 int product_gave_up();

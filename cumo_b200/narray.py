@@ -20,7 +20,11 @@ from . import _lib
 
 SFLOAT, DFLOAT, INT32, INT64, BIT, UINT64, UINT32 = range(7)
 _NP = {SFLOAT: np.float32, DFLOAT: np.float64, INT32: np.int32, INT64: np.int64, UINT64: np.uint64, UINT32: np.uint32}
+_TORCH = {}                                                          # element types of torch, once it is there
 _ESZ = {SFLOAT: 4, DFLOAT: 8, INT32: 4, INT64: 8, BIT: 1, UINT64: 8, UINT32: 4}   # Bit: unit is one bit
+
+
+_TYPESTR = {code: np.dtype(t).str for code, t in _NP.items()}
 
 
 class CumoError(Exception):
@@ -166,12 +170,13 @@ class NArray:
         """Borrow a CUDA tensor's memory (no copy); the tensor is kept alive by the view."""
         import torch
 
-        want = {SFLOAT: torch.float32, DFLOAT: torch.float64, INT32: torch.int32, INT64: torch.int64}[cls.dtype_code]
+        if not _TORCH:
+            _TORCH.update({SFLOAT: torch.float32, DFLOAT: torch.float64, INT32: torch.int32, INT64: torch.int64})
+        want = _TORCH[cls.dtype_code]
         if t.dtype != want or not t.is_cuda:
             raise TypeError(f"{cls.__name__}.from_torch needs a CUDA tensor of {want}")
-        es = t.element_size()
-        h = _lib.load().cb200_na_wrap(cls.dtype_code, t.dim(), _arr64(list(t.shape)),
-                                      _arr64([s * es for s in t.stride()]), c_void_p(t.data_ptr()), 0)
+        es, shape = _ESZ[cls.dtype_code], t.shape
+        h = _lib.load().cb200_na_wrap(cls.dtype_code, len(shape), _arr64(shape), _arr64([s * es for s in t.stride()]), t.data_ptr(), 0)
         return NArray._from_handle(h, keep=t)
 
     @classmethod
@@ -325,8 +330,11 @@ class NArray:
     def __cuda_array_interface__(self):
         if self.dtype_code == BIT:
             raise TypeError("a Bit array has no element-addressable interface")
-        return {"shape": self.shape, "typestr": np.dtype(_NP[self.dtype_code]).str, "data": (self.data_ptr, False),
-                "version": 3, "strides": self.steps if not self.contiguous() else None}
+        n, lib = self.ndim, _lib.load()
+        shape, steps = (c_int64 * max(1, n))(), (c_int64 * max(1, n))()
+        lib.cb200_na_shape(self._h, shape)
+        lib.cb200_na_steps(self._h, steps)
+        return {"shape": tuple(shape[:n]), "typestr": _TYPESTR[self.dtype_code], "data": (self.data_ptr, False), "version": 3, "strides": tuple(steps[:n])}
 
     # ---- host copies ------------------------------------------------------------------------------
     def to_numpy(self) -> np.ndarray:
