@@ -35,6 +35,8 @@ struct SplitShape {
     static constexpr int kStageBytes = P * (kABytes + kBBytes);
     static constexpr int kEpilogueBytes = 8 * 32 * kSpStageCols * 4;
     static constexpr int kStages = (232448 - 1024 - kEpilogueBytes) / kStageBytes < 4 ? (232448 - 1024 - kEpilogueBytes) / kStageBytes : 4;
+    static constexpr int kMains = BN == 256 ? 1 : 2;                     // accumulators of large products, taking turns where there is room
+    static constexpr uint32_t kTmemCols = BN == 64 ? 256 : 512;          // kMains + 1 accumulators of BN columns, a power of two
     static constexpr size_t kSmem = (size_t)kStages * kStageBytes + kEpilogueBytes + 256;
     static_assert(kStages >= 2, "two stages at least");
 };
@@ -102,15 +104,51 @@ __device__ __forceinline__ bool split_wait(uint64_t* bar, uint32_t parity, volat
     return false;
 }
 
-// MN-major, 128-byte swizzle: 8 rows of k (1024 bytes) per group, next 64 elements of the row axis 8192 bytes on
-__device__ __forceinline__ uint64_t umma_desc_mn(uint32_t saddr) {
-    uint64_t d = 0;
-    d |= (uint64_t)((saddr & 0x3ffffu) >> 4);
-    d |= (uint64_t)(8192u >> 4) << 16;
-    d |= (uint64_t)(1024u >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
+// ---- issuing the products -----------------------------------------------------------------------------------------------
+// One thread issues them all, so what it computes per instruction is time the tensor cores wait (measured: building both
+// 64-bit descriptors each time made every instruction take 130 to 190 cycles, whatever its shape).  A descriptor's upper half is
+// constant and its lower half a stage's base plus an offset known at compile time: the layouts are template arguments.
+//   K-major: rows of 128 bytes, 16 of K are 32 bytes on.  MN-major: 8 rows of k (1024 bytes) per group, 16 of K are 2048
+//   bytes on, the next 64 elements of the row axis 8192 (the leading byte offset, in the lower half).
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);      // stride byte offset, version, 128-byte swizzle
+template <bool K_MAJOR>
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr) { return ((saddr & 0x3ffffu) >> 4) | ((K_MAJOR ? 1u : 8192u >> 4) << 16); }
+
+template <int CG, bool FRESH>
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint32_t a_low, uint32_t b_low, uint32_t idesc) {
+    const uint64_t da = (uint64_t)kDescHigh << 32 | a_low, db = (uint64_t)kDescHigh << 32 | b_low;
+    if constexpr (CG == 1)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d_tmem), "l"(da), "l"(db), "r"(idesc), "n"(FRESH ? 0 : 1) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d_tmem), "l"(da), "l"(db), "r"(idesc), "n"(FRESH ? 0 : 1) : "memory");
+}
+
+// The large product of a stage (MAIN) or all its small ones, 64 of K; FRESH: the first instruction starts the accumulator anew.
+template <int P, int CG, int A_BYTES, int B_BYTES, bool AK, bool BK, bool MAIN, bool FRESH>
+__device__ __forceinline__ void issue_stage(uint32_t sa, uint32_t sb, uint32_t d_tmem, uint32_t idesc) {
+    constexpr int kTerms = P == 3 ? 6 : 3;
+    constexpr int ta[6] = {P == 3 ? 2 : 1, 0, P == 3 ? 1 : 0, 1, 0, 0};
+    constexpr int tb[6] = {0, P == 3 ? 2 : 1, P == 3 ? 1 : 0, 0, 1, 0};
+    const uint32_t a0 = desc_low<AK>(sa), b0 = desc_low<BK>(sb);
+#pragma unroll
+    for (int term = MAIN ? kTerms - 1 : 0; term < (MAIN ? kTerms : kTerms - 1); ++term)
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            const uint32_t a = a0 + ((ta[term] * A_BYTES + ks * (AK ? 32 : 2048)) >> 4), b = b0 + ((tb[term] * B_BYTES + ks * (BK ? 32 : 2048)) >> 4);
+            if (FRESH && term == (MAIN ? kTerms - 1 : 0) && ks == 0) mma_f16<CG, true>(d_tmem, a, b, idesc);
+            else mma_f16<CG, false>(d_tmem, a, b, idesc);
+        }
+}
+template <int P, int CG, int A_BYTES, int B_BYTES, bool MAIN, bool FRESH>
+__device__ __forceinline__ void issue(int layout, uint32_t sa, uint32_t sb, uint32_t d_tmem, uint32_t idesc) {
+    switch (layout) {                                            // bit 0: A K-major, bit 1: B K-major
+        case 0: issue_stage<P, CG, A_BYTES, B_BYTES, false, false, MAIN, FRESH>(sa, sb, d_tmem, idesc); break;
+        case 1: issue_stage<P, CG, A_BYTES, B_BYTES, true, false, MAIN, FRESH>(sa, sb, d_tmem, idesc); break;
+        case 2: issue_stage<P, CG, A_BYTES, B_BYTES, false, true, MAIN, FRESH>(sa, sb, d_tmem, idesc); break;
+        default: issue_stage<P, CG, A_BYTES, B_BYTES, true, true, MAIN, FRESH>(sa, sb, d_tmem, idesc); break;
+    }
 }
 
 // Out: how a finished 32-row x 32-column piece leaves shared memory.  Loads are issued ahead of the stores that they might
@@ -240,12 +278,12 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
     uint64_t* bars = reinterpret_cast<uint64_t*>(base + S::kStages * S::kStageBytes + S::kEpilogueBytes);
     uint64_t* full = bars;                          // [4] TMA -> MMA
     uint64_t* empty = bars + 4;                     // [4] MMA -> TMA
-    uint64_t* main_full = bars + 8;                 // MMA -> epilogue
-    uint64_t* main_empty = bars + 9;                // epilogue -> MMA, 8 warps of each CTA
-    uint64_t* cross_full = bars + 10;
-    uint64_t* cross_empty = bars + 11;
-    uint64_t* drain = bars + 12;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
+    uint64_t* main_full = bars + 8;                 // [2] MMA -> epilogue
+    uint64_t* main_empty = bars + 10;               // [2] epilogue -> MMA, 8 warps of each CTA
+    uint64_t* cross_full = bars + 12;
+    uint64_t* cross_empty = bars + 13;
+    uint64_t* drain = bars + 14;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -253,8 +291,9 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
     const bool misplaced = (smem_u32(base) & 1023u) != 0;       // the same in every CTA; nothing is launched into it then
     if (tid == 0) {
         for (int i = 0; i < 4; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
-        mbar_init(main_full, 1); mbar_init(cross_full, 1);
-        mbar_init(main_empty, 8 * CG); mbar_init(cross_empty, 8 * CG);
+        for (int i = 0; i < 2; ++i) { mbar_init(main_full + i, 1); mbar_init(main_empty + i, 8 * CG); }
+        mbar_init(cross_full, 1);
+        mbar_init(cross_empty, 8 * CG);
         mbar_init(drain, 1);
         abort_flag[0] = misplaced ? 1 : 0;
         abort_flag[1] = 0;                                       // never set: what the last waits poll
@@ -263,10 +302,10 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
     __syncthreads();
     if (warp == 1) {
         if constexpr (CG == 1) {
-            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)(2 * BN)) : "memory");
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(S::kTmemCols) : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         } else {
-            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)(2 * BN)) : "memory");
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(S::kTmemCols) : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
         }
     }
@@ -349,30 +388,7 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
         if (lane == 0 && rank == 0) {
             uint32_t it = 0, item = 0;
             bool ok = true;
-            const uint32_t a_step = g.a_k_major ? 32u : 2048u, b_step = g.b_k_major ? 32u : 2048u;     // bytes per 16 of K
-            constexpr int kTerms = P == 3 ? 6 : 3;
-            constexpr int ta[6] = {P == 3 ? 2 : 1, 0, P == 3 ? 1 : 0, 1, 0, 0};
-            constexpr int tb[6] = {0, P == 3 ? 2 : 1, P == 3 ? 1 : 0, 0, 1, 0};
-            // terms [t0, t1) of a stage; `fresh`: the first instruction starts the accumulator anew
-            auto issue = [&](uint32_t sa, uint32_t sb, uint32_t d_tmem, int t0, int t1, bool fresh) {
-#pragma unroll
-                for (int term = 0; term < kTerms; ++term) {
-                    if (term < t0 || term >= t1) continue;
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) {
-                        const uint32_t aa = sa + ta[term] * S::kABytes + ks * a_step, bb = sb + tb[term] * S::kBBytes + ks * b_step;
-                        const uint64_t da = g.a_k_major ? umma_desc(aa) : umma_desc_mn(aa);
-                        const uint64_t db = g.b_k_major ? umma_desc(bb) : umma_desc_mn(bb);
-                        const uint32_t accumulate = fresh && term == t0 && ks == 0 ? 0u : 1u;
-                        if constexpr (CG == 1)
-                            asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                                         ::"r"(d_tmem), "l"(da), "l"(db), "r"(g.idesc), "r"(accumulate) : "memory");
-                        else
-                            asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                                         ::"r"(d_tmem), "l"(da), "l"(db), "r"(g.idesc), "r"(accumulate) : "memory");
-                    }
-                }
-            };
+            const int layout = (g.a_k_major ? 1 : 0) | (g.b_k_major ? 2 : 0);
             for (int64_t t = 0; t < my_tiles && ok; ++t) {
                 const int piece = (int)((cluster + t * clusters) % g.splits);
                 const int begin = piece * g.per_split, end = (piece + 1) * g.per_split < g.kblocks ? (piece + 1) * g.per_split : g.kblocks;
@@ -383,19 +399,22 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t sa = smem_u32(base + slot * S::kStageBytes), sb = sa + P * S::kABytes;
                     // a tile's first block starts with the large products, whose accumulator the epilogue hands back first
-                    if (kb > begin) issue(sa, sb, tmem_base + BN, 0, kTerms - 1, false);
+                    constexpr uint32_t kCross = S::kMains * BN;
+                    const uint32_t which = item % S::kMains, turn = item / S::kMains;
+                    if (kb > begin) issue<P, CG, S::kABytes, S::kBBytes, false, false>(layout, sa, sb, tmem_base + kCross, g.idesc);
                     if (in_chunk == 0) {
-                        if (!split_wait<CG == 2>(main_empty, (item & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                        if (!split_wait<CG == 2>(main_empty + which, (turn & 1u) ^ 1u, abort_flag)) { ok = false; break; }
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     }
-                    issue(sa, sb, tmem_base, kTerms - 1, kTerms, in_chunk == 0);
+                    if (in_chunk == 0) issue<P, CG, S::kABytes, S::kBBytes, true, true>(layout, sa, sb, tmem_base + which * BN, g.idesc);
+                    else issue<P, CG, S::kABytes, S::kBBytes, true, false>(layout, sa, sb, tmem_base + which * BN, g.idesc);
                     if (kb == begin) {
                         if (!split_wait<CG == 2>(cross_empty, ((uint32_t)t & 1u) ^ 1u, abort_flag)) { ok = false; break; }
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        issue(sa, sb, tmem_base + BN, 0, kTerms - 1, true);
+                        issue<P, CG, S::kABytes, S::kBBytes, false, true>(layout, sa, sb, tmem_base + kCross, g.idesc);
                     }
                     split_commit<CG>(empty + slot);
-                    if (++in_chunk == g.chunk || kb + 1 == end) { split_commit<CG>(main_full); in_chunk = 0; ++item; }
+                    if (++in_chunk == g.chunk || kb + 1 == end) { split_commit<CG>(main_full + which); in_chunk = 0; ++item; }
                 }
                 if (ok) split_commit<CG>(cross_full);
             }
@@ -429,10 +448,11 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
 #pragma unroll 1
             for (uint32_t c = 0; c <= chunks; ++c) {
                 const bool cross = c == chunks;
-                uint64_t* bar = cross ? cross_full : main_full;
-                if (!__all_sync(0xffffffffu, split_wait<false>(bar, (cross ? (uint32_t)t : item) & 1u, abort_flag))) { ok = false; break; }
+                const uint32_t which = item % S::kMains, turn = item / S::kMains;
+                uint64_t* bar = cross ? cross_full : main_full + which;
+                if (!__all_sync(0xffffffffu, split_wait<false>(bar, (cross ? (uint32_t)t : turn) & 1u, abort_flag))) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t taddr = tmem_base + (cross ? (uint32_t)BN : 0u) + (uint32_t)(half * kCols) + ((quarter * 32u) << 16);
+                const uint32_t taddr = tmem_base + (cross ? S::kMains : which) * (uint32_t)BN + (uint32_t)(half * kCols) + ((quarter * 32u) << 16);
                 // 16 columns are added while the next 16 are on their way
                 uint32_t ra[16], rb[16];
                 tmem_ld16(taddr, ra);
@@ -451,7 +471,7 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
-                    uint64_t* back = cross ? cross_empty : main_empty;
+                    uint64_t* back = cross ? cross_empty : main_empty + which;
                     if constexpr (CG == 1) mbar_arrive(back);
                     else asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_cta(smem_u32(back), 0)) : "memory");
                 }
@@ -476,8 +496,8 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
     if constexpr (CG == 2) cluster_sync_all();                     // neither CTA leaves while the other may still arrive at its barriers
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (warp == 1) {
-        if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)(2 * BN)) : "memory");
-        else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)(2 * BN)) : "memory");
+        if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::kTmemCols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::kTmemCols) : "memory");
     }
     if ((abort_flag[0] | abort_flag[1]) && tid == 0) *reinterpret_cast<volatile int*>(g.gave_up) = 1;
 }
@@ -536,9 +556,9 @@ static int launch_shape(SplitKind kind, const Planes& a, const Planes& b, const 
     g.kblocks = (int)((a.k + kSpKB - 1) / kSpKB);
     g.tiles_m = (a.rows + 128 * CG - 1) / (128 * CG);
     g.tiles_n = (b.rows + BN - 1) / BN;
-    // Half pairs feed products whose errors add up over an iteration: short sums, whose own rounding is small, take the finest
-    // chunks (four truncating additions); longer ones, and the three-part products of a single layer, sixteen.
-    g.chunk = kind == kSplitHalfx2 && g.kblocks <= 16 ? 1 : 4;
+    // Half pairs feed products whose errors add up over an iteration: short sums, whose own rounding is small, take finer
+    // chunks (four truncating additions per block); longer ones, and the three-part products of a single layer, sixteen.
+    g.chunk = kind != kSplitHalfx2 || g.kblocks > 16 ? 4 : g.kblocks > 4 ? 2 : 1;
     g.symmetric = symmetric && BN == 128 * CG;
     g.per_split = (g.kblocks + splits - 1) / splits;
     g.splits = (g.kblocks + g.per_split - 1) / g.per_split;             // no piece is empty
