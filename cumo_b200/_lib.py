@@ -68,6 +68,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "cb200_na_size": (c_int64, [H]),
         "cb200_na_shape": (None, [H, P64]),
         "cb200_na_steps": (None, [H, P64]),
+        "cb200_na_facts": (None, [H, P64]),
         "cb200_na_offset": (c_int64, [H]),
         "cb200_na_base": (c_void_p, [H]),
         "cb200_na_is_contiguous": (c_int, [H]),

@@ -551,6 +551,12 @@ int cb200_na_ndim(const cb200_na_t* a) { return a->ndim; }
 int64_t cb200_na_size(const cb200_na_t* a) { return size_of(a); }
 void cb200_na_shape(const cb200_na_t* a, int64_t* shape) { memcpy(shape, a->shape, sizeof(int64_t) * a->ndim); }
 void cb200_na_steps(const cb200_na_t* a, int64_t* step) { memcpy(step, a->step, sizeof(int64_t) * a->ndim); }
+void cb200_na_facts(const cb200_na_t* a, int64_t* out) {
+    *out++ = a->ndim;
+    *out++ = (int64_t)(intptr_t)(a->dtype == CB200_BIT ? a->st->ptr : data_ptr(a));
+    for (int d = 0; d < a->ndim; ++d) *out++ = a->shape[d];
+    for (int d = 0; d < a->ndim; ++d) *out++ = a->step[d];
+}
 int64_t cb200_na_offset(const cb200_na_t* a) { return a->offset; }
 void* cb200_na_base(const cb200_na_t* a) { return a->st->ptr; }
 int cb200_na_is_contiguous(const cb200_na_t* a) { return is_contiguous(a) ? 1 : 0; }

@@ -10,7 +10,9 @@ namespace cb200 {
 
 // ---- the product on the CUDA cores ------------------------------------------------------------------------------------
 // 64 x 64 outputs per CTA, 4 x 4 per thread, 16 of K at a time through shared memory.  Lanes run along whichever axis of
-// each operand is contiguous.  Bound by the FMA rate at large sizes and by latency at small ones.
+// each operand is contiguous.  Every 64 of K the sums so far are put aside and new ones begun: the error of a long sum in
+// 32 bits then grows with the square root of its number of pieces, not of its terms.  Bound by the FMA rate at large sizes and by
+// latency at small ones.
 constexpr int kPcM = 64, kPcN = 64, kPcK = 16, kPcPad = 4;
 
 template <typename T>
@@ -25,11 +27,11 @@ product_cc_kernel(int64_t m, int64_t n, int64_t k, const Operand<T> A, const Ope
     const int ti = threadIdx.x / 16, tj = threadIdx.x % 16;
     const bool a_along_k = A.k == 1, b_along_k = B.k == 1;
     constexpr int PER = kPcM * kPcK / kBlock;
-    T ra[PER], rb[PER], acc[4][4];
+    T ra[PER], rb[PER], acc[4][4], aside[4][4];
 #pragma unroll
     for (int x = 0; x < 4; ++x)
 #pragma unroll
-        for (int y = 0; y < 4; ++y) acc[x][y] = T(0);
+        for (int y = 0; y < 4; ++y) acc[x][y] = aside[x][y] = T(0);
     auto fetch = [&](int64_t k0) {
 #pragma unroll
         for (int s = 0; s < PER; ++s) {
@@ -61,13 +63,19 @@ product_cc_kernel(int64_t m, int64_t n, int64_t k, const Operand<T> A, const Ope
 #pragma unroll
                 for (int y = 0; y < 4; ++y) acc[x][y] = av[x] * bv[y] + acc[x][y];
         }
+        if ((k0 / kPcK & 3) == 3) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) { aside[x][y] += acc[x][y]; acc[x][y] = T(0); }
+        }
     }
 #pragma unroll
     for (int x = 0; x < 4; ++x)
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
             const int64_t i = i0 + ti * 4 + x, j = j0 + tj + 16 * y;
-            if (i < m && j < n) finish(e, batch, i, j, acc[x][y]);
+            if (i < m && j < n) finish(e, batch, i, j, aside[x][y] + acc[x][y]);
         }
 }
 
@@ -223,12 +231,13 @@ struct SplitSet {
 
 static bool worth_splitting(int64_t m, int64_t n, int64_t k) { return m >= 32 && n >= 32 && k >= 32 && m * n * k >= (1LL << 22); }
 
-// The product on the CUDA cores: few rows of A, few rows of B (the same with the sides exchanged is not offered by the
-// epilogue's row-major output, so those take the tiles), or tiles.
+// Few rows ride along with a pass over the weights (16 to a pass).  Measured in SFloat: 64 x 1024 x 1024 26 us against 39
+// split, 33 x 4096 x 4096 105 against 80, so up to 32 rows always and up to 128 while there are under 2^28 products.
+static bool few_rows(int64_t m, int64_t n, int64_t k) { return k >= 16 && (m <= 32 || (m <= 128 && m * n * k <= (1LL << 28))); }
+
 template <typename T>
 static int product(int64_t m, int64_t n, int64_t k, const Operand<T>& a, const Operand<T>& b, const Epilogue<T>& e, cudaStream_t st) {
-    static const int most = getenv("CB_R") ? atoi(getenv("CB_R")) : 32;
-    if (m <= most && k >= 16) return launch_product_rows<T>(m, n, k, a, b, e, st);
+    if (few_rows(m, n, k)) return launch_product_rows<T>(m, n, k, a, b, e, st);
     return launch_product_cc<T>(m, n, k, 1, a, b, e, st);
 }
 
@@ -248,8 +257,7 @@ static int linear(int64_t m, int64_t n, int64_t k, const T* x, ssize_t x_row, ss
     e.res = residual; e.res_row = r_row / es; e.res_col = r_col / es;
     e.y = y; e.ld = n; e.pre = pre;
     if constexpr (sizeof(T) == 4) {
-        static const int most = getenv("CB_R") ? atoi(getenv("CB_R")) : 32;
-        if (m > most && worth_splitting(m, n, k)) {
+        if (!few_rows(m, n, k) && worth_splitting(m, n, k)) {
             const int late = product_gave_up();
             if (late) return late;
             Scratch scratch(current_stream());

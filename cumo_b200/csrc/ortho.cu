@@ -235,7 +235,7 @@ static int orthogonalize(int64_t batch, int64_t rows, int64_t columns, const T* 
     count_launch();
     if constexpr (sizeof(T) == 4) {
         const OrthoScales sc(steps, coefs);
-        if (sc.fits && m >= 32) return orthogonalize_split(batch, m, n, tall, G, steps, coefs, eps, (int)slices, sums, sc, out, scratch, st);
+        if (sc.fits) return orthogonalize_split(batch, m, n, tall, G, steps, coefs, eps, (int)slices, sums, sc, out, scratch, st);
     }
     T* x = reinterpret_cast<T*>(scratch.take((size_t)batch * m * n * es));
     T* x2 = reinterpret_cast<T*>(scratch.take((size_t)batch * m * n * es));

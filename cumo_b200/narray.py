@@ -56,8 +56,12 @@ def _raise_last():
     raise exc((msg or b"").decode())
 
 
+_INT64S = [c_int64 * max(1, n) for n in range(_lib.MAX_DIM + 1)]        # array types by length
+
+
 def _arr64(values):
-    return (c_int64 * max(1, len(values)))(*values)
+    n = len(values)
+    return (_INT64S[n] if n <= _lib.MAX_DIM else c_int64 * n)(*values)
 
 
 def _axis_mask(axis, ndim):
@@ -168,15 +172,14 @@ class NArray:
     @classmethod
     def from_torch(cls, t):
         """Borrow a CUDA tensor's memory (no copy); the tensor is kept alive by the view."""
-        import torch
-
         if not _TORCH:
+            import torch
             _TORCH.update({SFLOAT: torch.float32, DFLOAT: torch.float64, INT32: torch.int32, INT64: torch.int64})
-        want = _TORCH[cls.dtype_code]
-        if t.dtype != want or not t.is_cuda:
-            raise TypeError(f"{cls.__name__}.from_torch needs a CUDA tensor of {want}")
-        es, shape = _ESZ[cls.dtype_code], t.shape
-        h = _lib.load().cb200_na_wrap(cls.dtype_code, len(shape), _arr64(shape), _arr64([s * es for s in t.stride()]), t.data_ptr(), 0)
+        code, shape = cls.dtype_code, t.shape
+        if t.dtype != _TORCH[code] or not t.is_cuda:
+            raise TypeError(f"{cls.__name__}.from_torch needs a CUDA tensor of {_TORCH[code]}")
+        es = _ESZ[code]
+        h = _lib.load().cb200_na_wrap(code, len(shape), _arr64(shape), _arr64([s * es for s in t.stride()]), t.data_ptr(), 0)
         return NArray._from_handle(h, keep=t)
 
     @classmethod
@@ -282,6 +285,13 @@ class NArray:
     def ndim(self):
         return _lib.load().cb200_na_ndim(self._h)
 
+    def _facts(self):
+        """(address of the first element, shape, steps) from one call."""
+        buf = (c_int64 * (2 + 2 * _lib.MAX_DIM))()
+        _lib.load().cb200_na_facts(self._h, buf)
+        n = buf[0]
+        return buf[1], tuple(buf[2:2 + n]), tuple(buf[2 + n:2 + 2 * n])
+
     @property
     def shape(self):
         n = self.ndim
@@ -330,11 +340,8 @@ class NArray:
     def __cuda_array_interface__(self):
         if self.dtype_code == BIT:
             raise TypeError("a Bit array has no element-addressable interface")
-        n, lib = self.ndim, _lib.load()
-        shape, steps = (c_int64 * max(1, n))(), (c_int64 * max(1, n))()
-        lib.cb200_na_shape(self._h, shape)
-        lib.cb200_na_steps(self._h, steps)
-        return {"shape": tuple(shape[:n]), "typestr": _TYPESTR[self.dtype_code], "data": (self.data_ptr, False), "version": 3, "strides": tuple(steps[:n])}
+        ptr, shape, steps = self._facts()
+        return {"shape": shape, "typestr": _TYPESTR[self.dtype_code], "data": (ptr, False), "version": 3, "strides": steps}
 
     # ---- host copies ------------------------------------------------------------------------------
     def to_numpy(self) -> np.ndarray:
