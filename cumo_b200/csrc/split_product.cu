@@ -157,43 +157,65 @@ __device__ __forceinline__ void issue(int layout, uint32_t sa, uint32_t sb, uint
 struct FloatOut {
     Epilogue<float> e;
     bool packets;                      // y (and residual) take 16-byte accesses
-    __device__ __forceinline__ void piece(float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n, bool) const {
+    struct Ahead {};
+    __device__ __forceinline__ void ahead(Ahead&, int, int64_t, int64_t, int64_t, int64_t, int64_t) const {}
+    __device__ __forceinline__ void piece(float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n, bool, const Ahead&) const {
         const int rows = m - i0 < 32 ? (int)(m - i0) : 32;
         const int64_t y0 = batch * e.y_batch + i0 * e.ld + j0;
         const bool whole = packets && rows == 32 && j0 + 32 <= n;
-        if (!whole || e.bias || e.pre || e.act != kActNone) {
+        if (e.bias || e.pre || e.act != kActNone) {
             const int64_t j = j0 + lane;
             if (j < n) {
                 const float bias = e.bias ? e.bias[j * e.bias_step] : 0.f;
+                float* pre = e.pre ? e.pre + y0 + lane : nullptr;
+                float* t = tile + lane;
 #pragma unroll 2
-                for (int r = 0; r < rows; ++r) {
-                    float z = tile[r * kSpStageCols + lane];
+                for (int r = 0; r < rows; ++r, t += kSpStageCols) {
+                    float z = *t;
                     if (e.bias) z += bias;
-                    if (e.pre) e.pre[y0 + r * e.ld + lane] = z;
+                    if (pre) { *pre = z; pre += e.ld; }
                     if (e.act != kActNone) z = activate(z, e.act);
-                    if (whole) { tile[r * kSpStageCols + lane] = z; continue; }
-                    if (e.res) z += e.res[(i0 + r) * e.res_row + j * e.res_col];
-                    e.y[y0 + r * e.ld + lane] = z;
+                    *t = z;
                 }
             }
             __syncwarp();
         }
-        if (!whole) return;
-        const int r0 = lane >> 3, c0 = (lane & 7) * 4;
+        if (whole) {
+            const int r0 = lane >> 3, c0 = (lane & 7) * 4;
 #pragma unroll 1
-        for (int h = 0; h < 32; h += 16) {
-            float4 res[4];
-            if (e.res)
+            for (int h = 0; h < 32; h += 16) {
+                float4 res[4];
+                if (e.res)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) res[q] = __ldcs(reinterpret_cast<const float4*>(e.res + (i0 + h + q * 4 + r0) * e.res_row + j0 + c0));
+                    for (int q = 0; q < 4; ++q) res[q] = __ldcs(reinterpret_cast<const float4*>(e.res + (i0 + h + q * 4 + r0) * e.res_row + j0 + c0));
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int r = h + q * 4 + r0;
-                const float* t = tile + r * kSpStageCols + c0;
-                float4 v = make_float4(t[0], t[1], t[2], t[3]);
-                if (e.res) { v.x += res[q].x; v.y += res[q].y; v.z += res[q].z; v.w += res[q].w; }
-                *reinterpret_cast<float4*>(e.y + y0 + r * e.ld + c0) = v;
+                for (int q = 0; q < 4; ++q) {
+                    const int r = h + q * 4 + r0;
+                    const float* t = tile + r * kSpStageCols + c0;
+                    float4 v = make_float4(t[0], t[1], t[2], t[3]);
+                    if (e.res) { v.x += res[q].x; v.y += res[q].y; v.z += res[q].z; v.w += res[q].w; }
+                    *reinterpret_cast<float4*>(e.y + y0 + r * e.ld + c0) = v;
+                }
             }
+            return;
+        }
+        if (j0 + lane >= n) return;
+        // one column per lane, eight rows in flight
+        float* y = e.y + y0 + lane;
+        const float* res = e.res ? e.res + i0 * e.res_row + (j0 + lane) * e.res_col : nullptr;
+#pragma unroll 1
+        for (int h = 0; h < rows; h += 8) {
+            float v[8], w[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                v[q] = tile[(h + q) * kSpStageCols + lane];
+                w[q] = res && h + q < rows ? res[q * e.res_row] : 0.f;
+            }
+            if (res) res += 8 * e.res_row;
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (h + q < rows) y[q * e.ld] = e.res ? v[q] + w[q] : v[q];
+            y += 8 * e.ld;
         }
     }
 };
@@ -202,44 +224,42 @@ struct FloatOut {
 // between n and ld are padding that nothing reads).
 struct PlaneOut {
     PlaneEpilogue e;
-    __device__ __forceinline__ void piece(float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n, bool mirror) const {
+    struct Ahead { uint4 h[4], l[4]; };
+    // the piece's part of d, requested before the piece is there
+    __device__ __forceinline__ void ahead(Ahead& d, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t) const {
+        const int r0 = lane >> 2, c0 = (lane & 3) * 8;
+        if (!e.d || j0 + c0 >= e.ld) return;
+        const uint16_t* p = e.d + batch * e.batch_step + (i0 + r0) * e.ld + j0 + c0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q, p += 8 * e.ld)
+            if (i0 + q * 8 + r0 < m) { d.h[q] = *reinterpret_cast<const uint4*>(p); d.l[q] = *reinterpret_cast<const uint4*>(p + e.plane); }
+    }
+    __device__ __forceinline__ void piece(float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n, bool mirror, const Ahead& d) const {
         const int r0 = lane >> 2, c0 = (lane & 3) * 8;
         const int64_t at0 = batch * e.batch_step + (i0 + r0) * e.ld + j0 + c0;
         const bool here = j0 + c0 < e.ld;
-#pragma unroll 1
-        for (int h = 0; h < 32; h += 16) {
-            uint4 dh[2], dl[2];
 #pragma unroll
-            for (int q = 0; q < 2; ++q)
-                if (e.d && here && i0 + h + q * 8 + r0 < m) {
-                    const uint16_t* d = e.d + at0 + (h + q * 8) * e.ld;
-                    dh[q] = *reinterpret_cast<const uint4*>(d);
-                    dl[q] = *reinterpret_cast<const uint4*>(d + e.plane);
+        for (int q = 0; q < 4; ++q) {
+            if (!here || i0 + q * 8 + r0 >= m) continue;
+            float* t = tile + (q * 8 + r0) * kSpStageCols + c0;
+            float v[8];
+            const __half2* ph = reinterpret_cast<const __half2*>(&d.h[q]);
+            const __half2* pl = reinterpret_cast<const __half2*>(&d.l[q]);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) v[x] = t[x] * e.acc_scale;
+            if (e.d)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const float2 a = __half22float2(ph[x]), b = __half22float2(pl[x]);
+                    v[2 * x] += e.beta * ((a.x + b.x) * e.d_scale);
+                    v[2 * x + 1] += e.beta * ((a.y + b.y) * e.d_scale);
                 }
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const int r = h + q * 8 + r0;
-                if (!here || i0 + r >= m) continue;
-                float* t = tile + r * kSpStageCols + c0;
-                float v[8];
-                const __half2* ph = reinterpret_cast<const __half2*>(&dh[q]);
-                const __half2* pl = reinterpret_cast<const __half2*>(&dl[q]);
+            for (int x = 0; x < 8; ++x) v[x] *= e.out_scale;
+            store(v, at0 + q * 8 * e.ld);
+            if (mirror)
 #pragma unroll
-                for (int x = 0; x < 8; ++x) v[x] = t[x] * e.acc_scale;
-                if (e.d)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const float2 a = __half22float2(ph[x]), b = __half22float2(pl[x]);
-                        v[2 * x] += e.beta * ((a.x + b.x) * e.d_scale);
-                        v[2 * x + 1] += e.beta * ((a.y + b.y) * e.d_scale);
-                    }
-#pragma unroll
-                for (int x = 0; x < 8; ++x) v[x] *= e.out_scale;
-                store(v, at0 + (h + q * 8) * e.ld);
-                if (mirror)
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) t[x] = v[x];
-            }
+                for (int x = 0; x < 8; ++x) t[x] = v[x];
         }
         if (!mirror) return;
         __syncwarp();
@@ -289,6 +309,10 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0;
     const bool misplaced = (smem_u32(base) & 1023u) != 0;       // the same in every CTA; nothing is launched into it then
+    if (tid == 32) {                                            // the first loads do not wait for their descriptors then
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+    }
     if (tid == 0) {
         for (int i = 0; i < 4; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(main_full + i, 1); mbar_init(main_empty + i, 8 * CG); }
@@ -444,6 +468,9 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
             const uint32_t chunks = (uint32_t)((blocks + g.chunk - 1) / g.chunk);
 #pragma unroll
             for (int x = 0; x < kCols; ++x) sum[x] = 0.f;
+            const int64_t row0 = i0 + (int64_t)quarter * 32, col0 = j0 + half * kCols, in = g.splits > 1 ? part : batch;
+            typename Out::Ahead ahead;
+            if (row0 < g.m) out.ahead(ahead, lane, in, row0, col0, g.m, g.n);
             // the chunks of large products, then the small ones
 #pragma unroll 1
             for (uint32_t c = 0; c <= chunks; ++c) {
@@ -478,13 +505,13 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
                 if (!cross) ++item;
             }
             if (!ok) break;
-            const int64_t row0 = i0 + (int64_t)quarter * 32, col0 = j0 + half * kCols;
 #pragma unroll
             for (int q = 0; q < kCols / 32; ++q) {
 #pragma unroll
                 for (int x = 0; x < 32; ++x) piece[lane * kSpStageCols + x] = sum[q * 32 + x];
                 __syncwarp();
-                if (row0 < g.m) out.piece(piece, lane, g.splits > 1 ? part : batch, row0, col0 + q * 32, g.m, g.n, g.symmetric && i0 / (128 * CG) != j0 / BN);
+                if (row0 < g.m) out.piece(piece, lane, in, row0, col0 + q * 32, g.m, g.n, g.symmetric && i0 / (128 * CG) != j0 / BN, ahead);
+                if (q + 1 < kCols / 32 && row0 < g.m) out.ahead(ahead, lane, in, row0, col0 + (q + 1) * 32, g.m, g.n);
                 __syncwarp();
             }
         }
