@@ -159,7 +159,7 @@ struct FloatOut {
     bool packets;                      // y (and residual) take 16-byte accesses
     struct Ahead {};
     __device__ __forceinline__ void ahead(Ahead&, int, int64_t, int64_t, int64_t, int64_t, int64_t) const {}
-    __device__ __forceinline__ void piece(float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n, bool, const Ahead&) const {
+    __device__ __forceinline__ void piece(float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n, bool, Ahead&) const {
         const int rows = m - i0 < 32 ? (int)(m - i0) : 32;
         const int64_t y0 = batch * e.y_batch + i0 * e.ld + j0;
         const bool whole = packets && rows == 32 && j0 + 32 <= n;
@@ -224,27 +224,28 @@ struct FloatOut {
 // between n and ld are padding that nothing reads).
 struct PlaneOut {
     PlaneEpilogue e;
-    struct Ahead { uint4 h[4], l[4]; };
-    // the piece's part of d, requested before the piece is there
+    struct Ahead { uint4 h, l; };
+    // eight rows of the piece's part of d, requested before they are needed
     __device__ __forceinline__ void ahead(Ahead& d, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t) const {
         const int r0 = lane >> 2, c0 = (lane & 3) * 8;
-        if (!e.d || j0 + c0 >= e.ld) return;
+        if (!e.d || j0 + c0 >= e.ld || i0 + r0 >= m) return;
         const uint16_t* p = e.d + batch * e.batch_step + (i0 + r0) * e.ld + j0 + c0;
-#pragma unroll
-        for (int q = 0; q < 4; ++q, p += 8 * e.ld)
-            if (i0 + q * 8 + r0 < m) { d.h[q] = *reinterpret_cast<const uint4*>(p); d.l[q] = *reinterpret_cast<const uint4*>(p + e.plane); }
+        d.h = *reinterpret_cast<const uint4*>(p);
+        d.l = *reinterpret_cast<const uint4*>(p + e.plane);
     }
-    __device__ __forceinline__ void piece(float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n, bool mirror, const Ahead& d) const {
+    __device__ __forceinline__ void piece(float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n, bool mirror, Ahead& d) const {
         const int r0 = lane >> 2, c0 = (lane & 3) * 8;
         const int64_t at0 = batch * e.batch_step + (i0 + r0) * e.ld + j0 + c0;
         const bool here = j0 + c0 < e.ld;
-#pragma unroll
+#pragma unroll 1
         for (int q = 0; q < 4; ++q) {
+            Ahead cur = d;
+            if (q < 3) ahead(d, lane, batch, i0 + (q + 1) * 8, j0, m, n);
             if (!here || i0 + q * 8 + r0 >= m) continue;
             float* t = tile + (q * 8 + r0) * kSpStageCols + c0;
             float v[8];
-            const __half2* ph = reinterpret_cast<const __half2*>(&d.h[q]);
-            const __half2* pl = reinterpret_cast<const __half2*>(&d.l[q]);
+            const __half2* ph = reinterpret_cast<const __half2*>(&cur.h);
+            const __half2* pl = reinterpret_cast<const __half2*>(&cur.l);
 #pragma unroll
             for (int x = 0; x < 8; ++x) v[x] = t[x] * e.acc_scale;
             if (e.d)
@@ -505,13 +506,20 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
                 if (!cross) ++item;
             }
             if (!ok) break;
-#pragma unroll
+            // (one copy of the code that writes a piece: run once per piece, it costs the fetching of its instructions)
+#pragma unroll 1
             for (int q = 0; q < kCols / 32; ++q) {
 #pragma unroll
-                for (int x = 0; x < 32; ++x) piece[lane * kSpStageCols + x] = sum[q * 32 + x];
+                for (int w = 0; w < kCols / 32; ++w)
+                    if (w == q) {
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) piece[lane * kSpStageCols + x] = sum[w * 32 + x];
+                    }
                 __syncwarp();
-                if (row0 < g.m) out.piece(piece, lane, in, row0, col0 + q * 32, g.m, g.n, g.symmetric && i0 / (128 * CG) != j0 / BN, ahead);
-                if (q + 1 < kCols / 32 && row0 < g.m) out.ahead(ahead, lane, in, row0, col0 + (q + 1) * 32, g.m, g.n);
+                if (row0 < g.m) {
+                    out.piece(piece, lane, in, row0, col0 + q * 32, g.m, g.n, g.symmetric && i0 / (128 * CG) != j0 / BN, ahead);
+                    if (q + 1 < kCols / 32) out.ahead(ahead, lane, in, row0, col0 + (q + 1) * 32, g.m, g.n);
+                }
                 __syncwarp();
             }
         }
