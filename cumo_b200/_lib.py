@@ -89,6 +89,8 @@ def _declare(lib: ctypes.CDLL) -> None:
         "cb200_na_cum": (H, [c_char_p, H, c_int, c_int]),
         "cb200_na_linear": (H, [H, H, H, c_int, H, POINTER(H)]),
         "cb200_na_linear_grad": (c_int, [H, H, H, c_int, H, POINTER(H), POINTER(H), POINTER(H)]),
+        "cb200_na_orthogonalize": (H, [H, c_int, POINTER(c_double), c_double]),
+        "cb200_product_status": (c_int, []),
         "cb200_na_gated_cumsum": (H, [H, H, H, c_int]),
         "cb200_na_gated_cumsum_grad": (c_int, [H, H, H, H, c_int, POINTER(H), POINTER(H), POINTER(H)]),
         "cb200_na_where": (H, [H, c_int]),

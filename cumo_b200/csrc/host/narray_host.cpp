@@ -1041,6 +1041,26 @@ cb200_na_t* cb200_na_cum(const char* op_c, cb200_na_t* a, int axis, int nan) {
     return out;
 }
 
+// What an entry point with a status returned; an allocation that failed inside it is latched too and must not surface in the
+// next operation.
+static bool settled(int status, const char* what) {
+    if (status == 0) return launch_ok();
+    cb200_last_error(nullptr);
+    if (status == (int)cudaErrorLaunchTimeout) fail("CudaError", "%s: a bounded wait of an earlier product ran out; its results are not valid (cb200_product_status() clears this)", what);
+    else fail("CudaError", "%s: %s", what, cudaGetErrorString((cudaError_t)status));
+    return false;
+}
+
+// A temporary array goes back to the pool when the call returns, but a graph captured around the call would write to it again
+// at every replay, whoever holds it then: operators that need one refuse to be captured.
+static bool temporaries_allowed(const char* what) {
+    cudaStreamCaptureStatus c = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(cb200::current_stream(), &c) != cudaSuccess) { cudaGetLastError(); return true; }
+    if (c == cudaStreamCaptureStatusNone) return true;
+    fail("CudaError", "%s needs a temporary array here, which a captured graph cannot keep: pass contiguous operands of the full shape", what);
+    return false;
+}
+
 // ---- gated running sums ---------------------------------------------------------------------
 // Steps of `x` against a loop of `nd` dimensions (aligned at the last, repeated where its extent is 1 or missing; a single
 // element repeats everywhere), or an error.
@@ -1065,6 +1085,7 @@ static cb200_na* sum_to_shape_of(cb200_na* full, const cb200_na* like) {
     }
     cb200_na* r = full;
     if (mask) {
+        if (!temporaries_allowed("the sum over what an operand was repeated over")) { cb200_na_release(full); return nullptr; }
         r = size_of(full) ? (cb200_na*)cb200_na_reduce("sum", full, mask, 1, 0) : nullptr;
         if (!size_of(full)) r = make(like->dtype, like->ndim, like->shape, true);
         cb200_na_release(full);
@@ -1106,8 +1127,7 @@ cb200_na_t* cb200_na_gated_cumsum(cb200_na_t* x, cb200_na_t* gate, cb200_na_t* i
     auto f = x->dtype == CB200_SFLOAT ? cb200_sfloat_gated_cumsum_runs_kernel_launch : cb200_dfloat_gated_cumsum_runs_kernel_launch;
     const int status = f(data_ptr(x), data_ptr(gate), initial ? data_ptr(initial) : nullptr, data_ptr(out), (ssize_t)x->step[axis], (ssize_t)gstep[axis],
                          (ssize_t)out->step[axis], (uint64_t)x->shape[axis], k, oshape, ox, og, oi, oh);
-    if (status) { fail("CudaError", "gated_cumsum: %s", cudaGetErrorString((cudaError_t)status)); cb200_na_release(out); return nullptr; }
-    if (!launch_ok()) { cb200_na_release(out); return nullptr; }
+    if (!settled(status, "gated_cumsum")) { cb200_na_release(out); return nullptr; }
     return out;
 }
 
@@ -1161,8 +1181,7 @@ int cb200_na_gated_cumsum_grad(cb200_na_t* grad, cb200_na_t* gate, cb200_na_t* h
             if (!dgate) return give_up();
             status = launch();
         }
-        if (status) { fail("CudaError", "gated_cumsum_grad: %s", cudaGetErrorString((cudaError_t)status)); return give_up(); }
-        if (!launch_ok()) return give_up();
+        if (!settled(status, "gated_cumsum_grad")) return give_up();
     }
     dgate = sum_to_shape_of(dgate, gate);
     if (!dgate) return give_up();
@@ -1194,6 +1213,7 @@ struct Rows {
             last = d;
         }
         if (even) return true;
+        if (!temporaries_allowed("this operand's layout")) return false;
         cb200_na view = *x;
         view.ndim = nd;
         for (int d = 0; d < nd; ++d) { view.shape[d] = shape[d]; view.step[d] = step[d]; }
@@ -1240,8 +1260,7 @@ cb200_na_t* cb200_na_linear(cb200_na_t* x, cb200_na_t* w, cb200_na_t* bias, int 
         };
         status = x->dtype == CB200_SFLOAT ? run(cb200_sfloat_linear_kernel_launch, (float*)nullptr) : run(cb200_dfloat_linear_kernel_launch, (double*)nullptr);
     }
-    if (status) fail("CudaError", "linear: %s", cudaGetErrorString((cudaError_t)status));
-    if (status || !launch_ok()) { cb200_na_release(y); cb200_na_release(pre); return nullptr; }
+    if (!settled(status, "linear")) { cb200_na_release(y); cb200_na_release(pre); return nullptr; }
     if (pre_out) *pre_out = pre;
     return y;
 }
@@ -1278,14 +1297,49 @@ int cb200_na_linear_grad(cb200_na_t* grad, cb200_na_t* x, cb200_na_t* w, int act
                      (const T*)rp.p, rp.row, rp.col, activation, dx ? (T*)data_ptr(dx) : nullptr, dw ? (T*)data_ptr(dw) : nullptr, db ? (T*)data_ptr(db) : nullptr);
         };
         const int status = grad->dtype == CB200_SFLOAT ? run(cb200_sfloat_linear_grad_kernel_launch, (float*)nullptr) : run(cb200_dfloat_linear_grad_kernel_launch, (double*)nullptr);
-        if (status) fail("CudaError", "linear_grad: %s", cudaGetErrorString((cudaError_t)status));
-        ok = !status && launch_ok();
+        ok = settled(status, "linear_grad");
     }
     if (!ok) { cb200_na_release(dx); cb200_na_release(dw); cb200_na_release(db); return 1; }
     if (dx_out) *dx_out = dx;
     if (dw_out) *dw_out = dw;
     if (dbias_out) *dbias_out = db;
     return 0;
+}
+
+cb200_na_t* cb200_na_orthogonalize(cb200_na_t* g, int steps, const double* coefs, double eps) {
+    if (!is_float_type(g->dtype)) return (cb200_na*)fail("TypeError", "orthogonalize needs an SFloat or DFloat array");
+    if (g->ndim < 2) return (cb200_na*)fail("ShapeError", "orthogonalize needs an array of two or more dimensions");
+    if (steps < 0 || (steps && !coefs) || !(eps >= 0)) return (cb200_na*)fail("ArgumentError", "orthogonalize: bad steps, coefs or eps");
+    const int nd = g->ndim;
+    const cb200_na* in = g;
+    cb200_na* copy = nullptr;
+    int64_t batch = 1, bstep = 0;
+    bool even = true;
+    for (int d = nd - 3, last = -1; d >= 0; --d) {
+        batch *= g->shape[d];
+        if (g->shape[d] == 1) continue;
+        if (last < 0) bstep = g->step[d];
+        else even = even && g->step[d] == g->step[last] * g->shape[last];
+        last = d;
+    }
+    if (!even && size_of(g)) {
+        if (!temporaries_allowed("this batch's layout")) return nullptr;
+        copy = cast_to(g, g->dtype);
+        if (!copy) return nullptr;
+        in = copy;
+        bstep = in->step[nd - 3];
+        for (int d = nd - 3; d >= 0; --d) if (in->shape[d] != 1) { bstep = in->step[d]; break; }
+    }
+    cb200_na* out = make(g->dtype, nd, g->shape, false);
+    if (out) {
+        const ssize_t row = in->shape[nd - 2] != 1 ? (ssize_t)in->step[nd - 2] : 0, col = in->shape[nd - 1] != 1 ? (ssize_t)in->step[nd - 1] : 0;
+        const int status = g->dtype == CB200_SFLOAT
+            ? cb200_sfloat_orthogonalize_kernel_launch(batch, g->shape[nd - 2], g->shape[nd - 1], (const float*)data_ptr(in), (ssize_t)bstep, row, col, steps, coefs, eps, (float*)data_ptr(out))
+            : cb200_dfloat_orthogonalize_kernel_launch(batch, g->shape[nd - 2], g->shape[nd - 1], (const double*)data_ptr(in), (ssize_t)bstep, row, col, steps, coefs, eps, (double*)data_ptr(out));
+        if (!settled(status, "orthogonalize")) { cb200_na_release(out); out = nullptr; }
+    }
+    cb200_na_release(copy);
+    return out;
 }
 
 // ---- bincount ------------------------------------------------------------------------------

@@ -14,16 +14,22 @@
 namespace cb200 {
 
 // ---- |G|_F in 64 bits: slices of a matrix to partial sums of squares, folded in slice order ---------------------------
+// (rows and columns may be exchanged for this: the caller passes the contiguous axis as columns)
 template <typename T>
 __global__ void __launch_bounds__(kBlock)
-square_sums_kernel(const Operand<T> G, int64_t m, int64_t n, int slices, double* sums) {
-    const T* g = G.p + (int64_t)blockIdx.y * G.batch;
-    const int64_t total = m * n;
+square_sums_kernel(const T* g, int64_t g_batch, int64_t rows, int64_t columns, int64_t row_step, int64_t column_step, int slices, double* sums) {
+    g += (int64_t)blockIdx.y * g_batch;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     double s = 0;
-    for (int64_t f = (int64_t)blockIdx.x * kBlock + threadIdx.x; f < total; f += (int64_t)slices * kBlock) {
-        const int64_t i = f / n;
-        const double v = (double)g[i * G.row + (f - i * n) * G.k];
-        s += v * v;
+    for (int64_t i = (int64_t)blockIdx.x * kWarpsPerBlock + warp; i < rows; i += (int64_t)slices * kWarpsPerBlock) {
+        const T* r = g + i * row_step;
+        for (int64_t j0 = lane; j0 < columns; j0 += 32 * 8) {
+            T v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = j0 + u * 32 < columns ? r[(j0 + u * 32) * column_step] : T(0);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s = fma((double)v[u], (double)v[u], s);
+        }
     }
     __shared__ double part[kBlock];
     part[threadIdx.x] = s;
@@ -219,19 +225,33 @@ static int orthogonalize(int64_t batch, int64_t rows, int64_t columns, const T* 
                          const double* coefs, double eps, T* out) {
     CB200_TRACE_LAUNCH();
     constexpr ssize_t es = sizeof(T);
-    if (batch < 0 || rows < 0 || columns < 0 || steps < 0 || (steps && !coefs) || g_batch % es || g_row % es || g_col % es || batch > 65535)
+    if (batch < 0 || rows < 0 || columns < 0 || steps < 0 || (steps && !coefs) || g_batch % es || g_row % es || g_col % es)
         return (int)cudaErrorInvalidValue;
     if (batch == 0 || rows == 0 || columns == 0) return 0;
+    constexpr int64_t kMostBatch = 32768;                       // (grids count the matrices in 16 bits)
+    if (batch > kMostBatch) {
+        for (int64_t b = 0; b < batch; b += kMostBatch) {
+            const int rc = orthogonalize<T>(batch - b < kMostBatch ? batch - b : kMostBatch, rows, columns, g + b * (g_batch / es), g_batch, g_row, g_col, steps,
+                                            coefs, eps, out + b * rows * columns);
+            if (rc) return rc;
+        }
+        return 0;
+    }
     cudaStream_t st = current_stream();
     const bool tall = rows > columns;
     const int64_t m = tall ? columns : rows, n = tall ? rows : columns;
     const Operand<T> G = tall ? Operand<T>{g, g_col / es, g_row / es, g_batch / es} : Operand<T>{g, g_row / es, g_col / es, g_batch / es};
     Scratch scratch(st);
-    int64_t slices = (m * n + kBlock * 8 - 1) / (kBlock * 8);
+    const bool along_k = G.k == 1 || G.row != 1;
+    const int64_t sr = along_k ? m : n, sc_ = along_k ? n : m;
+    int64_t slices = (sr + kWarpsPerBlock - 1) / kWarpsPerBlock;
+    const int64_t enough = ((int64_t)sm_count() * 4 + batch - 1) / batch;
+    if (slices > enough) slices = enough;
     if (slices > 256) slices = 256;
     double* sums = reinterpret_cast<double*>(scratch.take((size_t)batch * slices * sizeof(double)));
     if (!sums) return (int)cudaErrorMemoryAllocation;
-    square_sums_kernel<T><<<dim3((unsigned)slices, (unsigned)batch), kBlock, 0, st>>>(G, m, n, (int)slices, sums);
+    square_sums_kernel<T><<<dim3((unsigned)slices, (unsigned)batch), kBlock, 0, st>>>(G.p, G.batch, sr, sc_, along_k ? G.row : G.k, along_k ? G.k : G.row,
+                                                                                  (int)slices, sums);
     count_launch();
     if constexpr (sizeof(T) == 4) {
         const OrthoScales sc(steps, coefs);
@@ -242,7 +262,7 @@ static int orthogonalize(int64_t batch, int64_t rows, int64_t columns, const T* 
     T* p = reinterpret_cast<T*>(scratch.take((size_t)batch * m * m * es));
     T* q = reinterpret_cast<T*>(scratch.take((size_t)batch * m * m * es));
     if (!x || !x2 || !p || !q) return (int)cudaErrorMemoryAllocation;
-    scale_kernel<T><<<dim3((unsigned)slices, (unsigned)batch), kBlock, 0, st>>>(G, m, n, (int)slices, sums, eps, x);
+    scale_kernel<T><<<dim3(256u, (unsigned)batch), kBlock, 0, st>>>(G, m, n, (int)slices, sums, eps, x);
     count_launch();
     int rc = (int)cudaGetLastError();
     for (int s = 0; s < steps && rc == 0; ++s) {

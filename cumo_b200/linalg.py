@@ -7,10 +7,10 @@ every operand into two TF32 numbers and wants both operands with K contiguous.
 """
 from __future__ import annotations
 
-from ctypes import byref, c_char_p, c_double, c_int, c_int64, c_size_t, c_ssize_t, c_void_p, create_string_buffer
+from ctypes import byref, c_char_p, c_double, c_int, c_int64, c_size_t, c_void_p, create_string_buffer
 
 from . import _lib
-from .narray import CudaError, CumoError, DFloat, SFloat, ShapeError, _raise_last
+from .narray import CumoError, DFloat, SFloat, ShapeError, _raise_last
 
 
 def gemm_nt(a: SFloat, bt: SFloat) -> SFloat:
@@ -106,26 +106,12 @@ def _activation(name):
     return ACTIVATIONS.index(name)
 
 
-def _ptr(x):
-    return c_void_p(x.data_ptr if x is not None else None)
-
-
-def _step(x, d):
-    return c_ssize_t(x.steps[d] if x is not None and x.shape[d] != 1 else 0)
-
-
 def _check_types(T, **operands):
     if T not in (SFloat, DFloat):
         raise TypeError("the operands must be SFloat or DFloat arrays")
     for name, x in operands.items():
         if x is not None and type(x) is not T:
             raise TypeError(f"{name} is {type(x).__name__}, the other operands are {T.__name__}")
-
-
-def _status(rc, what):
-    if rc:
-        _lib.load().cb200_last_error(None)
-        raise CudaError(f"{what} failed with CUDA status {rc}")
 
 
 def _handle(x):
@@ -169,30 +155,16 @@ def orthogonalize(g, steps=5, coefs=(3.4445, -4.7750, 2.0315), eps=1e-7):
     being taken.  `coefs` is one triple (a, b, c) for every step or a list of one triple per step.  With the default triple,
     which is quick but does not converge, five steps bring singular values above some thousandths of the norm to between 0.7
     and 1.2."""
-    T = type(g)
-    _check_types(T)
+    _check_types(type(g))
     if g.ndim < 2:
         raise ShapeError("orthogonalize needs an array of two or more dimensions")
-    if not isinstance(steps, int) or steps < 0:
+    if not isinstance(steps, int) or isinstance(steps, bool) or steps < 0:
         raise ValueError("steps must be a number of steps")
-    triples = [tuple(float(c) for c in t) for t in (coefs if hasattr(coefs[0], "__len__") else [coefs] * steps)]
+    coefs = list(coefs)
+    triples = [tuple(float(c) for c in t) for t in (coefs if not coefs or hasattr(coefs[0], "__len__") else [coefs] * steps)]
     if len(triples) != steps or any(len(t) != 3 for t in triples):
         raise ValueError("coefs must be three numbers, or three numbers for each step")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
     flat = [c for t in triples for c in t]
-    out = T(*g.shape)
-    rows, cols = g.shape[-2:]
-    batch_shape, st = g.shape[:-2], g.steps
-    lead = [(n, s) for n, s in zip(batch_shape, st) if n != 1]
-    if not all(a[1] == b[0] * b[1] for a, b in zip(lead, lead[1:])):
-        g = g.dup()                                       # batches that are not evenly spaced
-        lead = [(n, s) for n, s in zip(batch_shape, g.steps) if n != 1]
-    batch = 1
-    for n in batch_shape:
-        batch *= n
-    fn = getattr(_lib.load(), f"cb200_{out._tname}_orthogonalize_kernel_launch")
-    fn.restype, fn.argtypes = c_int, None
-    _status(fn(c_int64(batch), c_int64(rows), c_int64(cols), _ptr(g), c_ssize_t(lead[-1][1] if lead else 0), _step(g, g.ndim - 2), _step(g, g.ndim - 1),
-               c_int(steps), (c_double * max(1, len(flat)))(*flat), c_double(eps), _ptr(out)), "orthogonalize")
-    return out
+    return type(g)._from_handle(_lib.load().cb200_na_orthogonalize(g._h, steps, (c_double * max(1, len(flat)))(*flat), eps))

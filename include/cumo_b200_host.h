@@ -107,6 +107,8 @@ cb200_na_t* cb200_na_linear(cb200_na_t* x, cb200_na_t* w, cb200_na_t* bias, int 
 /* Its gradients for grad (.., n); each output may be NULL, pre too without an activation.  Returns 0, or 1 with cb200_host_error() set. */
 int cb200_na_linear_grad(cb200_na_t* grad, cb200_na_t* x, cb200_na_t* w, int activation, cb200_na_t* pre, cb200_na_t** dx, cb200_na_t** dw,
                          cb200_na_t** dbias);
+/* Newton-Schulz steps on every matrix of the last two dimensions (cb200_<T>_orthogonalize_kernel_launch); coefs: 3 * steps numbers. */
+cb200_na_t* cb200_na_orthogonalize(cb200_na_t* g, int steps, const double* coefs, double eps);
 /* h[t] = gate[t] * h[t-1] + x[t] along `axis`, in x's shape; gate is repeated to x's shape, initial (may be NULL: h[0] = x[0])
  * to the shape without the axis.  All SFloat or all DFloat. */
 cb200_na_t* cb200_na_gated_cumsum(cb200_na_t* x, cb200_na_t* gate, cb200_na_t* initial, int axis);
