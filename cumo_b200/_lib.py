@@ -61,6 +61,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "cb200_na_new": (H, [c_int, c_int, P64]),
         "cb200_na_zeros": (H, [c_int, c_int, P64]),
         "cb200_na_wrap": (H, [c_int, c_int, P64, P64, c_void_p, c_int64]),
+        "cb200_na_wrap_elements": (H, [c_int, c_int, P64, c_void_p]),
         "cb200_na_view": (H, [H, c_int, P64, P64, c_int64]),
         "cb200_na_release": (None, [H]),
         "cb200_na_dtype": (c_int, [H]),

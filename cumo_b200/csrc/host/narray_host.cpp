@@ -512,6 +512,14 @@ cb200_na_t* cb200_na_wrap(int dtype, int ndim, const int64_t* shape, const int64
     return a;
 }
 
+cb200_na_t* cb200_na_wrap_elements(int dtype, int ndim, const int64_t* shape_and_steps, void* device_ptr) {
+    if (dtype < 0 || dtype > CB200_UINT32 || dtype == CB200_BIT) return (cb200_na*)fail("TypeError", "no element steps for dtype %d", dtype);
+    if (ndim < 0 || ndim > kMaxD) return (cb200_na*)fail("ShapeError", "ndim %d out of range", ndim);
+    int64_t step[kMaxD];
+    for (int d = 0; d < ndim; ++d) step[d] = shape_and_steps[ndim + d] * kElemSize[dtype];
+    return cb200_na_wrap(dtype, ndim, shape_and_steps, step, device_ptr, 0);
+}
+
 cb200_na_t* cb200_na_view(cb200_na_t* a, int ndim, const int64_t* shape, const int64_t* step, int64_t offset) {
     if (ndim < 0 || ndim > kMaxD) return (cb200_na*)fail("ShapeError", "ndim %d out of range", ndim);
     // every element of the view must lie inside the parent's buffer

@@ -339,6 +339,10 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
     if constexpr (CG == 2) cluster_sync_all();                   // the peer's barriers exist before anything arrives at them
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *tmem_slot;
+    // Launched while the kernel in front of it may still run (so that launch and set-up cost nothing between the products of a
+    // chain): from here on its results are read, and the kernel behind may be launched in turn.
+    pdl_wait();
+    pdl_trigger();
 
     const int64_t cluster = blockIdx.x / CG, clusters = gridDim.x / CG;
     const int64_t my_tiles = misplaced || cluster >= g.n_tiles ? 0 : (g.n_tiles - cluster + clusters - 1) / clusters;
@@ -621,21 +625,18 @@ static int launch_shape(SplitKind kind, const Planes& a, const Planes& b, const 
     }
     const int64_t slots = sm_count() / CG;
     const unsigned grid = (unsigned)((g.n_tiles < slots ? g.n_tiles : slots) * CG);
-    if (CG == 1) {
-        kernel<<<grid, kSpThreads, S::kSmem, st>>>(g, ma, mb, out);
-        count_launch();
-        return (int)cudaGetLastError();
-    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kSpThreads);
     cfg.dynamicSmemBytes = S::kSmem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CG; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = CG; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = CG == 1 ? 1 : 2;
     const cudaError_t rc = cudaLaunchKernelEx(&cfg, kernel, g, ma, mb, out);
     if (rc != cudaSuccess) { cudaGetLastError(); return (int)rc; }
     count_launch();

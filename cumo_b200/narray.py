@@ -56,12 +56,12 @@ def _raise_last():
     raise exc((msg or b"").decode())
 
 
-_INT64S = [c_int64 * max(1, n) for n in range(_lib.MAX_DIM + 1)]        # array types by length
+_INT64S = [c_int64 * max(1, n) for n in range(2 * _lib.MAX_DIM + 1)]    # array types by length
 
 
 def _arr64(values):
     n = len(values)
-    return (_INT64S[n] if n <= _lib.MAX_DIM else c_int64 * n)(*values)
+    return (_INT64S[n] if n < len(_INT64S) else c_int64 * n)(*values)
 
 
 def _axis_mask(axis, ndim):
@@ -178,9 +178,12 @@ class NArray:
         code, shape = cls.dtype_code, t.shape
         if t.dtype != _TORCH[code] or not t.is_cuda:
             raise TypeError(f"{cls.__name__}.from_torch needs a CUDA tensor of {_TORCH[code]}")
-        es = _ESZ[code]
-        h = _lib.load().cb200_na_wrap(code, len(shape), _arr64(shape), _arr64([s * es for s in t.stride()]), t.data_ptr(), 0)
-        return NArray._from_handle(h, keep=t)
+        h = _lib.load().cb200_na_wrap_elements(code, len(shape), _arr64((*shape, *t.stride())), t.data_ptr())
+        if not h:
+            _raise_last()
+        obj = object.__new__(cls)
+        obj._h, obj._keep = h, t
+        return obj
 
     @classmethod
     def from_device_pointer(cls, ptr: int, shape, keep=None):

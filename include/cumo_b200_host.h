@@ -48,6 +48,8 @@ cb200_na_t* cb200_na_new(int dtype, int ndim, const int64_t* shape);            
 cb200_na_t* cb200_na_zeros(int dtype, int ndim, const int64_t* shape);
 /* borrow device memory owned by someone else (steps in bytes; bits for CB200_BIT) */
 cb200_na_t* cb200_na_wrap(int dtype, int ndim, const int64_t* shape, const int64_t* step, void* device_ptr, int64_t offset);
+/* the same with shape and steps one after the other, steps in elements (value types) */
+cb200_na_t* cb200_na_wrap_elements(int dtype, int ndim, const int64_t* shape_and_steps, void* device_ptr);
 /* a view of `a`: new shape/steps/offset (offset relative to a's first element, same unit as steps) */
 cb200_na_t* cb200_na_view(cb200_na_t* a, int ndim, const int64_t* shape, const int64_t* step, int64_t offset);
 void cb200_na_release(cb200_na_t* a);
