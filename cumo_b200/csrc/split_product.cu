@@ -595,9 +595,11 @@ static int launch_shape(SplitKind kind, const Planes& a, const Planes& b, const 
     g.kblocks = (int)((a.k + kSpKB - 1) / kSpKB);
     g.tiles_m = (a.rows + 128 * CG - 1) / (128 * CG);
     g.tiles_n = (b.rows + BN - 1) / BN;
-    // Half pairs feed products whose errors add up over an iteration: short sums, whose own rounding is small, take finer
-    // chunks (four truncating additions per block); longer ones, and the three-part products of a single layer, sixteen.
-    g.chunk = kind != kSplitHalfx2 || g.kblocks > 16 ? 4 : g.kblocks > 4 ? 2 : 1;
+    // Half pairs feed products whose errors add up over an iteration.  Where tiles are narrow, because there are few, reading an
+    // accumulator costs little and hides behind the other one: every block or two.  Full tiles belong to large matrices, whose own
+    // rounding in 32 bits is larger: four blocks, eight from 4096 on (4096 x 4096: error 1.4e-6 instead of 7e-7, where 32-bit sums
+    // have 3.2e-6).  The three-part products of a single layer take four.
+    g.chunk = kind != kSplitHalfx2 ? 4 : BN == 64 ? 1 : BN == 128 ? (g.kblocks > 16 ? 2 : 1) : g.kblocks >= 64 ? 8 : g.kblocks > 4 ? 4 : 1;
     g.symmetric = symmetric && BN == 128 * CG;
     g.per_split = (g.kblocks + splits - 1) / splits;
     g.splits = (g.kblocks + g.per_split - 1) / g.per_split;             // no piece is empty

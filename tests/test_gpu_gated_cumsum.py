@@ -166,6 +166,24 @@ def test_gates_that_stop_or_grow(shape, axis):
     assert np.array_equal(got, quiet)                        # 1e6 * 0 stays 0, however many steps
 
 
+@pytest.mark.parametrize("shape,axis", [((1, 3000, 32), 1), ((2, 5000), 1), ((1, 700, 5), 1)])
+def test_products_of_gates_that_nearly_vanish_and_return(shape, axis):
+    """Two gates that multiply to less than the type's normal range, then one that brings the product back: the state passes
+    through them without having been that small itself."""
+    import cumo_b200 as xp
+
+    n = shape[axis]
+    x, gate = np.zeros(shape, np.float32), np.full(shape, 0.5, np.float32)
+    xs, gs = np.moveaxis(x, axis, -1), np.moveaxis(gate, axis, -1)
+    for at in range(20, n - 40, 37):
+        xs[..., at] = 2.0 ** 90
+        gs[..., at + 1:at + 5] = [2.0 ** -70, 2.0 ** -75, 2.0 ** 80, 2.0 ** 60]       # state 2^90 -> 2^20 -> 2^-55 -> 2^25 -> 2^85
+        gs[..., at + 6] = 0
+    want, mag = ref.gated(x, gate, axis)
+    got = xp.SFloat.from_numpy(x).gated_cumsum(xp.SFloat.from_numpy(gate), axis=axis).to_numpy()
+    assert np.all(np.abs(got - want) <= ref.gated_bound(mag, gate, axis, 2.0 ** -24))
+
+
 def test_empty_and_token_by_token():
     import cumo_b200 as xp
 
