@@ -9,11 +9,11 @@
 namespace cb200 {
 
 // ---- the product on the CUDA cores ------------------------------------------------------------------------------------
-// 64 x 64 outputs per CTA, 4 x 4 per thread, 16 of K at a time through shared memory.  Lanes run along whichever axis of
+// 64 x 64 outputs per CTA, 4 x 4 per thread, 32 of K at a time through shared memory.  Lanes run along whichever axis of
 // each operand is contiguous.  Every 64 of K the sums so far are put aside and new ones begun: the error of a long sum in
 // 32 bits then grows with the square root of its number of pieces, not of its terms.  Bound by the FMA rate at large sizes and by
 // latency at small ones.
-constexpr int kPcM = 64, kPcN = 64, kPcK = 16, kPcPad = 4;
+constexpr int kPcM = 64, kPcN = 64, kPcK = 32, kPcPad = 4;
 
 template <typename T>
 __global__ void __launch_bounds__(kBlock)
@@ -63,7 +63,7 @@ product_cc_kernel(int64_t m, int64_t n, int64_t k, const Operand<T> A, const Ope
 #pragma unroll
                 for (int y = 0; y < 4; ++y) acc[x][y] = av[x] * bv[y] + acc[x][y];
         }
-        if ((k0 / kPcK & 3) == 3) {
+        if ((k0 / kPcK & 1) == 1) {
 #pragma unroll
             for (int x = 0; x < 4; ++x)
 #pragma unroll
@@ -237,7 +237,7 @@ static bool few_rows(int64_t m, int64_t n, int64_t k) { return k >= 16 && (m <= 
 
 template <typename T>
 static int product(int64_t m, int64_t n, int64_t k, const Operand<T>& a, const Operand<T>& b, const Epilogue<T>& e, cudaStream_t st) {
-    if (few_rows(m, n, k)) return launch_product_rows<T>(m, n, k, a, b, e, st);
+    if (few_rows(m, n, k)) return launch_product_rows<T>(m, n, k, 1, a, b, e, st);
     return launch_product_cc<T>(m, n, k, 1, a, b, e, st);
 }
 

@@ -86,7 +86,7 @@ int launch_product_cc(int64_t m, int64_t n, int64_t k, int64_t batch, const Oper
 
 // The same with few rows, where reading B once is what it costs: m up to a few dozen, any steps.
 template <typename T>
-int launch_product_rows(int64_t m, int64_t n, int64_t k, const Operand<T>& a, const Operand<T>& b, const Epilogue<T>& e, cudaStream_t st);
+int launch_product_rows(int64_t m, int64_t n, int64_t k, int64_t batch, const Operand<T>& a, const Operand<T>& b, const Epilogue<T>& e, cudaStream_t st);
 
 // Scratch of one call.  Outside a capture it comes from the pool callback and goes back to it when the call returns (the
 // next taker queues behind on the same stream).  Inside a capture it is an allocation node of the graph itself: two graphs

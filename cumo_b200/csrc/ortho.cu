@@ -255,7 +255,10 @@ static int orthogonalize(int64_t batch, int64_t rows, int64_t columns, const T* 
     count_launch();
     if constexpr (sizeof(T) == 4) {
         const OrthoScales sc(steps, coefs);
-        if (sc.fits) return orthogonalize_split(batch, m, n, tall, G, steps, coefs, eps, (int)slices, sums, sc, out, scratch, st);
+        // Matrices of few rows have short sums behind their results, and ordinary fp32 FMAs round those better than the tensor
+        // cores truncate them (80 x 1408: error 1.1e-6 against 1.8e-6); P's long sums are cut over clusters.
+        const bool few = m <= 128 && batch * m * m * n <= (1LL << 26);
+        if (sc.fits && !few) return orthogonalize_split(batch, m, n, tall, G, steps, coefs, eps, (int)slices, sums, sc, out, scratch, st);
     }
     T* x = reinterpret_cast<T*>(scratch.take((size_t)batch * m * n * es));
     T* x2 = reinterpret_cast<T*>(scratch.take((size_t)batch * m * n * es));
@@ -269,7 +272,8 @@ static int orthogonalize(int64_t batch, int64_t rows, int64_t columns, const T* 
         const T a = (T)coefs[3 * s], b = (T)coefs[3 * s + 1], c = (T)coefs[3 * s + 2];
         Epilogue<T> e = {};
         e.alpha = T(1); e.y = p; e.ld = m; e.y_batch = m * m;                              // P = X X^T
-        rc = launch_product_cc<T>(m, m, n, batch, {x, n, 1, m * n}, {x, n, 1, m * n}, e, st);
+        rc = m <= 128 && n >= 64 ? launch_product_rows<T>(m, m, n, batch, {x, n, 1, m * n}, {x, n, 1, m * n}, e, st)
+                                 : launch_product_cc<T>(m, m, n, batch, {x, n, 1, m * n}, {x, n, 1, m * n}, e, st);
         if (rc) break;
         e.alpha = c; e.beta = b; e.d = p; e.d_row = m; e.d_col = 1; e.d_batch = m * m; e.y = q;   // Q = b P + c P P
         rc = launch_product_cc<T>(m, m, m, batch, {p, m, 1, m * m}, {p, m, 1, m * m}, e, st);

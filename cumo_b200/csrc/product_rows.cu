@@ -19,7 +19,8 @@ constexpr int kRowsChunk = 512;                     // k per piece of A
 
 // Adds the cluster's partial sums red[MT][cols] in CTA order and finishes this CTA's share of the outputs.
 template <typename T, int MT>
-__device__ __forceinline__ void finish_rows(T* red, int cols, int cluster_size, int64_t i0, int64_t j0, int64_t m, int64_t n, const Epilogue<T>& e) {
+__device__ __forceinline__ void finish_rows(T* red, int cols, int cluster_size, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n,
+                                            const Epilogue<T>& e) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     if (cluster_size > 1) cluster.sync();
@@ -38,7 +39,7 @@ __device__ __forceinline__ void finish_rows(T* red, int cols, int cluster_size, 
         } else {
             s = red[f];
         }
-        finish(e, 0, i, j, s);
+        finish(e, batch, i, j, s);
     }
     if (cluster_size > 1) cluster.sync();                        // nobody leaves while its sums may still be read
 }
@@ -55,12 +56,14 @@ template <typename T, int N> struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) 
 
 template <typename T, int MT, bool PACKETS>
 __global__ void __launch_bounds__(kBlock)
-rows_by_columns_kernel(int64_t m, int64_t n, int64_t k, const Operand<T> A, const Operand<T> B, const Epilogue<T> e, int cluster_size, int64_t strips) {
+rows_by_columns_kernel(int64_t m, int64_t n, int64_t k, Operand<T> A, Operand<T> B, const Epilogue<T> e, int cluster_size, int64_t strips) {
     constexpr int V = 16 / sizeof(T), COLS = 32 * V, U = 8;
     extern __shared__ __align__(16) char smem[];
     T* xs = reinterpret_cast<T*>(smem);                          // [k of the piece][MT]
     T* part = reinterpret_cast<T*>(smem);                        // [8 warps][MT][COLS], after the last piece
     T* red = part + kWarpsPerBlock * MT * COLS;                  // [MT][COLS]
+    A.p += (int64_t)blockIdx.y * A.batch;
+    B.p += (int64_t)blockIdx.y * B.batch;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rank = blockIdx.x % cluster_size;
     const int64_t unit = blockIdx.x / cluster_size, j0 = (unit % strips) * COLS, i0 = (unit / strips) * MT;
@@ -127,16 +130,18 @@ rows_by_columns_kernel(int64_t m, int64_t n, int64_t k, const Operand<T> A, cons
         for (int w = 1; w < kWarpsPerBlock; ++w) s += part[w * MT * COLS + f];
         red[f] = s;
     }
-    finish_rows<T, MT>(red, COLS, cluster_size, i0, j0, m, n, e);
+    finish_rows<T, MT>(red, COLS, cluster_size, blockIdx.y, i0, j0, m, n, e);
 }
 
 template <typename T, int MT, int C, bool PACKETS>
 __global__ void __launch_bounds__(kBlock)
-rows_by_dots_kernel(int64_t m, int64_t n, int64_t k, const Operand<T> A, const Operand<T> B, const Epilogue<T> e, int cluster_size, int64_t strips) {
+rows_by_dots_kernel(int64_t m, int64_t n, int64_t k, Operand<T> A, Operand<T> B, const Epilogue<T> e, int cluster_size, int64_t strips) {
     constexpr int V = PACKETS ? 16 / sizeof(T) : 1, COLS = kWarpsPerBlock * C, SPAN = 32 * V;
     extern __shared__ __align__(16) char smem[];
     T* xs = reinterpret_cast<T*>(smem);                          // [MT][k of the piece]
     __shared__ T red[MT * COLS];
+    A.p += (int64_t)blockIdx.y * A.batch;
+    B.p += (int64_t)blockIdx.y * B.batch;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rank = blockIdx.x % cluster_size;
     const int64_t unit = blockIdx.x / cluster_size, j0 = (unit % strips) * COLS, i0 = (unit / strips) * MT;
@@ -206,22 +211,22 @@ rows_by_dots_kernel(int64_t m, int64_t n, int64_t k, const Operand<T> A, const O
             for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
             if (lane == 0) red[r * COLS + warp * C + c] = s;
         }
-    finish_rows<T, MT>(red, COLS, cluster_size, i0, j0, m, n, e);
+    finish_rows<T, MT>(red, COLS, cluster_size, blockIdx.y, i0, j0, m, n, e);
 }
 
 template <typename T, typename K>
-static int launch_rows_kernel(K kernel, int64_t m, int64_t n, int64_t k, const Operand<T>& a, const Operand<T>& b, const Epilogue<T>& e, int mt, int cols,
+static int launch_rows_kernel(K kernel, int64_t m, int64_t n, int64_t k, int64_t batch, const Operand<T>& a, const Operand<T>& b, const Epilogue<T>& e, int mt, int cols,
                               size_t smem, cudaStream_t st) {
     const int64_t strips = (n + cols - 1) / cols, units = strips * ((m + mt - 1) / mt);
     int cluster = 1;                                             // about three CTAs per SM, each with at least 64 of K
-    while (cluster < 8 && units * cluster < (int64_t)sm_count() * 2 && k > 64 * cluster) cluster *= 2;
-    if (units * cluster > 0x7fffffff) return (int)cudaErrorInvalidValue;
+    while (cluster < 8 && units * batch * cluster < (int64_t)sm_count() * 2 && k > 64 * cluster) cluster *= 2;
+    if (units * cluster > 0x7fffffff || batch > 65535) return (int)cudaErrorInvalidValue;
     if (smem > 40 * 1024) {
         const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (rc != cudaSuccess) { cudaGetLastError(); return (int)rc; }
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(units * cluster));
+    cfg.gridDim = dim3((unsigned)(units * cluster), (unsigned)batch);
     cfg.blockDim = dim3(kBlock);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
@@ -237,32 +242,32 @@ static int launch_rows_kernel(K kernel, int64_t m, int64_t n, int64_t k, const O
 }
 
 template <typename T, int MT>
-static int launch_rows_of(int64_t m, int64_t n, int64_t k, const Operand<T>& a, const Operand<T>& b, const Epilogue<T>& e, cudaStream_t st) {
+static int launch_rows_of(int64_t m, int64_t n, int64_t k, int64_t batch, const Operand<T>& a, const Operand<T>& b, const Epilogue<T>& e, cudaStream_t st) {
     constexpr int V = 16 / sizeof(T);
     if (b.k == 1 && b.row != 1) {
         constexpr int C = MT >= 8 ? 4 : 2;
         const bool packets = aligned16(b.p) && b.row % V == 0;
         constexpr size_t smem = (size_t)MT * kRowsChunk * sizeof(T);
-        if (packets) return launch_rows_kernel<T>(rows_by_dots_kernel<T, MT, C, true>, m, n, k, a, b, e, MT, kWarpsPerBlock * C, smem, st);
-        return launch_rows_kernel<T>(rows_by_dots_kernel<T, MT, C, false>, m, n, k, a, b, e, MT, kWarpsPerBlock * C, smem, st);
+        if (packets) return launch_rows_kernel<T>(rows_by_dots_kernel<T, MT, C, true>, m, n, k, batch, a, b, e, MT, kWarpsPerBlock * C, smem, st);
+        return launch_rows_kernel<T>(rows_by_dots_kernel<T, MT, C, false>, m, n, k, batch, a, b, e, MT, kWarpsPerBlock * C, smem, st);
     }
     constexpr size_t piece = (size_t)MT * kRowsChunk * sizeof(T), sums = (size_t)(kWarpsPerBlock + 1) * MT * 32 * V * sizeof(T);
     constexpr size_t smem = piece > sums ? piece : sums;
     const bool packets = b.row == 1 && aligned16(b.p) && b.k % V == 0 && n % V == 0;
-    if (packets) return launch_rows_kernel<T>(rows_by_columns_kernel<T, MT, true>, m, n, k, a, b, e, MT, 32 * V, smem, st);
-    return launch_rows_kernel<T>(rows_by_columns_kernel<T, MT, false>, m, n, k, a, b, e, MT, 32 * V, smem, st);
+    if (packets) return launch_rows_kernel<T>(rows_by_columns_kernel<T, MT, true>, m, n, k, batch, a, b, e, MT, 32 * V, smem, st);
+    return launch_rows_kernel<T>(rows_by_columns_kernel<T, MT, false>, m, n, k, batch, a, b, e, MT, 32 * V, smem, st);
 }
 
 template <typename T>
-int launch_product_rows(int64_t m, int64_t n, int64_t k, const Operand<T>& a, const Operand<T>& b, const Epilogue<T>& e, cudaStream_t st) {
-    if (m == 1) return launch_rows_of<T, 1>(m, n, k, a, b, e, st);
-    if (m == 2) return launch_rows_of<T, 2>(m, n, k, a, b, e, st);
-    if (m <= 4) return launch_rows_of<T, 4>(m, n, k, a, b, e, st);
-    if (m <= 8 || sizeof(T) == 8) return launch_rows_of<T, 8>(m, n, k, a, b, e, st);
-    if constexpr (sizeof(T) == 4) return launch_rows_of<T, 16>(m, n, k, a, b, e, st);
+int launch_product_rows(int64_t m, int64_t n, int64_t k, int64_t batch, const Operand<T>& a, const Operand<T>& b, const Epilogue<T>& e, cudaStream_t st) {
+    if (m == 1) return launch_rows_of<T, 1>(m, n, k, batch, a, b, e, st);
+    if (m == 2) return launch_rows_of<T, 2>(m, n, k, batch, a, b, e, st);
+    if (m <= 4) return launch_rows_of<T, 4>(m, n, k, batch, a, b, e, st);
+    if (m <= 8 || sizeof(T) == 8) return launch_rows_of<T, 8>(m, n, k, batch, a, b, e, st);
+    if constexpr (sizeof(T) == 4) return launch_rows_of<T, 16>(m, n, k, batch, a, b, e, st);
     return (int)cudaErrorInvalidValue;
 }
-template int launch_product_rows<float>(int64_t, int64_t, int64_t, const Operand<float>&, const Operand<float>&, const Epilogue<float>&, cudaStream_t);
-template int launch_product_rows<double>(int64_t, int64_t, int64_t, const Operand<double>&, const Operand<double>&, const Epilogue<double>&, cudaStream_t);
+template int launch_product_rows<float>(int64_t, int64_t, int64_t, int64_t, const Operand<float>&, const Operand<float>&, const Epilogue<float>&, cudaStream_t);
+template int launch_product_rows<double>(int64_t, int64_t, int64_t, int64_t, const Operand<double>&, const Operand<double>&, const Epilogue<double>&, cudaStream_t);
 
 }  // namespace cb200
