@@ -9,15 +9,16 @@
 namespace cb200 {
 
 // ---- the product on the CUDA cores ------------------------------------------------------------------------------------
-// 64 x 64 outputs per CTA, 4 x 4 per thread, 32 of K at a time through shared memory.  Lanes run along whichever axis of
+// 64 x 64 outputs per CTA, 4 x 4 per thread, 32 (16) of K at a time through shared memory.  Lanes run along whichever axis of
 // each operand is contiguous.  Every 64 of K the sums so far are put aside and new ones begun: the error of a long sum in
 // 32 bits then grows with the square root of its number of pieces, not of its terms.  Bound by the FMA rate at large sizes and by
 // latency at small ones.
-constexpr int kPcM = 64, kPcN = 64, kPcK = 32, kPcPad = 4;
+constexpr int kPcM = 64, kPcN = 64, kPcPad = 4;
 
 template <typename T>
 __global__ void __launch_bounds__(kBlock)
 product_cc_kernel(int64_t m, int64_t n, int64_t k, const Operand<T> A, const Operand<T> B, const Epilogue<T> e, int64_t tiles_n) {
+    constexpr int kPcK = sizeof(T) == 4 ? 32 : 16;               // (8-byte elements: 229 against 411 us for 256 x 2048 x 2048)
     __shared__ T As[kPcK][kPcM + kPcPad];
     __shared__ T Bs[kPcK][kPcN + kPcPad];
     const int64_t i0 = (int64_t)(blockIdx.x / tiles_n) * kPcM, j0 = (int64_t)(blockIdx.x % tiles_n) * kPcN;
@@ -63,7 +64,7 @@ product_cc_kernel(int64_t m, int64_t n, int64_t k, const Operand<T> A, const Ope
 #pragma unroll
                 for (int y = 0; y < 4; ++y) acc[x][y] = av[x] * bv[y] + acc[x][y];
         }
-        if ((k0 / kPcK & 1) == 1) {
+        if ((k0 / kPcK) % (64 / kPcK) == 64 / kPcK - 1) {
 #pragma unroll
             for (int x = 0; x < 4; ++x)
 #pragma unroll
@@ -229,7 +230,10 @@ struct SplitSet {
     }
 };
 
-static bool worth_splitting(int64_t m, int64_t n, int64_t k) { return m >= 32 && n >= 32 && k >= 32 && m * n * k >= (1LL << 22); }
+static bool worth_splitting(int64_t m, int64_t n, int64_t k) {
+    // (measured: 134 x 85 x 674 22 us split and 15 on the CUDA cores, 142 x 367 x 128 26 and 39)
+    return m >= 32 && n >= 32 && k >= 32 && m * n * k >= (k >= 128 ? 1LL << 22 : 1LL << 24);
+}
 
 // Few rows ride along with a pass over the weights (16 to a pass).  Measured in SFloat: 64 x 1024 x 1024 26 us against 39
 // split, 33 x 4096 x 4096 105 against 80, so up to 32 rows always and up to 128 while there are under 2^28 products.
