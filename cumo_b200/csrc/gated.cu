@@ -649,11 +649,10 @@ static int launch_side_by_side(GatedRuns& g, int packet, int64_t shared_runs) {
     }
     // strips as wide as leaves two CTAs per SM with at most eight to a cluster; the gradients hold a third operand in registers
     // and take half as many steps at a time
-    if (sizeof(T) == 8 || (groups + 31) / 32 * 8 >= (int64_t)sm_count()) {
+    if (sizeof(T) == 8 || (groups + 31) / 32 * 8 >= (int64_t)sm_count() || !heads(V / 2)) {
         if (!heads(V)) return (int)cudaErrorNotSupported;
         return launch_strip<T, V, GRAD ? 4 : 8, GM, GRAD>(g);
     }
-    if (!heads(V / 2)) return (int)cudaErrorNotSupported;
     return launch_strip<T, V / 2, GRAD ? 8 : 16, GM, GRAD>(g);
 }
 

@@ -281,7 +281,7 @@ template <typename T>
 static int linear_grad(int64_t m, int64_t n, int64_t k, const T* grad, ssize_t g_row, ssize_t g_col, const T* x, ssize_t x_row, ssize_t x_col,
                        const T* w, ssize_t w_row, ssize_t w_col, const T* pre, ssize_t p_row, ssize_t p_col, int activation, T* dx, T* dw, T* dbias) {
     CB200_TRACE_LAUNCH();
-    if (m < 0 || n < 0 || k < 1 || activation < 0 || activation >= kActCount || (activation != kActNone && !pre)) return (int)cudaErrorInvalidValue;
+    if (m < 0 || n < 0 || k < 1 || activation < 0 || activation >= kActCount || (activation != kActNone && !pre && m && n)) return (int)cudaErrorInvalidValue;
     constexpr ssize_t es = sizeof(T);
     if (g_row % es || g_col % es || x_row % es || x_col % es || w_row % es || w_col % es || p_row % es || p_col % es) return (int)cudaErrorInvalidValue;
     cudaStream_t st = current_stream();

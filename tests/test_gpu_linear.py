@@ -151,6 +151,10 @@ def test_layouts(dt):
     dx, dw, db = linalg.linear_grad(T(0, 9), T(0, 20), T.from_numpy(w))
     assert dx.shape == (0, 20) and not dw.to_numpy().any() and not db.to_numpy().any()
     assert linalg.linear(T.from_numpy(x3), T(20, 0)).shape == (3, 4, 5, 0)
+    dx, dw, db = linalg.linear_grad(T(0, 9), T(0, 20), T.from_numpy(w), activation="silu", pre=T(0, 9))
+    assert dx.shape == (0, 20) and not dw.to_numpy().any() and not db.to_numpy().any()
+    dx, dw, db = linalg.linear_grad(T(5, 0), T.ones(5, 20), T(20, 0), activation="silu", pre=T(5, 0))
+    assert not dx.to_numpy().any() and dw.shape == (20, 0) and db.shape == (0,)
 
 
 @pytest.mark.parametrize("m,k,n", [(4, 300, 500), (300, 257, 260), (512, 512, 512)])
