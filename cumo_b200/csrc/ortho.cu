@@ -121,7 +121,8 @@ struct OrthoScales {
             eq[s] = exponent(q * 1.001);
             ex[s + 1] = exponent(r);
             auto far = [](int e) { return e < -40 || e > 50; };
-            if (!std::isfinite(r) || !std::isfinite(q) || !std::isfinite(a) || far(ep[s]) || far(eq[s]) || far(ex[s + 1]) || std::fabs(a) > 1e12 || std::fabs(b) > 1e12 || std::fabs(c) > 1e12) { fits = false; return; }
+            auto large = [](double v) { return !(std::fabs(v) <= 1e12); };
+            if (!std::isfinite(r) || !std::isfinite(q) || large(a) || large(b) || large(c) || far(ep[s]) || far(eq[s]) || far(ex[s + 1])) { fits = false; return; }
         }
     }
 };

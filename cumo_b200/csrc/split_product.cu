@@ -4,10 +4,17 @@
 // Roles of the 12 warps of a CTA:
 //   warp 0      one thread issues the TMA loads of a K-block (64 elements of K, all planes of both operands) into a ring of
 //               128-byte-swizzled stages
-//   warp 1      allocates tensor memory; one thread issues the tcgen05.mma's: smallest products first
+//   warp 1      allocates tensor memory; one thread issues the tcgen05.mma's, the large products (first part x first part)
+//               into one accumulator, all the small ones into another
 //   warps 2, 3  idle; this warpgroup gives most of its registers to the others
-//   warps 4..11 epilogue: after every K-block they add the accumulator from tensor memory to registers, two accumulators taking turns so that the MMAs never wait; at the end of a tile the sums pass
-//               through a small shared-memory tile per warp, so that global memory is read and written along rows
+//   warps 4..11 epilogue: after every chunk of K-blocks they add the large products' accumulator to registers (two take turns
+//               where tensor memory has room, else the next block's small products run meanwhile); at the end of a tile the
+//               small ones follow and the sums pass through a small shared-memory tile per warp, so that global memory is read
+//               and written along rows
+// What bounds it (cycles counted in the issuing thread): three parts at 8192^3 3257 cycles per K-block of 3072 tensor cycles,
+// 4.4 ms, the power limit (1480 TFLOP/s of bf16 products); two parts at 4096^3 2211 of 1536, 2868 of the surplus per chunk going
+// into waiting for the accumulator: reading one takes some 57 bytes per cycle, which is why a chunk is as long as truncation
+// allows; narrow tiles the operands' way through L2 and shared memory.
 // With CG = 2 two CTAs of a cluster share a 256 x 256 tile: each loads its 128 rows of A and its half of B, the first CTA
 // issues the instructions for both.  Shared memory feeds 64 bytes per cycle to the tensor cores then, instead of the 128 of
 // a 128 x 128 tile (its limit), and each operand byte loaded is used twice as often.  Small problems take 128-row tiles of one
@@ -371,89 +378,89 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
 
     // 384 threads of 168 registers: 128 keep 56 each, which leaves 224 for each of the other 256 (56 + 2 * 224 = 3 * 168)
     if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 0) {
-        // ---- loads ------------------------------------------------------------------------------
-        if (lane == 0) {
-            uint32_t it = 0;
-            bool ok = true;
-            for (int64_t t = 0; t < my_tiles && ok; ++t) {
-                int64_t batch, i0, j0;
-                int piece;
-                tile_of(t, &batch, &i0, &j0, &piece);
-                j0 += rank * S::kBRows;
-                const int end = (piece + 1) * g.per_split < g.kblocks ? (piece + 1) * g.per_split : g.kblocks;
-                for (int kb = piece * g.per_split; kb < end; ++kb, ++it) {
-                    const uint32_t slot = it % S::kStages;
-                    if (!split_wait<false>(empty + slot, ((it / S::kStages) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
-                    if (rank == 0) mbar_expect_tx(full + slot, (uint32_t)(S::kStageBytes * CG));
-                    const uint32_t bar = CG == 2 ? in_cta(smem_u32(full + slot), 0) : smem_u32(full + slot);
-                    uint32_t dst = smem_u32(base + slot * S::kStageBytes);
-                    const int k0 = kb * kSpKB;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 0) {
+            // ---- loads ------------------------------------------------------------------------------
+            if (lane == 0) {
+                uint32_t it = 0;
+                bool ok = true;
+                for (int64_t t = 0; t < my_tiles && ok; ++t) {
+                    int64_t batch, i0, j0;
+                    int piece;
+                    tile_of(t, &batch, &i0, &j0, &piece);
+                    j0 += rank * S::kBRows;
+                    const int end = (piece + 1) * g.per_split < g.kblocks ? (piece + 1) * g.per_split : g.kblocks;
+                    for (int kb = piece * g.per_split; kb < end; ++kb, ++it) {
+                        const uint32_t slot = it % S::kStages;
+                        if (!split_wait<false>(empty + slot, ((it / S::kStages) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                        if (rank == 0) mbar_expect_tx(full + slot, (uint32_t)(S::kStageBytes * CG));
+                        const uint32_t bar = CG == 2 ? in_cta(smem_u32(full + slot), 0) : smem_u32(full + slot);
+                        uint32_t dst = smem_u32(base + slot * S::kStageBytes);
+                        const int k0 = kb * kSpKB;
 #pragma unroll
-                    for (int p = 0; p < P; ++p) {
-                        const int z = (int)(p * g.batch + batch);
-                        if (g.a_k_major) tma_load_3d<CG>(dst, &map_a, bar, k0, (int)i0, z);
-                        else { tma_load_3d<CG>(dst, &map_a, bar, (int)i0, k0, z); tma_load_3d<CG>(dst + 8192, &map_a, bar, (int)i0 + 64, k0, z); }
-                        dst += S::kABytes;
-                    }
-#pragma unroll
-                    for (int p = 0; p < P; ++p) {
-                        const int z = (int)(p * g.batch + batch);
-                        if (g.b_k_major) tma_load_3d<CG>(dst, &map_b, bar, k0, (int)j0, z);
-                        else {
-#pragma unroll
-                            for (int h = 0; h < S::kBRows / 64; ++h) tma_load_3d<CG>(dst + h * 8192, &map_b, bar, (int)j0 + h * 64, k0, z);
+                        for (int p = 0; p < P; ++p) {
+                            const int z = (int)(p * g.batch + batch);
+                            if (g.a_k_major) tma_load_3d<CG>(dst, &map_a, bar, k0, (int)i0, z);
+                            else { tma_load_3d<CG>(dst, &map_a, bar, (int)i0, k0, z); tma_load_3d<CG>(dst + 8192, &map_a, bar, (int)i0 + 64, k0, z); }
+                            dst += S::kABytes;
                         }
-                        dst += S::kBBytes;
+#pragma unroll
+                        for (int p = 0; p < P; ++p) {
+                            const int z = (int)(p * g.batch + batch);
+                            if (g.b_k_major) tma_load_3d<CG>(dst, &map_b, bar, k0, (int)j0, z);
+                            else {
+#pragma unroll
+                                for (int h = 0; h < S::kBRows / 64; ++h) tma_load_3d<CG>(dst + h * 8192, &map_b, bar, (int)j0 + h * 64, k0, z);
+                            }
+                            dst += S::kBBytes;
+                        }
                     }
                 }
+                if (!ok) for (int i = 0; i < 1000; ++i) __nanosleep(1000);      // gave up: copies still in flight land before the CTA leaves
             }
-            if (!ok) for (int i = 0; i < 1000; ++i) __nanosleep(1000);      // gave up: copies still in flight land before the CTA leaves
-        }
-        __syncwarp();
-    } else if (warp == 1) {
-        // ---- products ---------------------------------------------------------------------------
-        if (lane == 0 && rank == 0) {
-            uint32_t it = 0, item = 0;
-            bool ok = true;
-            const int layout = (g.a_k_major ? 1 : 0) | (g.b_k_major ? 2 : 0);
-            for (int64_t t = 0; t < my_tiles && ok; ++t) {
-                const int piece = (int)((cluster + t * clusters) % g.splits);
-                const int begin = piece * g.per_split, end = (piece + 1) * g.per_split < g.kblocks ? (piece + 1) * g.per_split : g.kblocks;
-                int in_chunk = 0;
-                for (int kb = begin; kb < end; ++kb, ++it) {
-                    const uint32_t slot = it % S::kStages;
-                    if (!split_wait<false>(full + slot, (it / S::kStages) & 1u, abort_flag)) { ok = false; break; }
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t sa = smem_u32(base + slot * S::kStageBytes), sb = sa + P * S::kABytes;
-                    // a tile's first block starts with the large products, whose accumulator the epilogue hands back first
-                    constexpr uint32_t kCross = S::kMains * BN;
-                    const uint32_t which = item % S::kMains, turn = item / S::kMains;
-                    if (kb > begin) issue<P, CG, S::kABytes, S::kBBytes, false, false>(layout, sa, sb, tmem_base + kCross, g.idesc);
-                    if (in_chunk == 0) {
-                        if (!split_wait<CG == 2>(main_empty + which, (turn & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+            __syncwarp();
+        } else if (warp == 1) {
+            // ---- products ---------------------------------------------------------------------------
+            if (lane == 0 && rank == 0) {
+                uint32_t it = 0, item = 0;
+                bool ok = true;
+                const int layout = (g.a_k_major ? 1 : 0) | (g.b_k_major ? 2 : 0);
+                for (int64_t t = 0; t < my_tiles && ok; ++t) {
+                    const int piece = (int)((cluster + t * clusters) % g.splits);
+                    const int begin = piece * g.per_split, end = (piece + 1) * g.per_split < g.kblocks ? (piece + 1) * g.per_split : g.kblocks;
+                    int in_chunk = 0;
+                    for (int kb = begin; kb < end; ++kb, ++it) {
+                        const uint32_t slot = it % S::kStages;
+                        if (!split_wait<false>(full + slot, (it / S::kStages) & 1u, abort_flag)) { ok = false; break; }
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint32_t sa = smem_u32(base + slot * S::kStageBytes), sb = sa + P * S::kABytes;
+                        // a tile's first block starts with the large products, whose accumulator the epilogue hands back first
+                        constexpr uint32_t kCross = S::kMains * BN;
+                        const uint32_t which = item % S::kMains, turn = item / S::kMains;
+                        if (kb > begin) issue<P, CG, S::kABytes, S::kBBytes, false, false>(layout, sa, sb, tmem_base + kCross, g.idesc);
+                        if (in_chunk == 0) {
+                            if (!split_wait<CG == 2>(main_empty + which, (turn & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        }
+                        if (in_chunk == 0) issue<P, CG, S::kABytes, S::kBBytes, true, true>(layout, sa, sb, tmem_base + which * BN, g.idesc);
+                        else issue<P, CG, S::kABytes, S::kBBytes, true, false>(layout, sa, sb, tmem_base + which * BN, g.idesc);
+                        if (kb == begin) {
+                            if (!split_wait<CG == 2>(cross_empty, ((uint32_t)t & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                            issue<P, CG, S::kABytes, S::kBBytes, false, true>(layout, sa, sb, tmem_base + kCross, g.idesc);
+                        }
+                        split_commit<CG>(empty + slot);
+                        if (++in_chunk == g.chunk || kb + 1 == end) { split_commit<CG>(main_full + which); in_chunk = 0; ++item; }
                     }
-                    if (in_chunk == 0) issue<P, CG, S::kABytes, S::kBBytes, true, true>(layout, sa, sb, tmem_base + which * BN, g.idesc);
-                    else issue<P, CG, S::kABytes, S::kBBytes, true, false>(layout, sa, sb, tmem_base + which * BN, g.idesc);
-                    if (kb == begin) {
-                        if (!split_wait<CG == 2>(cross_empty, ((uint32_t)t & 1u) ^ 1u, abort_flag)) { ok = false; break; }
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        issue<P, CG, S::kABytes, S::kBBytes, false, true>(layout, sa, sb, tmem_base + kCross, g.idesc);
-                    }
-                    split_commit<CG>(empty + slot);
-                    if (++in_chunk == g.chunk || kb + 1 == end) { split_commit<CG>(main_full + which); in_chunk = 0; ++item; }
+                    if (ok) split_commit<CG>(cross_full);
                 }
-                if (ok) split_commit<CG>(cross_full);
+                // what was issued finishes before tensor memory is freed, whatever happened above
+                if constexpr (CG == 1) asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(drain)) : "memory");
+                else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(drain)) : "memory");
+                split_wait<false>(drain, 0u, abort_flag + 1);
             }
-            // what was issued finishes before tensor memory is freed, whatever happened above
-            if constexpr (CG == 1) asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(drain)) : "memory");
-            else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(drain)) : "memory");
-            split_wait<false>(drain, 0u, abort_flag + 1);
+            __syncwarp();
         }
-        __syncwarp();
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         // ---- epilogue ---------------------------------------------------------------------------

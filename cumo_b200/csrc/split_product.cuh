@@ -6,7 +6,7 @@
 // six bfloat16 products; with two half-precision parts a1 b1 + (a1 b2 + a2 b1), three products.  Products of two 16-bit
 // numbers are exact in the tensor core; what it adds them into is 32 bits wide but truncates, an error that leans one way and
 // grows with the number of additions (2e-8 of the accumulator each, measured).  So the large products a1 b1 have an
-// accumulator of their own, which takes at most 256 of K -- sixteen additions -- before it is added into registers with
+// accumulator of their own, which takes 64 to 512 of K -- four to 32 additions -- before it is added into registers with
 // ordinary rounded additions; what truncation does to the accumulator of the small products is 2^-8 of that and less.
 #pragma once
 
