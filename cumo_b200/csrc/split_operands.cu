@@ -29,6 +29,7 @@ __device__ __forceinline__ float source_at(const SplitSource& s, int64_t i, int6
 // Bound by memory: 4 bytes read and 6 written per element (8 read with an activation's slope); 4096 x 4096 35 us, 4.8 TB/s.
 __global__ void __launch_bounds__(kBlock)
 split_kernel(const SplitJobs jobs) {
+    pdl_trigger();                                               // the product behind sets itself up meanwhile
     const SplitJob& job = jobs.job[blockIdx.y];
     const SplitSource& s = job.s;
     const int64_t C = job.C, ld = job.ld, groups = ld / 8, total = job.R * groups, plane = job.R * ld;
@@ -83,6 +84,7 @@ int launch_split(const SplitJobs& jobs, cudaStream_t st) {
 
 __global__ void __launch_bounds__(kBlock)
 fix_marked_kernel(const FixJobs jobs) {
+    pdl_wait();                                                  // launched while the product in front of it still runs
     if (*jobs.any == 0) return;
     const FixJob& x = jobs.job[blockIdx.y];
     const int64_t total = x.m * x.n;
@@ -99,9 +101,19 @@ fix_marked_kernel(const FixJobs jobs) {
 int launch_fix_marked(const FixJobs& jobs, cudaStream_t st) {
     int64_t most = 0;
     for (int i = 0; i < jobs.count; ++i) { const int64_t t = jobs.job[i].m * jobs.job[i].n; most = t > most ? t : most; }
-    fix_marked_kernel<<<dim3(grid_for((most + kBlock - 1) / kBlock, 2), (unsigned)jobs.count), kBlock, 0, st>>>(jobs);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid_for((most + kBlock - 1) / kBlock, 2), (unsigned)jobs.count);
+    cfg.blockDim = dim3(kBlock);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t rc = cudaLaunchKernelEx(&cfg, fix_marked_kernel, jobs);
+    if (rc != cudaSuccess) { cudaGetLastError(); return (int)rc; }
     count_launch();
-    return (int)cudaGetLastError();
+    return 0;
 }
 
 }  // namespace cb200
