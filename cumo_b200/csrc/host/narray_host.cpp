@@ -1084,13 +1084,16 @@ static bool repeated_steps(const cb200_na* x, int nd, const int64_t* shape, cons
     return fits;
 }
 
+// Is `x` repeated along dimension d of a loop?  Its shape says so, not its steps: a view of the full shape may have steps of 0.
+static bool repeated_at(const cb200_na* x, int nd, const int64_t* shape, int d) {
+    const int od = d - (nd - x->ndim);
+    return shape[d] != 1 && (size_of(x) == 1 || od < 0 || x->shape[od] == 1);
+}
+
 // `full` (of the loop's shape) summed over what `like` was repeated over, in `like`'s shape.  Takes `full` over.
 static cb200_na* sum_to_shape_of(cb200_na* full, const cb200_na* like) {
     uint32_t mask = 0;
-    for (int d = 0; d < full->ndim; ++d) {
-        const int od = d - (full->ndim - like->ndim);
-        if ((size_of(like) == 1 || od < 0 || like->shape[od] == 1) && full->shape[d] != 1) mask |= 1u << d;
-    }
+    for (int d = 0; d < full->ndim; ++d) if (repeated_at(like, full->ndim, full->shape, d)) mask |= 1u << d;
     cb200_na* r = full;
     if (mask) {
         if (!temporaries_allowed("the sum over what an operand was repeated over")) { cb200_na_release(full); return nullptr; }
@@ -1098,6 +1101,10 @@ static cb200_na* sum_to_shape_of(cb200_na* full, const cb200_na* like) {
         if (!size_of(full)) r = make(like->dtype, like->ndim, like->shape, true);
         cb200_na_release(full);
         if (!r) return nullptr;
+    }
+    if (size_of(r) != size_of(like)) {                      // (never: the mask leaves like's extents)
+        cb200_na_release(r);
+        return (cb200_na*)fail("ShapeError", "a gradient does not have its operand's shape");
     }
     r->ndim = like->ndim;                                   // a fresh contiguous array: only extents of 1 come or go
     for (int d = 0; d < like->ndim; ++d) r->shape[d] = like->shape[d];
@@ -1152,7 +1159,7 @@ int cb200_na_gated_cumsum_grad(cb200_na_t* grad, cb200_na_t* gate, cb200_na_t* h
     int64_t gshape[kMaxD];
     int repeated = 0, last_other = -1;
     for (int d = 0; d < grad->ndim; ++d) {
-        const bool rep = gstep[d] == 0 && grad->shape[d] != 1;
+        const bool rep = repeated_at(gate, grad->ndim, grad->shape, d);
         gshape[d] = rep ? 1 : grad->shape[d];
         repeated += rep;
         if (d != axis) last_other = d;

@@ -211,3 +211,30 @@ def test_ones_are_cumsum_and_repeated_calls_agree():
     gate = xp.SFloat.from_numpy(np.random.default_rng(2).uniform(0.8, 1, (3, 5000)).astype(np.float32))
     a, b = X.gated_cumsum(gate, axis=1), X.gated_cumsum(gate, axis=1)
     assert np.array_equal(a.to_numpy(), b.to_numpy())
+
+@pytest.mark.parametrize("dt", [np.float32, np.float64])
+@pytest.mark.parametrize("head", [16, 64, 128, 6])
+@pytest.mark.parametrize("where", ["heads", "time", "batch"])
+def test_gate_of_the_full_shape_with_steps_of_zero(head, where, dt):
+    """An expanded tensor is a gate of its own in every place: its gradient has the full shape, nothing summed, whichever
+    dimension the steps of 0 run along -- heads that a warp could sum included -- and owns every element it shows."""
+    import torch
+
+    import cumo_b200 as xp
+
+    T, u = arrays(xp, dt), ref.U[np.dtype(dt)]
+    shape = (2, 40, 3, head)
+    short = {"heads": (2, 40, 3, 1), "time": (2, 1, 3, head), "batch": (1, 40, 3, head)}[where]
+    rng = np.random.default_rng(head)
+    small = rng.uniform(0.5, 1, short).astype(dt)
+    x, grad = rng.standard_normal(shape).astype(dt), rng.standard_normal(shape).astype(dt)
+    wide = torch.from_numpy(small).cuda().expand(*shape)
+    assert 0 in wide.stride()
+    h = T.from_numpy(x).gated_cumsum(T.from_torch(wide), axis=1)
+    dx, dgate = T.from_numpy(grad).gated_cumsum_grad(T.from_torch(wide), h, axis=1)
+    full = np.broadcast_to(small, shape)
+    want, want_gate, _, mag, before, later = ref.gated_grad(grad, full, h.to_numpy(), 1)
+    bound = np.flip(ref.gated_bound(np.flip(mag, 1), np.flip(later, 1), 1, u), 1)
+    assert dgate.shape == shape
+    assert np.all(np.abs(dx.to_numpy() - want) <= bound)
+    assert np.all(np.abs(dgate.to_numpy() - want_gate) <= (bound + 3 * u * mag) * np.abs(before))
