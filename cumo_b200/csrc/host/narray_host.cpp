@@ -1090,13 +1090,14 @@ static bool repeated_at(const cb200_na* x, int nd, const int64_t* shape, int d) 
     return shape[d] != 1 && (size_of(x) == 1 || od < 0 || x->shape[od] == 1);
 }
 
-// `full` (of the loop's shape) summed over what `like` was repeated over, in `like`'s shape.  Takes `full` over.
+// `full` (of the loop's shape) summed over what `like` was repeated over, in `like`'s shape.  Takes `full` over, a temporary
+// array then: callers ask for it (sum_allowed) before they launch what writes to it, because a launch that a capture has
+// recorded writes at every replay, whatever became of the call.
 static cb200_na* sum_to_shape_of(cb200_na* full, const cb200_na* like) {
     uint32_t mask = 0;
     for (int d = 0; d < full->ndim; ++d) if (repeated_at(like, full->ndim, full->shape, d)) mask |= 1u << d;
     cb200_na* r = full;
     if (mask) {
-        if (!temporaries_allowed("the sum over what an operand was repeated over")) { cb200_na_release(full); return nullptr; }
         r = size_of(full) ? (cb200_na*)cb200_na_reduce("sum", full, mask, 1, 0) : nullptr;
         if (!size_of(full)) r = make(like->dtype, like->ndim, like->shape, true);
         cb200_na_release(full);
@@ -1165,6 +1166,10 @@ int cb200_na_gated_cumsum_grad(cb200_na_t* grad, cb200_na_t* gate, cb200_na_t* h
         if (d != axis) last_other = d;
     }
     const bool fold = repeated == 1 && last_other >= 0 && gshape[last_other] != grad->shape[last_other];
+    bool sums = repeated && !fold;
+    for (int d = 0; initial && d + 1 < grad->ndim; ++d) sums = sums || repeated_at(initial, grad->ndim - 1, state, d);
+    auto sum_allowed = []() { return temporaries_allowed("the sum over what an operand was repeated over"); };
+    if (sums && !sum_allowed()) return 1;
     cb200_na* dx = make(grad->dtype, grad->ndim, grad->shape, false);
     cb200_na* dgate = dx ? make(grad->dtype, grad->ndim, fold ? gshape : grad->shape, size_of(grad) == 0) : nullptr;
     cb200_na* dinit = dgate && initial ? make(grad->dtype, grad->ndim - 1, state, size_of(grad) == 0) : nullptr;
@@ -1190,7 +1195,8 @@ int cb200_na_gated_cumsum_grad(cb200_na_t* grad, cb200_na_t* gate, cb200_na_t* h
                      (ssize_t)dgate->step[axis], (uint64_t)grad->shape[axis], k, oshape, o1, o2, o3, o4, o5, o6, o7);
         };
         int status = launch();
-        if (status == (int)cudaErrorNotSupported && fold) {       // not that many of them: every product, summed below
+        if (status == (int)cudaErrorNotSupported && fold) {       // not that many of them (nothing was launched): every product, summed below
+            if (!sum_allowed()) return give_up();
             cb200_na_release(dgate);
             dgate = make(grad->dtype, grad->ndim, grad->shape, false);
             if (!dgate) return give_up();

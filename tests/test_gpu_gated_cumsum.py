@@ -238,3 +238,47 @@ def test_gate_of_the_full_shape_with_steps_of_zero(head, where, dt):
     assert dgate.shape == shape
     assert np.all(np.abs(dx.to_numpy() - want) <= bound)
     assert np.all(np.abs(dgate.to_numpy() - want_gate) <= (bound + 3 * u * mag) * np.abs(before))
+
+
+@pytest.mark.parametrize("gate_shape,state_shape", [((2, 1, 3, 16), None), ((1, 40, 3, 16), None), ((2, 40, 3, 1), (16,)), ((16,), (2, 3, 16)), ((2, 40, 1, 1), None)])
+def test_a_capture_refuses_sums_before_anything_is_recorded(gate_shape, state_shape):
+    """Gradients that need a temporary array are refused in a capture with nothing launched: the graph that is finished
+    afterwards leaves the memory alone that the refused call had held."""
+    import torch
+
+    import cumo_b200 as xp
+    from cumo_b200 import _lib
+
+    lib = _lib.load()
+    S = xp.SFloat.from_torch
+    shape = (2, 40, 3, 16)
+    x, grad = torch.randn(shape, device="cuda"), torch.randn(shape, device="cuda")
+    gate, own_gate = torch.rand(gate_shape, device="cuda"), torch.rand(shape, device="cuda")
+    state = None if state_shape is None else torch.randn(state_shape, device="cuda")
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        lib.cb200_set_stream(stream.cuda_stream)
+        try:
+            init = None if state is None else S(state)
+            h = S(x).gated_cumsum(S(gate), axis=1, initial=init)
+            want = [g.to_numpy() for g in S(grad).gated_cumsum_grad(S(gate), h, axis=1, initial=init)]
+            S(grad).gated_cumsum_grad(S(own_gate), h, axis=1)       # fills the stream's pool: a capture may not allocate
+            stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                before = _lib.launch_count()
+                with pytest.raises(xp.CudaError):
+                    S(grad).gated_cumsum_grad(S(gate), h, axis=1, initial=init)
+                assert _lib.launch_count() == before
+                kept = S(grad).gated_cumsum_grad(S(own_gate), h, axis=1)
+            others = [xp.SFloat.zeros(*shape) for _ in range(8)]    # whatever the refused call gave back is among these
+            graph.replay()
+            stream.synchronize()
+            assert not any(o.to_numpy().any() for o in others)
+            again = S(grad).gated_cumsum_grad(S(gate), h, axis=1, initial=init)
+            assert all(np.array_equal(a.to_numpy(), b) for a, b in zip(again, want))
+            eager = S(grad).gated_cumsum_grad(S(own_gate), h, axis=1)
+            assert all(np.array_equal(a.to_numpy(), b.to_numpy()) for a, b in zip(kept, eager))
+        finally:
+            lib.cb200_set_stream(None)
