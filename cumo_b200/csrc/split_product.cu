@@ -27,6 +27,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <mutex>
 
 namespace cb200 {
@@ -593,6 +594,8 @@ static bool planes_map(CUtensorMap* map, const Planes& x, int planes, int box_ro
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+static std::atomic<unsigned long long> launched_tiles[3][2];         // 256, 128, 64 columns; whole, one side of the diagonal
+
 template <int P, int CG, int BN, typename Out>
 static int launch_shape(SplitKind kind, const Planes& a, const Planes& b, const Out& out, bool symmetric, int splits, cudaStream_t st) {
     using S = SplitShape<P, CG, BN>;
@@ -649,6 +652,7 @@ static int launch_shape(SplitKind kind, const Planes& a, const Planes& b, const 
     const cudaError_t rc = cudaLaunchKernelEx(&cfg, kernel, g, ma, mb, out);
     if (rc != cudaSuccess) { cudaGetLastError(); return (int)rc; }
     count_launch();
+    launched_tiles[BN == 256 ? 0 : BN == 128 ? 1 : 2][g.symmetric ? 1 : 0].fetch_add(1, std::memory_order_relaxed);
     return 0;
 }
 
@@ -736,4 +740,10 @@ extern "C" int cb200_product_status(void) {
     const int v = *const_cast<volatile int*>(w);
     *const_cast<volatile int*>(w) = 0;
     return v;
+}
+
+// Launches of the product in this process whose tiles are 256 (two CTAs), 128 or 64 columns wide; of those the ones that compute
+// one side of a symmetric result, or the others.
+extern "C" unsigned long long cb200_split_product_launches(int columns, int symmetric) {
+    return cb200::launched_tiles[columns == 256 ? 0 : columns == 128 ? 1 : 2][symmetric ? 1 : 0].load(std::memory_order_relaxed);
 }

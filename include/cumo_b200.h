@@ -638,6 +638,9 @@ CB200_DECL_LINEAR(sfloat, float) CB200_DECL_LINEAR(dfloat, double)
  * process since the last call; 1: one did, and results since then are not valid (the entry points above return
  * cudaErrorLaunchTimeout until this is called); -1: unknown.  Synchronises the device. */
 int cb200_product_status(void);
+/* Launches of that product in this process with tiles of 256 (a pair of CTAs), 128 or 64 columns: those that compute one side of a
+ * symmetric result, or the others. */
+unsigned long long cb200_split_product_launches(int columns, int symmetric);
 
 #ifdef __cplusplus
 }
