@@ -167,6 +167,7 @@ struct SplitMatrix {
     uint16_t* planes;
     int64_t ld;
     Marks marks;
+    uint8_t *hot_row, *hot_col;       // marks of the products' outputs along the axes that the matrix keeps (each axis by one product at most)
     // as operand of a contraction over the matrix's columns (over_columns) or rows
     Planes operand(bool over_columns) const {
         Planes p;
@@ -177,6 +178,7 @@ struct SplitMatrix {
         return p;
     }
     const uint8_t* marks_of(bool over_columns) const { return over_columns != swapped ? marks.row : marks.col; }
+    uint8_t* hot_of(bool over_columns) const { return over_columns != swapped ? hot_row : hot_col; }
     bool turned(bool over_columns) const { return over_columns == swapped; }
 };
 
@@ -197,7 +199,7 @@ struct SplitSet {
     // scratch for all of them, marks cleared by one memset, then one launch that splits them
     int split(Scratch& scratch, cudaStream_t st) {
         size_t marks = 16;
-        for (int i = 0; i < count; ++i) marks += (size_t)(x[i].R + x[i].C);
+        for (int i = 0; i < count; ++i) marks += 2 * (size_t)(x[i].R + x[i].C);
         char* mk = scratch.take(marks);
         if (!mk) return (int)cudaErrorMemoryAllocation;
         const int rc = (int)cudaMemsetAsync(mk, 0, marks, st);
@@ -210,8 +212,11 @@ struct SplitSet {
             SplitMatrix& a = x[i];
             a.planes = reinterpret_cast<uint16_t*>(scratch.take((size_t)3 * a.R * a.ld * 2));
             if (!a.planes) return (int)cudaErrorMemoryAllocation;
-            a.marks = {reinterpret_cast<uint8_t*>(mk), reinterpret_cast<uint8_t*>(mk) + a.R, any};
-            mk += a.R + a.C;
+            uint8_t* at = reinterpret_cast<uint8_t*>(mk);
+            a.marks = {at, at + a.R, any};
+            a.hot_row = at + a.R + a.C;
+            a.hot_col = a.hot_row + a.R;
+            mk += 2 * (a.R + a.C);
             jobs.job[i] = {a.src, a.R, a.C, a.ld, a.planes, a.marks};
         }
         return launch_split(jobs, st);
@@ -220,8 +225,8 @@ struct SplitSet {
     int product(int a, bool a_over_columns, int b, bool b_over_columns, const Epilogue<float>& e, Scratch& scratch, cudaStream_t st) {
         const Planes pa = x[a].operand(a_over_columns), pb = x[b].operand(b_over_columns);
         fixes.job[fixes.count++] = {pa.rows, pb.rows, pa.k, x[a].src, x[b].src, x[a].turned(a_over_columns), x[b].turned(b_over_columns),
-                                    x[a].marks_of(a_over_columns), x[b].marks_of(b_over_columns), e};
-        return launch_split_product(kSplitBf16x3, pa, pb, e, scratch, st);
+                                    x[a].marks_of(a_over_columns), x[b].marks_of(b_over_columns), x[a].hot_of(a_over_columns), x[b].hot_of(b_over_columns), e};
+        return launch_split_product(kSplitBf16x3, pa, pb, e, Hot{x[a].hot_of(a_over_columns), x[b].hot_of(b_over_columns), x[0].marks.any}, scratch, st);
     }
     // what the marks ask for, once all products are queued
     int fix(cudaStream_t st) {

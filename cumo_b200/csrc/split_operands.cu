@@ -90,7 +90,7 @@ fix_marked_kernel(const FixJobs jobs) {
     const int64_t total = x.m * x.n;
     for (int64_t f = (int64_t)blockIdx.x * kBlock + threadIdx.x; f < total; f += (int64_t)gridDim.x * kBlock) {
         const int64_t i = f / x.n, j = f - i * x.n;
-        if (!x.a_marks[i] && !x.b_marks[j]) continue;
+        if (!x.a_marks[i] && !x.b_marks[j] && !(x.hot_row[i] && x.hot_col[j])) continue;
         float acc = 0.f;
         for (int64_t c = 0; c < x.k && acc == acc; ++c)          // (a NaN stays)
             acc = fmaf(x.a_turned ? source_at(x.a, c, i) : source_at(x.a, i, c), x.b_turned ? source_at(x.b, c, j) : source_at(x.b, j, c), acc);

@@ -163,12 +163,18 @@ __device__ __forceinline__ void issue(int layout, uint32_t sa, uint32_t sb, uint
 // alias, several 16-byte packets per lane; rows of the piece are padded by one float, which keeps every access below free of
 // bank conflicts.  The float form:
 struct FloatOut {
+    static constexpr bool kMarks = true;
     Epilogue<float> e;
+    Hot hot;                           // null: nothing is marked (pieces of K, which join_pieces_kernel looks at)
     bool packets;                      // y (and residual) take 16-byte accesses
     struct Ahead {};
     __device__ __forceinline__ void ahead(Ahead&, int, int64_t, int64_t, int64_t, int64_t, int64_t) const {}
-    __device__ __forceinline__ void piece(float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n, bool, Ahead&) const {
+    __device__ __forceinline__ void piece(float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n, bool, bool beyond, Ahead&) const {
         const int rows = m - i0 < 32 ? (int)(m - i0) : 32;
+        if (beyond && hot.any && j0 + lane < n)
+#pragma unroll 1
+            for (int r = 0; r < rows; ++r)
+                if (beyond_range(tile[r * kSpStageCols + lane])) mark_hot(hot, i0 + r, j0 + lane);
         const int64_t y0 = batch * e.y_batch + i0 * e.ld + j0;
         const bool whole = packets && rows == 32 && j0 + 32 <= n;
         if (e.bias || e.pre || e.act != kActNone) {
@@ -231,6 +237,7 @@ struct FloatOut {
 // ... and the form that leaves as two half-precision planes (ld is a multiple of 8, so packets are always aligned; columns
 // between n and ld are padding that nothing reads).
 struct PlaneOut {
+    static constexpr bool kMarks = false;
     PlaneEpilogue e;
     struct Ahead { uint4 h, l; };
     // eight rows of the piece's part of d, requested before they are needed
@@ -241,7 +248,7 @@ struct PlaneOut {
         d.h = *reinterpret_cast<const uint4*>(p);
         d.l = *reinterpret_cast<const uint4*>(p + e.plane);
     }
-    __device__ __forceinline__ void piece(float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n, bool mirror, Ahead& d) const {
+    __device__ __forceinline__ void piece(float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n, bool mirror, bool, Ahead& d) const {
         const int r0 = lane >> 2, c0 = (lane & 3) * 8;
         const int64_t at0 = batch * e.batch_step + (i0 + r0) * e.ld + j0 + c0;
         const bool here = j0 + c0 < e.ld;
@@ -521,15 +528,20 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
             // (one copy of the code that writes a piece: run once per piece, it costs the fetching of its instructions)
 #pragma unroll 1
             for (int q = 0; q < kCols / 32; ++q) {
+                float none = 0.f;                                  // NaN once a sum is not finite
 #pragma unroll
                 for (int w = 0; w < kCols / 32; ++w)
                     if (w == q) {
 #pragma unroll
-                        for (int x = 0; x < 32; ++x) piece[lane * kSpStageCols + x] = sum[w * 32 + x];
+                        for (int x = 0; x < 32; ++x) {
+                            piece[lane * kSpStageCols + x] = sum[w * 32 + x];
+                            if (Out::kMarks) none = fmaf(sum[w * 32 + x], 0.f, none);
+                        }
                     }
+                const bool beyond = Out::kMarks && __any_sync(0xffffffffu, none != 0.f);
                 __syncwarp();
                 if (row0 < g.m) {
-                    out.piece(piece, lane, in, row0, col0 + q * 32, g.m, g.n, g.symmetric && i0 / (128 * CG) != j0 / BN, ahead);
+                    out.piece(piece, lane, in, row0, col0 + q * 32, g.m, g.n, g.symmetric && i0 / (128 * CG) != j0 / BN, beyond, ahead);
                     if (q + 1 < kCols / 32) out.ahead(ahead, lane, in, row0, col0 + (q + 1) * 32, g.m, g.n);
                 }
                 __syncwarp();
@@ -690,7 +702,7 @@ static int launch_any(SplitKind kind, const Planes& a, const Planes& b, const Ou
 
 // The pieces' results added in order, and the epilogue.
 __global__ void __launch_bounds__(kBlock)
-join_pieces_kernel(int64_t m, int64_t n, int splits, const float* pieces, const Epilogue<float> e) {
+join_pieces_kernel(int64_t m, int64_t n, int splits, const float* pieces, const Epilogue<float> e, const Hot hot) {
     const int64_t total = m * n;
     for (int64_t f = (int64_t)blockIdx.x * kBlock + threadIdx.x; f < total; f += (int64_t)gridDim.x * kBlock) {
         float part[8];
@@ -700,11 +712,12 @@ join_pieces_kernel(int64_t m, int64_t n, int splits, const float* pieces, const 
 #pragma unroll
         for (int s = 1; s < 8; ++s) if (s < splits) z += part[s];
         const int64_t i = f / n;
+        if (beyond_range(z)) mark_hot(hot, i, f - i * n);
         finish(e, 0, i, f - i * n, z);
     }
 }
 
-int launch_split_product(SplitKind kind, const Planes& a, const Planes& b, const Epilogue<float>& e, Scratch& scratch, cudaStream_t st) {
+int launch_split_product(SplitKind kind, const Planes& a, const Planes& b, const Epilogue<float>& e, const Hot& hot, Scratch& scratch, cudaStream_t st) {
     if (e.alpha != 1.0f || e.d || a.batch != 1) return (int)cudaErrorInvalidValue;
     Shape shape = choose_shape(kind == kSplitBf16x3 ? 6 : 3, a, b, false, 8);
     Epilogue<float> way = e;
@@ -717,11 +730,11 @@ int launch_split_product(SplitKind kind, const Planes& a, const Planes& b, const
         way = Epilogue<float>{};
         way.alpha = 1.f; way.y = pieces; way.ld = b.rows; way.y_batch = a.rows * b.rows;
     }
-    const FloatOut out = {way, way.ld % 4 == 0 && aligned16(way.y) && way.y_batch % 4 == 0 &&
+    const FloatOut out = {way, pieces ? Hot{} : hot, way.ld % 4 == 0 && aligned16(way.y) && way.y_batch % 4 == 0 &&
                                    (!way.res || (way.res_col == 1 && way.res_row % 4 == 0 && aligned16(way.res)))};
     int rc = kind == kSplitBf16x3 ? launch_any<3>(kind, a, b, out, false, shape, st) : launch_any<2>(kind, a, b, out, false, shape, st);
     if (rc || shape.splits == 1) return rc;
-    join_pieces_kernel<<<grid_for((a.rows * b.rows + kBlock - 1) / kBlock, 8), kBlock, 0, st>>>(a.rows, b.rows, shape.splits, pieces, e);
+    join_pieces_kernel<<<grid_for((a.rows * b.rows + kBlock - 1) / kBlock, 8), kBlock, 0, st>>>(a.rows, b.rows, shape.splits, pieces, e, hot);
     count_launch();
     return (int)cudaGetLastError();
 }

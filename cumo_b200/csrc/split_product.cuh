@@ -38,19 +38,29 @@ struct PlaneEpilogue {
     int64_t batch_step;
 };
 
+// Where outputs beyond the range are marked: rows and columns of the result (see Marks).
+struct Hot { uint8_t* row; uint8_t* col; int* any; };
+__device__ __forceinline__ bool beyond_range(float v) { return !(fabsf(v) <= 3.402823466e38f); }
+__device__ __forceinline__ void mark_hot(const Hot& h, int64_t i, int64_t j) { h.row[i] = 1; h.col[j] = 1; *h.any = 1; }
+
 // C = A . B^T (per batch entry), contraction over k; the result leaves through `e` (float) or `pe` (planes).  Returns a
 // cudaError_t; cudaErrorNotSupported when tensor maps cannot be had, in which case nothing was launched.
-int launch_split_product(SplitKind kind, const Planes& a, const Planes& b, const Epilogue<float>& e, Scratch& scratch, cudaStream_t st);
+// Outputs beyond the range are marked in `hot`.
+int launch_split_product(SplitKind kind, const Planes& a, const Planes& b, const Epilogue<float>& e, const Hot& hot, Scratch& scratch, cudaStream_t st);
 // `symmetric` says that the result is (A = B, or A and B symmetric and equal, and d symmetric): about half the tiles are computed.
 int launch_split_product(const Planes& a, const Planes& b, const PlaneEpilogue& e, bool symmetric, cudaStream_t st);
 
 // Elements that have no parts (infinities, NaN, what bfloat16 rounds to infinity) are left out of the planes and marked by
-// row and by column; fix_marked() then computes the outputs they touch from the operands themselves.
+// row and by column; fix_marked() then computes the outputs they touch from the operands themselves.  So it does for outputs
+// that leave the range as sums of parts: there, and just below its end, the parts' products may overflow to either side of what
+// they add up to.  Those are marked by row and column of the result (`hot`); where a marked row and a marked column cross, the
+// output is computed again.
 struct Marks {
     uint8_t* row;
     uint8_t* col;
     int* any;
 };
+
 // v(i, j) = p[i * row + j * col], times act'(pre(i, j)) when act is not kActNone.
 struct SplitSource {
     const float* p; int64_t row, col;
@@ -68,7 +78,7 @@ struct SplitJob {
 struct SplitJobs { SplitJob job[3]; int count; };
 int launch_split(const SplitJobs& jobs, cudaStream_t st);
 
-// Outputs i, j with a[i] or b[j] marked, in float from the operands: element (row, k) of A at (row, k) of `a`, or (k, row)
+// Outputs i, j with a[i] or b[j] marked, or hot_row[i] and hot_col[j], in float from the operands: element (row, k) of A at (row, k) of `a`, or (k, row)
 // if a_turned; B alike.  Returns at once on the device when nothing was marked.  Up to two products in one launch.
 struct FixJob {
     int64_t m, n, k;
@@ -76,6 +86,8 @@ struct FixJob {
     bool a_turned, b_turned;
     const uint8_t* a_marks;
     const uint8_t* b_marks;
+    const uint8_t* hot_row;
+    const uint8_t* hot_col;
     Epilogue<float> e;
 };
 struct FixJobs { FixJob job[2]; int count; const int* any; };

@@ -196,3 +196,67 @@ def test_wide_recurrences(shape, axis, gate_shape, initial):
     if initial:
         first = np.take(full, 0, axis).astype(np.float64)
         assert np.all(np.abs(got[2].to_numpy() - dinit) <= first * (np.take(bound, 0, axis) + 2 * U * np.take(mag, 0, axis)))
+
+
+@pytest.mark.parametrize("m,k,n", [(300, 257, 260), (1300, 200, 1100), (2100, 130, 2310)])
+def test_products_beyond_the_range(m, k, n):
+    """Finite operands whose products leave the range of the type give infinities, not NaN, and products just inside it stay
+    finite: an output is what 32-bit arithmetic makes of its operands, whatever their parts' products do on the way."""
+    import cumo_b200 as xp
+    from cumo_b200 import linalg
+
+    S = xp.SFloat.from_numpy
+    rng = np.random.default_rng(m)
+    x, w, bias, _ = data(m, k, n, seed=4)
+    sx, sw = rng.choice([-1.0, 1.0], m), rng.choice([-1.0, 1.0], n)
+    big_rows, big_cols = rng.permutation(m)[: m // 3], rng.permutation(n)[: n // 4]
+    x[:, 17], w[17] = 0, 0
+    x[big_rows, 17] = (sx * rng.uniform(1, 2, m) * 1e30)[big_rows]
+    w[17, big_cols] = (sw * rng.uniform(1, 2, n) * 1e30)[big_cols]
+    huge = np.zeros((m, n), bool)
+    huge[np.ix_(big_rows, big_cols)] = True
+    for name in (None, "relu", "sigmoid", "tanh"):
+        with Ran() as ran:
+            y, pre = linalg.linear(S(x), S(w), bias=S(bias), activation=name, keep=True)
+        assert ran.tiles
+        pre, y = pre.to_numpy(), y.to_numpy()
+        sign = np.outer(sx, sw)
+        assert np.array_equal(pre[huge], np.where(sign[huge] > 0, np.inf, -np.inf))
+        z = d(x) @ d(w) + d(bias)
+        assert np.all(np.abs(pre - z)[~huge] <= (ref.product_bound(d(x), d(w), U) + U * np.abs(z))[~huge])
+        ends = {None: (np.inf, -np.inf), "relu": (np.inf, 0), "sigmoid": (1, 0), "tanh": (1, -1)}[name]
+        assert np.array_equal(y[huge], np.where(sign[huge] > 0, *ends))
+    # the largest products that are still finite: 8 and fewer leading bits of their operands, rounded up, are not
+    edge = np.sqrt(np.finfo(np.float32).max.astype(np.float64))
+    x[big_rows, 17] = (sx * edge * (1 - rng.uniform(2.0 ** -20, 2.0 ** -8, m)))[big_rows]
+    w[17, big_cols] = (sw * edge * (1 - rng.uniform(2.0 ** -20, 2.0 ** -8, n)))[big_cols]
+    got = linalg.linear(S(x), S(w)).to_numpy()
+    z = d(x) @ d(w)
+    assert np.all(np.abs(z) < np.finfo(np.float32).max)
+    assert np.all(np.abs(got - z) <= ref.product_bound(d(x), d(w), U))
+
+
+@pytest.mark.parametrize("m,k,n", [(300, 257, 260), (2100, 130, 2310)])
+def test_gradients_beyond_the_range(m, k, n):
+    import cumo_b200 as xp
+    from cumo_b200 import linalg
+
+    S = xp.SFloat.from_numpy
+    rng = np.random.default_rng(n)
+    x, w, _, grad = data(m, k, n, seed=6)
+    grad[:, 5], w[:, 5], x[:, 9] = 0, 0, 0
+    rows, cols = rng.permutation(m)[:40], rng.permutation(k)[:30]
+    rows, cols = rows[rows != 3], cols[cols != 9]
+    sr, sc = rng.choice([-1.0, 1.0], m), rng.choice([-1.0, 1.0], k)
+    grad[rows, 5] = (sr * rng.uniform(1, 2, m) * 1e30)[rows]
+    w[cols, 5] = (sc * rng.uniform(1, 2, k) * 1e30)[cols]
+    x[3, 9], grad[3] = 1e30, (rng.choice([-1.0, 1.0], n) * rng.uniform(1, 2, n) * 1e30).astype(np.float32)
+    grad[3, 5] = 0
+    dx, dw = linalg.linear_grad(S(grad), S(x), S(w), want=("x", "w"))
+    dx, dw = dx.to_numpy(), dw.to_numpy()
+    zx, zw = d(grad) @ d(w).T, d(x).T @ d(grad)
+    top = np.finfo(np.float32).max
+    for got, z, bound in ((dx, zx, ref.product_bound(d(grad), d(w).T, U)), (dw, zw, ref.product_bound(d(x).T, d(grad), U))):
+        far = np.abs(z) > 2 * float(top)
+        assert far.any() and np.array_equal(got[far], np.sign(z[far]) * np.inf)
+        assert np.all(np.abs(got - z)[~far] <= bound[~far])
