@@ -226,7 +226,7 @@ struct SplitSet {
         const Planes pa = x[a].operand(a_over_columns), pb = x[b].operand(b_over_columns);
         fixes.job[fixes.count++] = {pa.rows, pb.rows, pa.k, x[a].src, x[b].src, x[a].turned(a_over_columns), x[b].turned(b_over_columns),
                                     x[a].marks_of(a_over_columns), x[b].marks_of(b_over_columns), x[a].hot_of(a_over_columns), x[b].hot_of(b_over_columns), e};
-        return launch_split_product(kSplitBf16x3, pa, pb, e, Hot{x[a].hot_of(a_over_columns), x[b].hot_of(b_over_columns), x[0].marks.any}, scratch, st);
+        return launch_split_product(pa, pb, e, Hot{x[a].hot_of(a_over_columns), x[b].hot_of(b_over_columns), x[0].marks.any}, scratch, st);
     }
     // what the marks ask for, once all products are queued
     int fix(cudaStream_t st) {

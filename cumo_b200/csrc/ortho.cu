@@ -7,10 +7,6 @@
 // Work per step and matrix of m <= n: 2 m^2 n (P) + 2 m^3 (P P) + 2 m^2 n (the product with X).
 #include "split_product.cuh"
 
-#include <cuda_fp16.h>
-
-#include <cmath>
-
 namespace cb200 {
 
 // ---- |G|_F in 64 bits: slices of a matrix to partial sums of squares, folded in slice order ---------------------------
@@ -83,53 +79,13 @@ static int turn(int64_t batch, int64_t m, int64_t n, const T* in, T* out, cudaSt
     count_launch();
     return (int)cudaGetLastError();
 }
-// ---- single precision: the iteration on half-precision planes ---------------------------------------------------------
-// After the division by |G|_F no singular value is above 1, and what a step makes of them is bounded by the largest value of
-// its polynomial; no entry of a matrix is above its largest singular value.  So every intermediate can be held as two halves
-// (22 bits) under a power of two that the host chooses from the coefficients alone, with entries up to 2^14 and everything
-// down to 2^-25 of that largest entry kept to the full 22 bits: three products per term instead of six.
-struct OrthoScales {
-    // powers of two: an intermediate v is stored as v * 2^e
-    static constexpr int kMostSteps = 64;
-    int ex[kMostSteps + 1], ep[kMostSteps], eq[kMostSteps];
-    bool fits;
-    static int exponent(double bound) {                       // largest e with bound * 2^e <= 2^14
-        if (!(bound > 0)) return 0;
-        int e;
-        std::frexp(bound, &e);
-        return 14 - e;
-    }
-    OrthoScales(int steps, const double* coefs) : fits(steps >= 1 && steps <= kMostSteps) {
-        if (!fits) return;
-        double r = 1.001;                                     // (rounding of the norm and of the parts)
-        ex[0] = exponent(r);
-        for (int s = 0; s < steps; ++s) {
-            const double a = coefs[3 * s], b = coefs[3 * s + 1], c = coefs[3 * s + 2], t = r * r;
-            double q = std::fabs(b * t + c * t * t);
-            if (c != 0 && -b / (2 * c) > 0 && -b / (2 * c) < t) q = std::fmax(q, std::fabs(b * b / (4 * c)));
-            auto poly = [&](double x) { return std::fabs(x * (a + x * x * (b + x * x * c))); };
-            double top = poly(r);
-            auto at = [&](double u) { if (u > 0 && u < t) top = std::fmax(top, poly(std::sqrt(u))); };
-            if (c != 0) {
-                const double disc = 9 * b * b - 20 * a * c;
-                if (disc >= 0) { at((-3 * b + std::sqrt(disc)) / (10 * c)); at((-3 * b - std::sqrt(disc)) / (10 * c)); }
-            } else if (b != 0) {
-                at(-a / (3 * b));
-            }
-            r = top * 1.001;
-            ep[s] = exponent(t * 1.001);
-            eq[s] = exponent(q * 1.001);
-            ex[s + 1] = exponent(r);
-            auto far = [](int e) { return e < -40 || e > 50; };
-            auto large = [](double v) { return !(std::fabs(v) <= 1e12); };
-            if (!std::isfinite(r) || !std::isfinite(q) || large(a) || large(b) || large(c) || far(ep[s]) || far(eq[s]) || far(ex[s + 1])) { fits = false; return; }
-        }
-    }
-};
 
-// X0 * 2^e as two planes [plane][batch][m][ld] through 32 x 32 tiles, lanes along whichever axis of G is contiguous.
+// ---- single precision: the iteration on planes ------------------------------------------------------------------------
+// X, P and Q are held as three bfloat16 parts each, all 24 bits of a float under its own exponent: rows, columns and single
+// elements that are small beside the others, and matrices that are small beside eps, keep the digits that they have in 32 bits.
+// X0 as planes [plane][batch][m][ld] through 32 x 32 tiles, lanes along whichever axis of G is contiguous.
 __global__ void __launch_bounds__(kBlock)
-scale_planes_kernel(const Operand<float> G, int64_t m, int64_t n, int64_t tiles_n, int slices, const double* sums, double eps, float scale, uint16_t* planes,
+scale_planes_kernel(const Operand<float> G, int64_t m, int64_t n, int64_t tiles_n, int slices, const double* sums, double eps, uint16_t* planes,
                     int64_t ld, int64_t plane) {
     __shared__ double inv;
     __shared__ float tile[32][33];
@@ -149,30 +105,31 @@ scale_planes_kernel(const Operand<float> G, int64_t m, int64_t n, int64_t tiles_
         if (down) tile[lane][r] = v; else tile[r][lane] = v;
     }
     __syncthreads();
-    __half* out = reinterpret_cast<__half*>(planes) + (int64_t)blockIdx.y * m * ld;
+    uint16_t* out = planes + (int64_t)blockIdx.y * m * ld;
     for (int r = warp; r < 32; r += kWarpsPerBlock) {
         const int64_t i = i0 + r, j = j0 + lane;
         if (i >= m || j >= n) continue;
-        const double v = (double)tile[r][lane] * inv;
-        const float f = (float)v * scale;
-        const __half hi = __float2half_rn(f);
-        out[i * ld + j] = hi;
-        out[plane + i * ld + j] = __float2half_rn(f - __half2float(hi));
+        uint32_t a, b, c;
+        split3_all((float)((double)tile[r][lane] * inv), a, b, c);
+        out[i * ld + j] = (uint16_t)a;
+        out[plane + i * ld + j] = (uint16_t)b;
+        out[2 * plane + i * ld + j] = (uint16_t)c;
     }
 }
 
-// out[b][i][j] (or [j][i]) = (hi + lo) * scale
+// out[b][i][j] (or [j][i]) = the sum of the parts
 __global__ void __launch_bounds__(kBlock)
-join_planes_kernel(int64_t m, int64_t n, int64_t tiles_n, const uint16_t* planes, int64_t ld, int64_t plane, float scale, bool tall, float* out) {
+join_planes_kernel(int64_t m, int64_t n, int64_t tiles_n, const uint16_t* planes, int64_t ld, int64_t plane, bool tall, float* out) {
     __shared__ float tile[32][33];
     const int64_t i0 = (int64_t)(blockIdx.x / tiles_n) * 32, j0 = (int64_t)(blockIdx.x % tiles_n) * 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const __half* in = reinterpret_cast<const __half*>(planes) + (int64_t)blockIdx.y * m * ld;
+    const uint16_t* in = planes + (int64_t)blockIdx.y * m * ld;
     out += (int64_t)blockIdx.y * m * n;
     for (int r = warp; r < 32; r += kWarpsPerBlock) {
         const int64_t i = i0 + r, j = j0 + lane;
         if (i < m && j < n) {
-            const float v = (__half2float(in[i * ld + j]) + __half2float(in[plane + i * ld + j])) * scale;
+            const uint16_t* p = in + i * ld + j;
+            const float v = bf16_at(p[0]) + (bf16_at(p[plane]) + bf16_at(p[2 * plane]));
             if (tall) tile[r][lane] = v; else out[i * n + j] = v;
         }
     }
@@ -183,39 +140,37 @@ join_planes_kernel(int64_t m, int64_t n, int64_t tiles_n, const uint16_t* planes
 }
 
 static int orthogonalize_split(int64_t batch, int64_t m, int64_t n, bool tall, const Operand<float>& G, int steps, const double* coefs, double eps, int slices,
-                               const double* sums, const OrthoScales& sc, float* out, Scratch& scratch, cudaStream_t st) {
+                               const double* sums, float* out, Scratch& scratch, cudaStream_t st) {
     int rc = product_gave_up();
     if (rc) return rc;
     const int64_t ldx = planes_ld(n), ldp = planes_ld(m), px = batch * m * ldx, pp = batch * m * ldp;
-    uint16_t* x = reinterpret_cast<uint16_t*>(scratch.take((size_t)px * 4));
-    uint16_t* x2 = reinterpret_cast<uint16_t*>(scratch.take((size_t)px * 4));
-    uint16_t* p = reinterpret_cast<uint16_t*>(scratch.take((size_t)pp * 4));
-    uint16_t* q = reinterpret_cast<uint16_t*>(scratch.take((size_t)pp * 4));
+    uint16_t* x = reinterpret_cast<uint16_t*>(scratch.take((size_t)px * 6));
+    uint16_t* x2 = reinterpret_cast<uint16_t*>(scratch.take((size_t)px * 6));
+    uint16_t* p = reinterpret_cast<uint16_t*>(scratch.take((size_t)pp * 6));
+    uint16_t* q = reinterpret_cast<uint16_t*>(scratch.take((size_t)pp * 6));
     if (!x || !x2 || !p || !q) return (int)cudaErrorMemoryAllocation;
     const int64_t tm = (m + 31) / 32, tn = (n + 31) / 32;
     if (tm * tn > 0x7fffffff) return (int)cudaErrorInvalidValue;
     const dim3 grid((unsigned)(tm * tn), (unsigned)batch);
-    auto two = [](int e) { return (float)std::ldexp(1.0, e); };
-    scale_planes_kernel<<<grid, kBlock, 0, st>>>(G, m, n, tn, slices, sums, eps, two(sc.ex[0]), x, ldx, px);
+    scale_planes_kernel<<<grid, kBlock, 0, st>>>(G, m, n, tn, slices, sums, eps, x, ldx, px);
     count_launch();
     rc = (int)cudaGetLastError();
     for (int s = 0; s < steps && rc == 0; ++s) {
         const float a = (float)coefs[3 * s], b = (float)coefs[3 * s + 1], c = (float)coefs[3 * s + 2];
         const Planes X = {x, m, n, batch, ldx, true}, Xn = {x, n, m, batch, ldx, false}, P = {p, m, m, batch, ldp, true}, Q = {q, m, m, batch, ldp, true};
         PlaneEpilogue e = {};
-        e.acc_scale = two(-2 * sc.ex[s]); e.out_scale = two(sc.ep[s]); e.out = p; e.ld = ldp; e.plane = pp; e.batch_step = m * ldp;          // P = X X^T
+        e.alpha = 1.f; e.out = p; e.ld = ldp; e.plane = pp; e.batch_step = m * ldp;              // P = X X^T
         rc = launch_split_product(X, X, e, true, st);
         if (rc) break;
-        e.acc_scale = c * two(-2 * sc.ep[s]); e.beta = b; e.d = p; e.d_scale = two(-sc.ep[s]); e.out_scale = two(sc.eq[s]); e.out = q;      // Q = b P + c P P
+        e.alpha = c; e.beta = b; e.d = p; e.out = q;                                             // Q = b P + c P P
         rc = launch_split_product(P, P, e, true, st);
         if (rc) break;
-        e.acc_scale = two(-sc.eq[s] - sc.ex[s]); e.beta = a; e.d = x; e.d_scale = two(-sc.ex[s]); e.out_scale = two(sc.ex[s + 1]);           // X <- a X + Q X
-        e.out = x2; e.ld = ldx; e.plane = px; e.batch_step = m * ldx;
+        e.alpha = 1.f; e.beta = a; e.d = x; e.out = x2; e.ld = ldx; e.plane = px; e.batch_step = m * ldx;      // X <- a X + Q X
         rc = launch_split_product(Q, Xn, e, false, st);
         uint16_t* t = x; x = x2; x2 = t;
     }
     if (rc) return rc;
-    join_planes_kernel<<<grid, kBlock, 0, st>>>(m, n, tn, x, ldx, px, two(-sc.ex[steps]), tall, out);
+    join_planes_kernel<<<grid, kBlock, 0, st>>>(m, n, tn, x, ldx, px, tall, out);
     count_launch();
     return (int)cudaGetLastError();
 }
@@ -255,11 +210,10 @@ static int orthogonalize(int64_t batch, int64_t rows, int64_t columns, const T* 
                                                                                   (int)slices, sums);
     count_launch();
     if constexpr (sizeof(T) == 4) {
-        const OrthoScales sc(steps, coefs);
         // Matrices of few rows have short sums behind their results, and ordinary fp32 FMAs round those better than the tensor
         // cores truncate them (80 x 1408: error 1.1e-6 against 1.8e-6); P's long sums are cut over clusters.
         const bool few = m <= 128 && batch * m * m * n <= (1LL << 26);
-        if (sc.fits && !few) return orthogonalize_split(batch, m, n, tall, G, steps, coefs, eps, (int)slices, sums, sc, out, scratch, st);
+        if (!few) return orthogonalize_split(batch, m, n, tall, G, steps, coefs, eps, (int)slices, sums, out, scratch, st);
     }
     T* x = reinterpret_cast<T*>(scratch.take((size_t)batch * m * n * es));
     T* x2 = reinterpret_cast<T*>(scratch.take((size_t)batch * m * n * es));

@@ -1,23 +1,7 @@
 // Operands of the tensor-core product: floats into bfloat16 planes, and the outputs that infinities and NaN reach.
 #include "split_product.cuh"
 
-#include <cuda_bf16.h>
-
 namespace cb200 {
-
-// a = a1 + a2 + a3 with each part the bfloat16 nearest to what the parts before it leave: 8 bits each, so that three hold
-// all 24 (parts under 2^-126 are lost, which only operands under 2^-102 have).  What rounds to infinity in the first part has
-// no such parts.
-__device__ __forceinline__ bool split3(float v, uint32_t& a, uint32_t& b, uint32_t& c) {
-    const bool fine = (__float_as_uint(v) & 0x7fffffffu) < 0x7f7f8000u;
-    if (!fine) v = 0.f;
-    const __nv_bfloat16 x = __float2bfloat16_rn(v);
-    const float r = v - __bfloat162float(x);
-    const __nv_bfloat16 y = __float2bfloat16_rn(r);
-    const __nv_bfloat16 z = __float2bfloat16_rn(r - __bfloat162float(y));
-    a = __bfloat16_as_ushort(x); b = __bfloat16_as_ushort(y); c = __bfloat16_as_ushort(z);
-    return fine;
-}
 
 __device__ __forceinline__ float source_at(const SplitSource& s, int64_t i, int64_t j) {
     float v = s.p[i * s.row + j * s.col];

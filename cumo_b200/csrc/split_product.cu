@@ -24,9 +24,6 @@
 #include "tc_common.cuh"
 #include "tile_tma.cuh"
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <atomic>
 #include <mutex>
 
@@ -36,11 +33,11 @@ constexpr int kSpThreads = 384;                 // a warpgroup for loads and pro
 constexpr int kSpKB = 64;                       // K per stage: one 128-byte swizzle row of 16-bit elements
 constexpr int kSpStageCols = 33;                // epilogue tile: 32 x 32 floats, rows padded by one
 
-template <int P, int CG, int BN>
+template <int CG, int BN>
 struct SplitShape {
     static constexpr int kBRows = BN / CG;                               // rows of B a CTA loads
     static constexpr int kABytes = 128 * 128, kBBytes = kBRows * 128;    // per plane
-    static constexpr int kStageBytes = P * (kABytes + kBBytes);
+    static constexpr int kStageBytes = kParts * (kABytes + kBBytes);
     static constexpr int kEpilogueBytes = 8 * 32 * kSpStageCols * 4;
     static constexpr int kStages = (232448 - 1024 - kEpilogueBytes) / kStageBytes < 4 ? (232448 - 1024 - kEpilogueBytes) / kStageBytes : 4;
     static constexpr int kMains = BN == 256 ? 1 : 2;                     // accumulators of large products, taking turns where there is room
@@ -134,11 +131,11 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint32_t a_low, uint32_
 }
 
 // The large product of a stage (MAIN) or all its small ones, 64 of K; FRESH: the first instruction starts the accumulator anew.
-template <int P, int CG, int A_BYTES, int B_BYTES, bool AK, bool BK, bool MAIN, bool FRESH>
+template <int CG, int A_BYTES, int B_BYTES, bool AK, bool BK, bool MAIN, bool FRESH>
 __device__ __forceinline__ void issue_stage(uint32_t sa, uint32_t sb, uint32_t d_tmem, uint32_t idesc) {
-    constexpr int kTerms = P == 3 ? 6 : 3;
-    constexpr int ta[6] = {P == 3 ? 2 : 1, 0, P == 3 ? 1 : 0, 1, 0, 0};
-    constexpr int tb[6] = {0, P == 3 ? 2 : 1, P == 3 ? 1 : 0, 0, 1, 0};
+    constexpr int kTerms = 6;
+    constexpr int ta[kTerms] = {2, 0, 1, 1, 0, 0};
+    constexpr int tb[kTerms] = {0, 2, 1, 0, 1, 0};
     const uint32_t a0 = desc_low<AK>(sa), b0 = desc_low<BK>(sb);
 #pragma unroll
     for (int term = MAIN ? kTerms - 1 : 0; term < (MAIN ? kTerms : kTerms - 1); ++term)
@@ -149,13 +146,13 @@ __device__ __forceinline__ void issue_stage(uint32_t sa, uint32_t sb, uint32_t d
             else mma_f16<CG, false>(d_tmem, a, b, idesc);
         }
 }
-template <int P, int CG, int A_BYTES, int B_BYTES, bool MAIN, bool FRESH>
+template <int CG, int A_BYTES, int B_BYTES, bool MAIN, bool FRESH>
 __device__ __forceinline__ void issue(int layout, uint32_t sa, uint32_t sb, uint32_t d_tmem, uint32_t idesc) {
     switch (layout) {                                            // bit 0: A K-major, bit 1: B K-major
-        case 0: issue_stage<P, CG, A_BYTES, B_BYTES, false, false, MAIN, FRESH>(sa, sb, d_tmem, idesc); break;
-        case 1: issue_stage<P, CG, A_BYTES, B_BYTES, true, false, MAIN, FRESH>(sa, sb, d_tmem, idesc); break;
-        case 2: issue_stage<P, CG, A_BYTES, B_BYTES, false, true, MAIN, FRESH>(sa, sb, d_tmem, idesc); break;
-        default: issue_stage<P, CG, A_BYTES, B_BYTES, true, true, MAIN, FRESH>(sa, sb, d_tmem, idesc); break;
+        case 0: issue_stage<CG, A_BYTES, B_BYTES, false, false, MAIN, FRESH>(sa, sb, d_tmem, idesc); break;
+        case 1: issue_stage<CG, A_BYTES, B_BYTES, true, false, MAIN, FRESH>(sa, sb, d_tmem, idesc); break;
+        case 2: issue_stage<CG, A_BYTES, B_BYTES, false, true, MAIN, FRESH>(sa, sb, d_tmem, idesc); break;
+        default: issue_stage<CG, A_BYTES, B_BYTES, true, true, MAIN, FRESH>(sa, sb, d_tmem, idesc); break;
     }
 }
 
@@ -234,19 +231,19 @@ struct FloatOut {
     }
 };
 
-// ... and the form that leaves as two half-precision planes (ld is a multiple of 8, so packets are always aligned; columns
-// between n and ld are padding that nothing reads).
+// ... and the form that leaves as planes (ld is a multiple of 8, so packets are always aligned; columns between n and ld are
+// padding that nothing reads).
 struct PlaneOut {
     static constexpr bool kMarks = false;
     PlaneEpilogue e;
-    struct Ahead { uint4 h, l; };
+    struct Ahead { uint4 part[kParts]; };
     // eight rows of the piece's part of d, requested before they are needed
     __device__ __forceinline__ void ahead(Ahead& d, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t) const {
         const int r0 = lane >> 2, c0 = (lane & 3) * 8;
         if (!e.d || j0 + c0 >= e.ld || i0 + r0 >= m) return;
         const uint16_t* p = e.d + batch * e.batch_step + (i0 + r0) * e.ld + j0 + c0;
-        d.h = *reinterpret_cast<const uint4*>(p);
-        d.l = *reinterpret_cast<const uint4*>(p + e.plane);
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) d.part[q] = *reinterpret_cast<const uint4*>(p + q * e.plane);
     }
     __device__ __forceinline__ void piece(float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n, bool mirror, bool, Ahead& d) const {
         const int r0 = lane >> 2, c0 = (lane & 3) * 8;
@@ -254,24 +251,28 @@ struct PlaneOut {
         const bool here = j0 + c0 < e.ld;
 #pragma unroll 1
         for (int q = 0; q < 4; ++q) {
-            Ahead cur = d;
-            if (q < 3) ahead(d, lane, batch, i0 + (q + 1) * 8, j0, m, n);
-            if (!here || i0 + q * 8 + r0 >= m) continue;
+            const bool live = here && i0 + q * 8 + r0 < m;
             float* t = tile + (q * 8 + r0) * kSpStageCols + c0;
             float v[8];
-            const __half2* ph = reinterpret_cast<const __half2*>(&cur.h);
-            const __half2* pl = reinterpret_cast<const __half2*>(&cur.l);
+            if (live) {
 #pragma unroll
-            for (int x = 0; x < 8; ++x) v[x] = t[x] * e.acc_scale;
-            if (e.d)
+                for (int x = 0; x < 8; ++x) v[x] = t[x] * e.alpha;
+                if (e.d) {
+                    const uint32_t* part[kParts];
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const float2 a = __half22float2(ph[x]), b = __half22float2(pl[x]);
-                    v[2 * x] += e.beta * ((a.x + b.x) * e.d_scale);
-                    v[2 * x + 1] += e.beta * ((a.y + b.y) * e.d_scale);
+                    for (int w = 0; w < kParts; ++w) part[w] = reinterpret_cast<const uint32_t*>(&d.part[w]);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {                // smallest part first: the sum is the number itself
+                        float lo = 0.f, hi = 0.f;
+#pragma unroll
+                        for (int w = kParts - 1; w >= 0; --w) { lo += bf16_at(part[w][x] & 0xffffu); hi += __uint_as_float(part[w][x] & 0xffff0000u); }
+                        v[2 * x] = fmaf(e.beta, lo, v[2 * x]);
+                        v[2 * x + 1] = fmaf(e.beta, hi, v[2 * x + 1]);
+                    }
                 }
-#pragma unroll
-            for (int x = 0; x < 8; ++x) v[x] *= e.out_scale;
+            }
+            if (q < 3) ahead(d, lane, batch, i0 + (q + 1) * 8, j0, m, n);
+            if (!live) continue;
             store(v, at0 + q * 8 * e.ld);
             if (mirror)
 #pragma unroll
@@ -290,24 +291,23 @@ struct PlaneOut {
         }
     }
     __device__ __forceinline__ void store(const float (&v)[8], int64_t at) const {
-        uint4 oh, ol;
-        __half2* qh = reinterpret_cast<__half2*>(&oh);
-        __half2* ql = reinterpret_cast<__half2*>(&ol);
+        uint32_t out[kParts][4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-            qh[x] = __floats2half2_rn(v[2 * x], v[2 * x + 1]);
-            const float2 f = __half22float2(qh[x]);
-            ql[x] = __floats2half2_rn(v[2 * x] - f.x, v[2 * x + 1] - f.y);
+            uint32_t a0, b0, c0, a1, b1, c1;
+            split3_all(v[2 * x], a0, b0, c0);
+            split3_all(v[2 * x + 1], a1, b1, c1);
+            out[0][x] = a0 | a1 << 16; out[1][x] = b0 | b1 << 16; out[2][x] = c0 | c1 << 16;
         }
-        *reinterpret_cast<uint4*>(e.out + at) = oh;
-        *reinterpret_cast<uint4*>(e.out + at + e.plane) = ol;
+#pragma unroll
+        for (int w = 0; w < kParts; ++w) *reinterpret_cast<uint4*>(e.out + at + w * e.plane) = make_uint4(out[w][0], out[w][1], out[w][2], out[w][3]);
     }
 };
 
-template <int P, int CG, int BN, typename Out>
+template <int CG, int BN, typename Out>
 __global__ void __launch_bounds__(kSpThreads, 1)
 split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Out out) {
-    using S = SplitShape<P, CG, BN>;
+    using S = SplitShape<CG, BN>;
     extern __shared__ __align__(1024) char smem_raw[];
     char* base = smem_raw;
     float* pieces = reinterpret_cast<float*>(base + S::kStages * S::kStageBytes);
@@ -406,14 +406,14 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
                         uint32_t dst = smem_u32(base + slot * S::kStageBytes);
                         const int k0 = kb * kSpKB;
 #pragma unroll
-                        for (int p = 0; p < P; ++p) {
+                        for (int p = 0; p < kParts; ++p) {
                             const int z = (int)(p * g.batch + batch);
                             if (g.a_k_major) tma_load_3d<CG>(dst, &map_a, bar, k0, (int)i0, z);
                             else { tma_load_3d<CG>(dst, &map_a, bar, (int)i0, k0, z); tma_load_3d<CG>(dst + 8192, &map_a, bar, (int)i0 + 64, k0, z); }
                             dst += S::kABytes;
                         }
 #pragma unroll
-                        for (int p = 0; p < P; ++p) {
+                        for (int p = 0; p < kParts; ++p) {
                             const int z = (int)(p * g.batch + batch);
                             if (g.b_k_major) tma_load_3d<CG>(dst, &map_b, bar, k0, (int)j0, z);
                             else {
@@ -441,21 +441,21 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
                         const uint32_t slot = it % S::kStages;
                         if (!split_wait<false>(full + slot, (it / S::kStages) & 1u, abort_flag)) { ok = false; break; }
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint32_t sa = smem_u32(base + slot * S::kStageBytes), sb = sa + P * S::kABytes;
+                        const uint32_t sa = smem_u32(base + slot * S::kStageBytes), sb = sa + kParts * S::kABytes;
                         // a tile's first block starts with the large products, whose accumulator the epilogue hands back first
                         constexpr uint32_t kCross = S::kMains * BN;
                         const uint32_t which = item % S::kMains, turn = item / S::kMains;
-                        if (kb > begin) issue<P, CG, S::kABytes, S::kBBytes, false, false>(layout, sa, sb, tmem_base + kCross, g.idesc);
+                        if (kb > begin) issue<CG, S::kABytes, S::kBBytes, false, false>(layout, sa, sb, tmem_base + kCross, g.idesc);
                         if (in_chunk == 0) {
                             if (!split_wait<CG == 2>(main_empty + which, (turn & 1u) ^ 1u, abort_flag)) { ok = false; break; }
                             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         }
-                        if (in_chunk == 0) issue<P, CG, S::kABytes, S::kBBytes, true, true>(layout, sa, sb, tmem_base + which * BN, g.idesc);
-                        else issue<P, CG, S::kABytes, S::kBBytes, true, false>(layout, sa, sb, tmem_base + which * BN, g.idesc);
+                        if (in_chunk == 0) issue<CG, S::kABytes, S::kBBytes, true, true>(layout, sa, sb, tmem_base + which * BN, g.idesc);
+                        else issue<CG, S::kABytes, S::kBBytes, true, false>(layout, sa, sb, tmem_base + which * BN, g.idesc);
                         if (kb == begin) {
                             if (!split_wait<CG == 2>(cross_empty, ((uint32_t)t & 1u) ^ 1u, abort_flag)) { ok = false; break; }
                             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                            issue<P, CG, S::kABytes, S::kBBytes, false, true>(layout, sa, sb, tmem_base + kCross, g.idesc);
+                            issue<CG, S::kABytes, S::kBBytes, false, true>(layout, sa, sb, tmem_base + kCross, g.idesc);
                         }
                         split_commit<CG>(empty + slot);
                         if (++in_chunk == g.chunk || kb + 1 == end) { split_commit<CG>(main_full + which); in_chunk = 0; ++item; }
@@ -594,46 +594,44 @@ int product_gave_up() {
     return w && *const_cast<const volatile int*>(w) ? (int)cudaErrorLaunchTimeout : 0;
 }
 
-static bool planes_map(CUtensorMap* map, const Planes& x, int planes, int box_rows, SplitKind kind) {
+static bool planes_map(CUtensorMap* map, const Planes& x, int box_rows) {
     TensorMapEncodeFn enc = tensor_map_encoder();
     if (!enc || !aligned16(x.p) || x.ld % 8 != 0) return false;
-    if (x.inner() > (1LL << 31) - 1024 || x.outer() > (1LL << 31) - 1024 || planes * x.batch > 0x7fffffff) return false;
-    cuuint64_t dim[3] = {(cuuint64_t)x.inner(), (cuuint64_t)x.outer(), (cuuint64_t)(planes * x.batch)};
+    if (x.inner() > (1LL << 31) - 1024 || x.outer() > (1LL << 31) - 1024 || kParts * x.batch > 0x7fffffff) return false;
+    cuuint64_t dim[3] = {(cuuint64_t)x.inner(), (cuuint64_t)x.outer(), (cuuint64_t)(kParts * x.batch)};
     cuuint64_t stride[2] = {(cuuint64_t)x.ld * 2, (cuuint64_t)(x.outer() * x.ld * 2)};
     cuuint32_t box[3] = {64, (cuuint32_t)(x.k_major ? box_rows : kSpKB), 1};
     cuuint32_t estr[3] = {1, 1, 1};
-    return enc(map, kind == kSplitBf16x3 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, x.p, dim, stride, box, estr,
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, x.p, dim, stride, box, estr,
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 static std::atomic<unsigned long long> launched_tiles[3][2];         // 256, 128, 64 columns; whole, one side of the diagonal
 
-template <int P, int CG, int BN, typename Out>
-static int launch_shape(SplitKind kind, const Planes& a, const Planes& b, const Out& out, bool symmetric, int splits, cudaStream_t st) {
-    using S = SplitShape<P, CG, BN>;
+template <int CG, int BN, typename Out>
+static int launch_shape(const Planes& a, const Planes& b, const Out& out, bool symmetric, int splits, cudaStream_t st) {
+    using S = SplitShape<CG, BN>;
     SplitArgs g;
     memset(&g, 0, sizeof g);
     g.m = a.rows; g.n = b.rows; g.batch = a.batch;
     g.kblocks = (int)((a.k + kSpKB - 1) / kSpKB);
     g.tiles_m = (a.rows + 128 * CG - 1) / (128 * CG);
     g.tiles_n = (b.rows + BN - 1) / BN;
-    // Half pairs feed products whose errors add up over an iteration.  Where tiles are narrow, because there are few, reading an
-    // accumulator costs little and hides behind the other one: every block or two.  Full tiles belong to large matrices, whose own
-    // rounding in 32 bits is larger: four blocks, eight from 4096 on (4096 x 4096: error 1.4e-6 instead of 7e-7, where 32-bit sums
-    // have 3.2e-6).  The three-part products of a single layer take four.
-    g.chunk = kind != kSplitHalfx2 ? 4 : BN == 64 ? 1 : BN == 128 ? (g.kblocks > 16 ? 2 : 1) : g.kblocks >= 64 ? 8 : g.kblocks > 4 ? 4 : 1;
+// K-blocks to an accumulator: four, a fraction of a rounding of what a single layer's product is good to.  Products whose
+    // errors add up over an iteration take fewer where tiles are narrow, because there are few: reading an accumulator costs little
+    // there and hides behind the other one.
+    g.chunk = Out::kMarks || (BN == 256 && g.kblocks > 4) ? 4 : BN == 128 && g.kblocks > 16 ? 2 : 1;
     g.symmetric = symmetric && BN == 128 * CG;
     g.per_split = (g.kblocks + splits - 1) / splits;
     g.splits = (g.kblocks + g.per_split - 1) / g.per_split;             // no piece is empty
     g.n_tiles = g.splits * (g.symmetric ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n) * a.batch;
     g.a_k_major = a.k_major; g.b_k_major = b.k_major;
-    const uint32_t fmt = kind == kSplitBf16x3 ? 1u : 0u;
-    g.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((a.k_major ? 0u : 1u) << 15) | ((b.k_major ? 0u : 1u) << 16) | ((uint32_t)(BN >> 3) << 17) |
+    g.idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((a.k_major ? 0u : 1u) << 15) | ((b.k_major ? 0u : 1u) << 16) | ((uint32_t)(BN >> 3) << 17) |
               ((uint32_t)((128 * CG) >> 4) << 24);
     if (!gave_up_word(&g.gave_up)) return (int)cudaErrorMemoryAllocation;
     CUtensorMap ma, mb;
-    if (!planes_map(&ma, a, P, 128, kind) || !planes_map(&mb, b, P, S::kBRows, kind)) return (int)cudaErrorNotSupported;
-    auto kernel = split_product_kernel<P, CG, BN, Out>;
+    if (!planes_map(&ma, a, 128) || !planes_map(&mb, b, S::kBRows)) return (int)cudaErrorNotSupported;
+    auto kernel = split_product_kernel<CG, BN, Out>;
     static std::mutex mu;
     static bool ready[64] = {};
     int dev = 0;
@@ -674,7 +672,7 @@ static int launch_shape(SplitKind kind, const Planes& a, const Planes& b, const 
 // pieces, writing and adding up their results (about 2500 bytes per cycle) and one more launch.
 struct Shape { int tile, splits; };
 
-static Shape choose_shape(int terms, const Planes& a, const Planes& b, bool symmetric, int most_splits) {
+static Shape choose_shape(const Planes& a, const Planes& b, bool symmetric, int most_splits) {
     const int64_t sms = sm_count(), kblocks = (a.k + kSpKB - 1) / kSpKB;
     const int64_t tm[3] = {256, 128, 128}, tn[3] = {256, 128, 64}, cycles[3] = {128, 95, 70}, slots[3] = {sms / 2, sms, sms};
     Shape best = {0, 1};
@@ -684,7 +682,7 @@ static Shape choose_shape(int terms, const Planes& a, const Planes& b, bool symm
         const int64_t tiles = (symmetric && tm[t] == tn[t] ? across * (across + 1) / 2 : across * ((b.rows + tn[t] - 1) / tn[t])) * a.batch;
         for (int s = 1; s <= most_splits && (s == 1 || kblocks / s >= 2); ++s) {
             const int64_t rounds = (tiles * s + slots[t] - 1) / slots[t];
-            int64_t cost = rounds * ((kblocks + s - 1) / s * 4 * terms * cycles[t] + 3000);
+            int64_t cost = rounds * ((kblocks + s - 1) / s * 24 * cycles[t] + 3000);
             if (s > 1) cost += 6000 + (int64_t)(s + 1) * a.rows * b.rows * 4 / 2500;
             if (cost < least) { least = cost; best = {t, s}; }
         }
@@ -692,12 +690,12 @@ static Shape choose_shape(int terms, const Planes& a, const Planes& b, bool symm
     return best;
 }
 
-template <int P, typename Out>
-static int launch_any(SplitKind kind, const Planes& a, const Planes& b, const Out& out, bool symmetric, Shape shape, cudaStream_t st) {
+template <typename Out>
+static int launch_any(const Planes& a, const Planes& b, const Out& out, bool symmetric, Shape shape, cudaStream_t st) {
     if (a.k != b.k || a.batch != b.batch || a.k < 1 || (symmetric && a.rows != b.rows)) return (int)cudaErrorInvalidValue;
-    if (shape.tile == 0) return launch_shape<P, 2, 256, Out>(kind, a, b, out, symmetric, shape.splits, st);
-    if (shape.tile == 1) return launch_shape<P, 1, 128, Out>(kind, a, b, out, symmetric, shape.splits, st);
-    return launch_shape<P, 1, 64, Out>(kind, a, b, out, symmetric, shape.splits, st);
+    if (shape.tile == 0) return launch_shape<2, 256, Out>(a, b, out, symmetric, shape.splits, st);
+    if (shape.tile == 1) return launch_shape<1, 128, Out>(a, b, out, symmetric, shape.splits, st);
+    return launch_shape<1, 64, Out>(a, b, out, symmetric, shape.splits, st);
 }
 
 // The pieces' results added in order, and the epilogue.
@@ -717,9 +715,9 @@ join_pieces_kernel(int64_t m, int64_t n, int splits, const float* pieces, const 
     }
 }
 
-int launch_split_product(SplitKind kind, const Planes& a, const Planes& b, const Epilogue<float>& e, const Hot& hot, Scratch& scratch, cudaStream_t st) {
+int launch_split_product(const Planes& a, const Planes& b, const Epilogue<float>& e, const Hot& hot, Scratch& scratch, cudaStream_t st) {
     if (e.alpha != 1.0f || e.d || a.batch != 1) return (int)cudaErrorInvalidValue;
-    Shape shape = choose_shape(kind == kSplitBf16x3 ? 6 : 3, a, b, false, 8);
+    Shape shape = choose_shape(a, b, false, 8);
     Epilogue<float> way = e;
     float* pieces = nullptr;
     if (shape.splits > 1) {
@@ -732,7 +730,7 @@ int launch_split_product(SplitKind kind, const Planes& a, const Planes& b, const
     }
     const FloatOut out = {way, pieces ? Hot{} : hot, way.ld % 4 == 0 && aligned16(way.y) && way.y_batch % 4 == 0 &&
                                    (!way.res || (way.res_col == 1 && way.res_row % 4 == 0 && aligned16(way.res)))};
-    int rc = kind == kSplitBf16x3 ? launch_any<3>(kind, a, b, out, false, shape, st) : launch_any<2>(kind, a, b, out, false, shape, st);
+    int rc = launch_any(a, b, out, false, shape, st);
     if (rc || shape.splits == 1) return rc;
     join_pieces_kernel<<<grid_for((a.rows * b.rows + kBlock - 1) / kBlock, 8), kBlock, 0, st>>>(a.rows, b.rows, shape.splits, pieces, e, hot);
     count_launch();
@@ -740,7 +738,7 @@ int launch_split_product(SplitKind kind, const Planes& a, const Planes& b, const
 }
 int launch_split_product(const Planes& a, const Planes& b, const PlaneEpilogue& e, bool symmetric, cudaStream_t st) {
     const PlaneOut out = {e};
-    return launch_any<2>(kSplitHalfx2, a, b, out, symmetric, choose_shape(3, a, b, symmetric, 1), st);
+    return launch_any(a, b, out, symmetric, choose_shape(a, b, symmetric, 1), st);
 }
 
 }  // namespace cb200

@@ -1,9 +1,10 @@
-// Single-precision products on the 16-bit tensor cores: operands held as a few 16-bit parts ("planes") each.
+// Single-precision products on the 16-bit tensor cores: operands held as three 16-bit parts ("planes") each.
 //
-// A float is the sum of three bfloat16 numbers to its last bit (8 + 8 + 8 bits, the float's own exponent range), and of two
-// half-precision numbers to 2^-22 of it while it is well inside their narrower range.  With a = a1 + a2 + a3, b alike,
+// A float is the sum of three bfloat16 numbers to its last bit (8 + 8 + 8 bits, the float's own exponent range).  With
+// a = a1 + a2 + a3, b alike,
 //     a b = a1 b1 + (a1 b2 + a2 b1) + (a2 b2 + a1 b3 + a3 b1) + terms of 2^-24 a b and below,
-// six bfloat16 products; with two half-precision parts a1 b1 + (a1 b2 + a2 b1), three products.  Products of two 16-bit
+// six bfloat16 products.  (Two half-precision parts would take three, but hold 22 bits only of numbers within 2^16 of the largest
+// under a common power of two: rows of a matrix that are small beside the others would lose theirs.)  Products of two 16-bit
 // numbers are exact in the tensor core; what it adds them into is 32 bits wide but truncates, an error that leans one way and
 // grows with the number of additions (2e-8 of the accumulator each, measured).  So the large products a1 b1 have an
 // accumulator of their own, which takes 64 to 512 of K -- four to 32 additions -- before it is added into registers with
@@ -12,9 +13,37 @@
 
 #include "linear.cuh"
 
+#include <cuda_bf16.h>
+
 namespace cb200 {
 
-enum SplitKind { kSplitBf16x3 = 0, kSplitHalfx2 = 1 };
+constexpr int kParts = 3;
+
+// a = a1 + a2 + a3 with each part the bfloat16 nearest to what the parts before it leave: 8 bits each, so that three hold
+// all 24 (parts under 2^-126 are lost, which only operands under 2^-102 have).  What rounds to infinity in the first part has
+// no such parts: false, and zeros.
+__device__ __forceinline__ bool split3(float v, uint32_t& a, uint32_t& b, uint32_t& c) {
+    const bool fine = (__float_as_uint(v) & 0x7fffffffu) < 0x7f7f8000u;
+    if (!fine) v = 0.f;
+    const __nv_bfloat16 x = __float2bfloat16_rn(v);
+    const float r = v - __bfloat162float(x);
+    const __nv_bfloat16 y = __float2bfloat16_rn(r);
+    const __nv_bfloat16 z = __float2bfloat16_rn(r - __bfloat162float(y));
+    a = __bfloat16_as_ushort(x); b = __bfloat16_as_ushort(y); c = __bfloat16_as_ushort(z);
+    return fine;
+}
+// The same for what must not be left out: infinities and NaN are their own first part, and what only rounds to infinity is cut off.
+__device__ __forceinline__ void split3_all(float v, uint32_t& a, uint32_t& b, uint32_t& c) {
+    if (split3(v, a, b, c)) return;
+    const uint32_t bits = __float_as_uint(v), mag = bits & 0x7fffffffu;
+    a = (bits >> 16) | (mag > 0x7f800000u ? 0x40u : 0u);
+    if (mag >= 0x7f800000u) return;
+    const float r = v - __uint_as_float(bits & 0xffff0000u);
+    const __nv_bfloat16 y = __float2bfloat16_rn(r);
+    b = __bfloat16_as_ushort(y);
+    c = __bfloat16_as_ushort(__float2bfloat16_rn(r - __bfloat162float(y)));
+}
+__device__ __forceinline__ float bf16_at(uint32_t bits) { return __uint_as_float(bits << 16); }
 
 // A matrix of `rows` x `k` (per batch entry) as planes in global memory.  k_major: rows of k contiguous elements, ld apart;
 // otherwise k rows of `rows` contiguous elements.  Plane p of batch entry b starts at (p * batch + b) * rows_or_k * ld.
@@ -28,11 +57,10 @@ struct Planes {
 };
 inline int64_t planes_ld(int64_t inner) { return (inner + 7) / 8 * 8; }
 
-// Out of a product of planes into planes (orthogonalisation): v = acc * acc_scale + beta * d * d_scale, stored as two
-// halves of v * out_scale.  All scales are powers of two.
+// Out of a product of planes into planes (orthogonalisation): alpha * acc + beta * d.
 struct PlaneEpilogue {
-    float acc_scale, beta, d_scale, out_scale;
-    const uint16_t* d;                  // planes of the same shape as the output (two), or null
+    float alpha, beta;
+    const uint16_t* d;                  // planes of the same shape as the output, or null
     uint16_t* out;
     int64_t ld, plane;                  // elements per row; elements from one plane to the next
     int64_t batch_step;
@@ -46,7 +74,7 @@ __device__ __forceinline__ void mark_hot(const Hot& h, int64_t i, int64_t j) { h
 // C = A . B^T (per batch entry), contraction over k; the result leaves through `e` (float) or `pe` (planes).  Returns a
 // cudaError_t; cudaErrorNotSupported when tensor maps cannot be had, in which case nothing was launched.
 // Outputs beyond the range are marked in `hot`.
-int launch_split_product(SplitKind kind, const Planes& a, const Planes& b, const Epilogue<float>& e, const Hot& hot, Scratch& scratch, cudaStream_t st);
+int launch_split_product(const Planes& a, const Planes& b, const Epilogue<float>& e, const Hot& hot, Scratch& scratch, cudaStream_t st);
 // `symmetric` says that the result is (A = B, or A and B symmetric and equal, and d symmetric): about half the tiles are computed.
 int launch_split_product(const Planes& a, const Planes& b, const PlaneEpilogue& e, bool symmetric, cudaStream_t st);
 

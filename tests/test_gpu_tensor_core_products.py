@@ -260,3 +260,77 @@ def test_gradients_beyond_the_range(m, k, n):
         far = np.abs(z) > 2 * float(top)
         assert far.any() and np.array_equal(got[far], np.sign(z[far]) * np.inf)
         assert np.all(np.abs(got - z)[~far] <= bound[~far])
+
+
+# kinds of matrices whose entries differ in size: what 32-bit arithmetic keeps of the small ones is kept
+def uneven(kind, shape, rng):
+    g = rng.standard_normal(shape).astype(np.float32)
+    rows, cols = np.ones(shape[-2]), np.ones(shape[-1])
+    rows[1::2], cols[::3] = 2.0 ** -17, 2.0 ** -20                   # about 1e-5 and 1e-6 of the others
+    if kind == "rows":
+        return (g * rows[:, None]).astype(np.float32), rows[:, None] < 1
+    if kind == "columns":
+        return (g * cols).astype(np.float32), np.broadcast_to(cols < 1, g.shape[-2:])
+    apart = (rows[:, None] < 1) != (cols < 1)                        # two blocks that hardly touch
+    return np.where(apart, g * np.float32(2.0 ** -24), g), apart
+
+
+@pytest.mark.parametrize("steps", [1, 5, 15])
+@pytest.mark.parametrize("shape", [(256, 512), (512, 256), (1030, 1500), (2100, 2300), (3, 300, 500)])
+@pytest.mark.parametrize("kind", ["rows", "columns", "blocks"])
+def test_entries_of_different_sizes(kind, shape, steps):
+    """Rows, columns or blocks that are 1e-5 to 1e-7 of the rest, as dead units and rare tokens leave them: each group's error
+    relative to the group itself is what plain 32-bit arithmetic's is, within the factor that roundings of another order take."""
+    import torch
+
+    import cumo_b200 as xp
+    from cumo_b200 import linalg
+
+    torch.backends.cuda.matmul.allow_tf32 = False
+    g, small = uneven(kind, shape, np.random.default_rng(3 + sum(shape)))
+    want, plain = in_64_bits(g, steps, MUON)
+    got = linalg.orthogonalize(xp.SFloat.from_numpy(g), steps=steps).to_numpy()
+    for group in (small, ~small):
+        mask = np.broadcast_to(group, g.shape[-2:])
+        off, most, size = (np.sqrt((a[..., mask] ** 2).sum(-1)) for a in (got - want, plain - want, want))
+        assert np.all(off <= 4 * most)
+        if steps == 5 and kind == "rows":
+            assert np.all(off <= 2e-6 * size)
+
+
+@pytest.mark.parametrize("norm", [1e-5, 1e-9, 1e-12, 1e-14, 1e-17, 1e-22])
+@pytest.mark.parametrize("shape", [(200, 300), (300, 200), (40, 60)])
+def test_matrices_far_below_eps(shape, norm):
+    """g / (|g| + eps) is about g / eps then, however small: its digits stay."""
+    import torch
+
+    import cumo_b200 as xp
+    from cumo_b200 import linalg
+
+    torch.backends.cuda.matmul.allow_tf32 = False
+    g = np.random.default_rng(7).standard_normal(shape)
+    g = (g / np.linalg.norm(g) * norm).astype(np.float32)
+    for steps in (1, 5):
+        want, plain = in_64_bits(g, steps, MUON)
+        got = linalg.orthogonalize(xp.SFloat.from_numpy(g), steps=steps).to_numpy()
+        assert np.linalg.norm(got - want) <= 4 * np.linalg.norm(plain - want)
+
+
+def test_more_steps_and_larger_coefficients_than_usual():
+    import torch
+
+    import cumo_b200 as xp
+    from cumo_b200 import linalg
+
+    torch.backends.cuda.matmul.allow_tf32 = False
+    g = np.random.default_rng(11).standard_normal((200, 300)).astype(np.float32)
+    for steps, coefs in ((70, (1.5, -0.5, 0.0)), (2, (3e6, -1e7, 8e6))):
+        want, plain = in_64_bits(g, steps, coefs)
+        with Ran() as ran:
+            got = linalg.orthogonalize(xp.SFloat.from_numpy(g), steps=steps, coefs=coefs).to_numpy()
+        assert ran.tiles == {(64, 0)}
+        assert np.linalg.norm(got - want) <= 4 * np.linalg.norm(plain - want)
+    # a last step close to the end of the range
+    got = linalg.orthogonalize(xp.SFloat.from_numpy(g), steps=2, coefs=[(1.0, 0.0, 0.0), (3e38, 0.0, 0.0)]).to_numpy()
+    x = g.astype(np.float64) / (np.linalg.norm(g.astype(np.float64)) + 1e-7)
+    assert np.all(np.abs(got - 3e38 * x) <= 1e-5 * np.abs(3e38 * x))
