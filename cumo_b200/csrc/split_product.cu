@@ -156,22 +156,27 @@ __device__ __forceinline__ void issue(int layout, uint32_t sa, uint32_t sb, uint
     }
 }
 
+// Marks a piece of the result that holds a number beyond the range (out of line: hardly ever called, and code in the way costs
+// its fetching).
+__device__ __noinline__ void mark_piece(const Hot hot, int64_t i0, int rows, int64_t j0, int cols) {
+    for (int r = 0; r < rows; ++r) hot.row[i0 + r] = 1;
+    for (int c = 0; c < cols; ++c) hot.col[j0 + c] = 1;
+    *hot.any = 1;
+}
+
 // Out: how a finished 32-row x 32-column piece leaves shared memory.  Loads are issued ahead of the stores that they might
 // alias, several 16-byte packets per lane; rows of the piece are padded by one float, which keeps every access below free of
 // bank conflicts.  The float form:
 struct FloatOut {
-    static constexpr bool kMarks = true;
+    static constexpr bool kIterated = false;
     Epilogue<float> e;
-    Hot hot;                           // null: nothing is marked (pieces of K, which join_pieces_kernel looks at)
+    Hot hot;                           // (a piece of K that leaves the range marks what it is added to)
     bool packets;                      // y (and residual) take 16-byte accesses
     struct Ahead {};
     __device__ __forceinline__ void ahead(Ahead&, int, int64_t, int64_t, int64_t, int64_t, int64_t) const {}
-    __device__ __forceinline__ void piece(float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n, bool, bool beyond, Ahead&) const {
+    __device__ __forceinline__ void piece(float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n, bool, Ahead&) const {
         const int rows = m - i0 < 32 ? (int)(m - i0) : 32;
-        if (beyond && hot.any && j0 + lane < n)
-#pragma unroll 1
-            for (int r = 0; r < rows; ++r)
-                if (beyond_range(tile[r * kSpStageCols + lane])) mark_hot(hot, i0 + r, j0 + lane);
+        float none = 0.f;                                         // NaN once a sum is not finite, then the whole piece is marked
         const int64_t y0 = batch * e.y_batch + i0 * e.ld + j0;
         const bool whole = packets && rows == 32 && j0 + 32 <= n;
         if (e.bias || e.pre || e.act != kActNone) {
@@ -183,6 +188,7 @@ struct FloatOut {
 #pragma unroll 2
                 for (int r = 0; r < rows; ++r, t += kSpStageCols) {
                     float z = *t;
+                    none = fmaf(z, 0.f, none);
                     if (e.bias) z += bias;
                     if (pre) { *pre = z; pre += e.ld; }
                     if (e.act != kActNone) z = activate(z, e.act);
@@ -204,10 +210,12 @@ struct FloatOut {
                     const int r = h + q * 4 + r0;
                     const float* t = tile + r * kSpStageCols + c0;
                     float4 v = make_float4(t[0], t[1], t[2], t[3]);
+                    none = fmaf((v.x + v.y) + (v.z + v.w), 0.f, none);
                     if (e.res) { v.x += res[q].x; v.y += res[q].y; v.z += res[q].z; v.w += res[q].w; }
                     *reinterpret_cast<float4*>(e.y + y0 + r * e.ld + c0) = v;
                 }
             }
+            if (none != 0.f) mark_piece(hot, i0, rows, j0, 32);
             return;
         }
         if (j0 + lane >= n) return;
@@ -220,6 +228,7 @@ struct FloatOut {
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
                 v[q] = tile[(h + q) * kSpStageCols + lane];
+                none = fmaf(v[q], 0.f, none);
                 w[q] = res && h + q < rows ? res[q * e.res_row] : 0.f;
             }
             if (res) res += 8 * e.res_row;
@@ -228,13 +237,14 @@ struct FloatOut {
                 if (h + q < rows) y[q * e.ld] = e.res ? v[q] + w[q] : v[q];
             y += 8 * e.ld;
         }
+        if (none != 0.f) mark_piece(hot, i0, rows, j0, n - j0 < 32 ? (int)(n - j0) : 32);
     }
 };
 
 // ... and the form that leaves as planes (ld is a multiple of 8, so packets are always aligned; columns between n and ld are
 // padding that nothing reads).
 struct PlaneOut {
-    static constexpr bool kMarks = false;
+    static constexpr bool kIterated = true;      // its results go into further products
     PlaneEpilogue e;
     struct Ahead { uint4 part[kParts]; };
     // eight rows of the piece's part of d, requested before they are needed
@@ -245,7 +255,7 @@ struct PlaneOut {
 #pragma unroll
         for (int q = 0; q < kParts; ++q) d.part[q] = *reinterpret_cast<const uint4*>(p + q * e.plane);
     }
-    __device__ __forceinline__ void piece(float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n, bool mirror, bool, Ahead& d) const {
+    __device__ __forceinline__ void piece(float* tile, int lane, int64_t batch, int64_t i0, int64_t j0, int64_t m, int64_t n, bool mirror, Ahead& d) const {
         const int r0 = lane >> 2, c0 = (lane & 3) * 8;
         const int64_t at0 = batch * e.batch_step + (i0 + r0) * e.ld + j0 + c0;
         const bool here = j0 + c0 < e.ld;
@@ -528,20 +538,15 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
             // (one copy of the code that writes a piece: run once per piece, it costs the fetching of its instructions)
 #pragma unroll 1
             for (int q = 0; q < kCols / 32; ++q) {
-                float none = 0.f;                                  // NaN once a sum is not finite
 #pragma unroll
                 for (int w = 0; w < kCols / 32; ++w)
                     if (w == q) {
 #pragma unroll
-                        for (int x = 0; x < 32; ++x) {
-                            piece[lane * kSpStageCols + x] = sum[w * 32 + x];
-                            if (Out::kMarks) none = fmaf(sum[w * 32 + x], 0.f, none);
-                        }
+                        for (int x = 0; x < 32; ++x) piece[lane * kSpStageCols + x] = sum[w * 32 + x];
                     }
-                const bool beyond = Out::kMarks && __any_sync(0xffffffffu, none != 0.f);
                 __syncwarp();
                 if (row0 < g.m) {
-                    out.piece(piece, lane, in, row0, col0 + q * 32, g.m, g.n, g.symmetric && i0 / (128 * CG) != j0 / BN, beyond, ahead);
+                    out.piece(piece, lane, in, row0, col0 + q * 32, g.m, g.n, g.symmetric && i0 / (128 * CG) != j0 / BN, ahead);
                     if (q + 1 < kCols / 32) out.ahead(ahead, lane, in, row0, col0 + (q + 1) * 32, g.m, g.n);
                 }
                 __syncwarp();
@@ -620,7 +625,7 @@ static int launch_shape(const Planes& a, const Planes& b, const Out& out, bool s
 // K-blocks to an accumulator: four, a fraction of a rounding of what a single layer's product is good to.  Products whose
     // errors add up over an iteration take fewer where tiles are narrow, because there are few: reading an accumulator costs little
     // there and hides behind the other one.
-    g.chunk = Out::kMarks || (BN == 256 && g.kblocks > 4) ? 4 : BN == 128 && g.kblocks > 16 ? 2 : 1;
+    g.chunk = !Out::kIterated || (BN == 256 && g.kblocks > 4) ? 4 : BN == 128 && g.kblocks > 16 ? 2 : 1;
     g.symmetric = symmetric && BN == 128 * CG;
     g.per_split = (g.kblocks + splits - 1) / splits;
     g.splits = (g.kblocks + g.per_split - 1) / g.per_split;             // no piece is empty
@@ -700,7 +705,7 @@ static int launch_any(const Planes& a, const Planes& b, const Out& out, bool sym
 
 // The pieces' results added in order, and the epilogue.
 __global__ void __launch_bounds__(kBlock)
-join_pieces_kernel(int64_t m, int64_t n, int splits, const float* pieces, const Epilogue<float> e, const Hot hot) {
+join_pieces_kernel(int64_t m, int64_t n, int splits, const float* pieces, const Epilogue<float> e) {
     const int64_t total = m * n;
     for (int64_t f = (int64_t)blockIdx.x * kBlock + threadIdx.x; f < total; f += (int64_t)gridDim.x * kBlock) {
         float part[8];
@@ -710,7 +715,6 @@ join_pieces_kernel(int64_t m, int64_t n, int splits, const float* pieces, const 
 #pragma unroll
         for (int s = 1; s < 8; ++s) if (s < splits) z += part[s];
         const int64_t i = f / n;
-        if (beyond_range(z)) mark_hot(hot, i, f - i * n);
         finish(e, 0, i, f - i * n, z);
     }
 }
@@ -728,11 +732,11 @@ int launch_split_product(const Planes& a, const Planes& b, const Epilogue<float>
         way = Epilogue<float>{};
         way.alpha = 1.f; way.y = pieces; way.ld = b.rows; way.y_batch = a.rows * b.rows;
     }
-    const FloatOut out = {way, pieces ? Hot{} : hot, way.ld % 4 == 0 && aligned16(way.y) && way.y_batch % 4 == 0 &&
+    const FloatOut out = {way, hot, way.ld % 4 == 0 && aligned16(way.y) && way.y_batch % 4 == 0 &&
                                    (!way.res || (way.res_col == 1 && way.res_row % 4 == 0 && aligned16(way.res)))};
     int rc = launch_any(a, b, out, false, shape, st);
     if (rc || shape.splits == 1) return rc;
-    join_pieces_kernel<<<grid_for((a.rows * b.rows + kBlock - 1) / kBlock, 8), kBlock, 0, st>>>(a.rows, b.rows, shape.splits, pieces, e, hot);
+    join_pieces_kernel<<<grid_for((a.rows * b.rows + kBlock - 1) / kBlock, 8), kBlock, 0, st>>>(a.rows, b.rows, shape.splits, pieces, e);
     count_launch();
     return (int)cudaGetLastError();
 }

@@ -68,8 +68,6 @@ struct PlaneEpilogue {
 
 // Where outputs beyond the range are marked: rows and columns of the result (see Marks).
 struct Hot { uint8_t* row; uint8_t* col; int* any; };
-__device__ __forceinline__ bool beyond_range(float v) { return !(fabsf(v) <= 3.402823466e38f); }
-__device__ __forceinline__ void mark_hot(const Hot& h, int64_t i, int64_t j) { h.row[i] = 1; h.col[j] = 1; *h.any = 1; }
 
 // C = A . B^T (per batch entry), contraction over k; the result leaves through `e` (float) or `pe` (planes).  Returns a
 // cudaError_t; cudaErrorNotSupported when tensor maps cannot be had, in which case nothing was launched.
