@@ -11,8 +11,10 @@
 // A stretch of steps maps the state before it to the state after it by h -> A*h + B, with A the product of its gates and B
 // its result from a zero state.  Stretches are folded in parallel with these pairs to find the state in front of each;
 // every stretch is then walked again, from registers, starting from that state, so that each output is the formula's own
-// sequence of rounded steps.  A is a product of many factors in (0, 1) as a rule: for 32-bit elements it and the
-// composition are held in 64 bits, where it neither underflows in a way that could be seen in 32 bits nor loses digits.
+// sequence of rounded steps.  Pairs are composed in 64 bits.  Within a stretch of up to sixteen steps A and B are folded in the
+// element type (a rounding per step, as the walk itself makes), A in 64 bits where the runs are contiguous; for 32-bit elements
+// they are folded again in 64 bits where a product of gates comes near the ends of the range, or B leaves it: the state of the run
+// may be in range all the same.  (64-bit elements have nothing wider to go to: sums from zero have to stay in their range.)
 //
 // Three plans, all bound by memory traffic (3 s bytes per element forward, 5 s backward):
 //   walk    a thread per run (or per 16-byte group of neighbouring runs), in order: many runs, or few steps
@@ -307,8 +309,22 @@ gated_strip_kernel(const GatedRuns g, int cluster_size) {
             }
             warp_A[warp][x][lane] = starts ? 0.0 : wide;
         }
+        T none = T(0);                                           // NaN once a B is not finite
 #pragma unroll
-        for (int v = 0; v < V; ++v) warp_B[warp][v][lane] = (double)B[v];
+        for (int v = 0; v < V; ++v) { warp_B[warp][v][lane] = (double)B[v]; none = gfma(B[v], T(0), none); }
+        // what leaves the range from a zero state need not do so from the stretch's own: once more in 64 bits, from the slots
+        if (sizeof(T) == 4 && none != T(0)) {
+#pragma unroll 1
+            for (int v = 0; v < V; ++v) {
+                double wide = 0.0;
+#pragma unroll 1
+                for (int i = 0; i < steps; ++i) {
+                    const double step = (double)mine_u[i * kBlock].v[v];
+                    wide = i == 0 ? step : fma((double)mine_a[i * kBlock].v[GM == kGateShared ? 0 : v], wide, step);
+                }
+                warp_B[warp][v][lane] = wide;
+            }
+        }
         __syncthreads();                                         // (the slots have been read)
         if (round + 1 < rounds) fetch(s0 + per_round);
         const int buf = (int)(round & 1);
@@ -514,6 +530,11 @@ gated_rows_kernel(const GatedRuns g, int cluster_size) {
             const bool starts = s0 + me * I == 0 && !enters;     // the first step of all starts from nothing
             if (starts) A = 0.0;
             double B = (double)b;
+            if (sizeof(T) == 4 && !(fabs(B) <= 3.4028235e38)) {  // (as in the strips: not from its own state, perhaps)
+                B = (double)x[0];
+#pragma unroll
+                for (int i = 1; i < I; ++i) B = fma((double)c[i], B, (double)x[i]);
+            }
             // pairs of this and all threads before it, within the warp
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {

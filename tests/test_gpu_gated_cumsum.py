@@ -282,3 +282,27 @@ def test_a_capture_refuses_sums_before_anything_is_recorded(gate_shape, state_sh
             assert all(np.array_equal(a.to_numpy(), b.to_numpy()) for a, b in zip(kept, eager))
         finally:
             lib.cb200_set_stream(None)
+
+
+@pytest.mark.parametrize("shape,axis", [((1, 3000, 32), 1), ((1, 700, 5), 1), ((2, 5000), 1), ((3, 300), 1), ((2, 100, 2400), 1), ((4, 33, 6), 1), ((2, 16, 3), 1)])
+def test_sums_that_leave_the_range_from_zero_but_not_from_their_state(shape, axis):
+    """A state of -3e38 and a few steps of +2e38: the state stays inside the range of the type, while the same steps summed
+    from zero, as a stretch is before the state in front of it is known, do not."""
+    import cumo_b200 as xp
+
+    n = shape[axis]
+    x, gate = np.zeros(shape, np.float32), np.ones(shape, np.float32)
+    xs = np.moveaxis(x, axis, 0)
+    xs[0] = -3e38
+    for at in range(2, n - 3, 23):
+        xs[at], xs[at + 1] = 2e38, 2e38                      # -3e38 -> -1e38 -> 1e38 -> (back below) ...
+        xs[at + 2] = -4 / 3 * 3e38 * 0.75                    # -> -2e38, then
+        xs[at + 3] = -1e38                                   # -> -3e38
+    want, mag = ref.gated(x, gate, axis)
+    assert np.abs(want).max() < 3.2e38
+    X, G = xp.SFloat.from_numpy(x), xp.SFloat.from_numpy(gate)
+    got = X.gated_cumsum(G, axis=axis)
+    assert np.all(np.abs(got.to_numpy() - want) <= ref.gated_bound(mag, gate, axis, 2.0 ** -24))
+    back = xp.SFloat.from_numpy(np.ascontiguousarray(np.flip(x, axis)))       # the gradient runs the other way
+    dx = back.gated_cumsum_grad(G, xp.SFloat.zeros(*shape), axis=axis)[0].to_numpy()
+    assert np.all(np.abs(np.flip(dx, axis) - want) <= ref.gated_bound(mag, gate, axis, 2.0 ** -24))
