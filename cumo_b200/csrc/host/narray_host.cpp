@@ -561,6 +561,7 @@ void cb200_na_shape(const cb200_na_t* a, int64_t* shape) { memcpy(shape, a->shap
 void cb200_na_steps(const cb200_na_t* a, int64_t* step) { memcpy(step, a->step, sizeof(int64_t) * a->ndim); }
 void cb200_na_facts(const cb200_na_t* a, int64_t* out) {
     *out++ = a->ndim;
+    *out++ = is_contiguous(a);
     *out++ = (int64_t)(intptr_t)(a->dtype == CB200_BIT ? a->st->ptr : data_ptr(a));
     for (int d = 0; d < a->ndim; ++d) *out++ = a->shape[d];
     for (int d = 0; d < a->ndim; ++d) *out++ = a->step[d];

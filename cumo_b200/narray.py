@@ -289,11 +289,11 @@ class NArray:
         return _lib.load().cb200_na_ndim(self._h)
 
     def _facts(self):
-        """(address of the first element, shape, steps) from one call."""
-        buf = (c_int64 * (2 + 2 * _lib.MAX_DIM))()
+        """(address of the first element, shape, steps -- None if contiguous) from one call."""
+        buf = (c_int64 * (3 + 2 * _lib.MAX_DIM))()
         _lib.load().cb200_na_facts(self._h, buf)
         n = buf[0]
-        return buf[1], tuple(buf[2:2 + n]), tuple(buf[2 + n:2 + 2 * n])
+        return buf[2], tuple(buf[3:3 + n]), None if buf[1] else tuple(buf[3 + n:3 + 2 * n])
 
     @property
     def shape(self):

@@ -59,7 +59,7 @@ int64_t cb200_na_size(const cb200_na_t* a);
 void cb200_na_shape(const cb200_na_t* a, int64_t* shape);
 void cb200_na_steps(const cb200_na_t* a, int64_t* step);
 int64_t cb200_na_offset(const cb200_na_t* a);
-void cb200_na_facts(const cb200_na_t* a, int64_t* out); /* ndim, address of the first element (value types), shape[ndim], step[ndim] */
+void cb200_na_facts(const cb200_na_t* a, int64_t* out); /* ndim, contiguous (0 / 1), address of the first element (value types), shape[ndim], step[ndim] */
 void* cb200_na_base(const cb200_na_t* a);              /* start of the underlying buffer */
 int  cb200_na_is_contiguous(const cb200_na_t* a);
 void cb200_na_set_inplace(cb200_na_t* a, int on);      /* `x.inplace`: the next operation writes into x */
