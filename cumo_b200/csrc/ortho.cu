@@ -11,12 +11,32 @@ namespace cb200 {
 
 // ---- |G|_F in 64 bits: slices of a matrix to partial sums of squares, folded in slice order ---------------------------
 // (rows and columns may be exchanged for this: the caller passes the contiguous axis as columns)
+// Squares of 64-bit elements above 2^500 or below 2^-500 have sums of their own, of the elements scaled by 2^-600 and 2^600.
+template <typename T> constexpr int kSquareSums = sizeof(T) == 8 ? 3 : 1;
+constexpr double kFarUp = 0x1p500, kFarDown = 0x1p-500, kUp = 0x1p600, kDown = 0x1p-600;
+
+// What an element is multiplied by: (v * half) * inv * half = v / (norm + eps), half = 1 unless the norm is far from 1.
+struct Inverse { double inv, half; };
+template <typename T>
+__device__ __forceinline__ Inverse inverse_norm(const double* s, double eps) {
+    if (!(s[0] - s[0] == 0)) return {s[0] - s[0], 1.0};              // infinite or NaN: every element becomes NaN
+    if constexpr (sizeof(T) == 8) {
+        const double high = s[1], low = s[2];
+        if (!(high - high == 0)) return {high - high, 1.0};
+        if (high > 0) return {1.0 / (sqrt(high + s[0] * kDown * kDown) + eps * kDown), 0x1p-300};
+        if (s[0] == 0 && low > 0 && eps < 0x1p-300) return {1.0 / (sqrt(low) + eps * kUp), 0x1p300};
+        return {1.0 / (sqrt(s[0] + low * kDown * kDown) + eps), 1.0};
+    }
+    return {1.0 / (sqrt(s[0]) + eps), 1.0};
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kBlock)
 square_sums_kernel(const T* g, int64_t g_batch, int64_t rows, int64_t columns, int64_t row_step, int64_t column_step, int slices, double* sums) {
     g += (int64_t)blockIdx.y * g_batch;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    double s = 0;
+    constexpr int K = kSquareSums<T>;
+    double s = 0, far[2] = {0, 0};
     for (int64_t i = (int64_t)blockIdx.x * kWarpsPerBlock + warp; i < rows; i += (int64_t)slices * kWarpsPerBlock) {
         const T* r = g + i * row_step;
         for (int64_t j0 = lane; j0 < columns; j0 += 32 * 8) {
@@ -24,28 +44,44 @@ square_sums_kernel(const T* g, int64_t g_batch, int64_t rows, int64_t columns, i
 #pragma unroll
             for (int u = 0; u < 8; ++u) v[u] = j0 + u * 32 < columns ? r[(j0 + u * 32) * column_step] : T(0);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) s = fma((double)v[u], (double)v[u], s);
+            for (int u = 0; u < 8; ++u) {
+                if constexpr (K == 1) {
+                    s = fma((double)v[u], (double)v[u], s);
+                } else {
+                    const double a = fabs((double)v[u]);
+                    const bool up = !(a <= kFarUp), down = a < kFarDown;       // (a NaN counts as up)
+                    const double b = up ? a * kDown : down ? a * kUp : a, sq = b * b;
+                    s += up || down ? 0.0 : sq;
+                    far[0] += up ? sq : 0.0;
+                    far[1] += down ? sq : 0.0;
+                }
+            }
         }
     }
     __shared__ double part[kBlock];
-    part[threadIdx.x] = s;
-    __syncthreads();
-    for (int w = kBlock / 2; w > 0; w >>= 1) {
-        if ((int)threadIdx.x < w) part[threadIdx.x] += part[threadIdx.x + w];
+#pragma unroll
+    for (int c = 0; c < K; ++c) {
+        part[threadIdx.x] = c == 0 ? s : far[c - 1];
         __syncthreads();
+        for (int w = kBlock / 2; w > 0; w >>= 1) {
+            if ((int)threadIdx.x < w) part[threadIdx.x] += part[threadIdx.x + w];
+            __syncthreads();
+        }
+        if (threadIdx.x == 0) sums[((int64_t)blockIdx.y * slices + blockIdx.x) * K + c] = part[0];
     }
-    if (threadIdx.x == 0) sums[(int64_t)blockIdx.y * slices + blockIdx.x] = part[0];
 }
 
-// X0, row-major.  Sums beyond the type's range (or a NaN) make every element NaN, as the products would.
+// X0, row-major.  An infinity or a NaN makes every element NaN, as the products would.
 template <typename T>
 __global__ void __launch_bounds__(kBlock)
 scale_kernel(const Operand<T> G, int64_t m, int64_t n, int slices, const double* sums, double eps, T* x) {
-    __shared__ double inv;
+    __shared__ Inverse by;
+    constexpr int K = kSquareSums<T>;
     if (threadIdx.x == 0) {
-        double s = 0;
-        for (int k = 0; k < slices; ++k) s += sums[(int64_t)blockIdx.y * slices + k];
-        inv = s - s == 0 ? 1.0 / (sqrt(s) + eps) : s - s;
+        double s[K] = {};
+        for (int k = 0; k < slices; ++k)
+            for (int c = 0; c < K; ++c) s[c] += sums[((int64_t)blockIdx.y * slices + k) * K + c];
+        by = inverse_norm<T>(s, eps);
     }
     __syncthreads();
     const T* g = G.p + (int64_t)blockIdx.y * G.batch;
@@ -53,7 +89,7 @@ scale_kernel(const Operand<T> G, int64_t m, int64_t n, int slices, const double*
     T* out = x + (int64_t)blockIdx.y * total;
     for (int64_t f = (int64_t)blockIdx.x * kBlock + threadIdx.x; f < total; f += (int64_t)gridDim.x * kBlock) {
         const int64_t i = f / n;
-        out[f] = (T)((double)g[i * G.row + (f - i * n) * G.k] * inv);
+        out[f] = (T)((double)g[i * G.row + (f - i * n) * G.k] * by.half * by.inv * by.half);
     }
 }
 
@@ -93,7 +129,7 @@ scale_planes_kernel(const Operand<float> G, int64_t m, int64_t n, int64_t tiles_
         double s = 0;
         for (int k = threadIdx.x; k < slices; k += 32) s += sums[(int64_t)blockIdx.y * slices + k];
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (threadIdx.x == 0) inv = s - s == 0 ? 1.0 / (sqrt(s) + eps) : s - s;
+        if (threadIdx.x == 0) inv = inverse_norm<float>(&s, eps).inv;
     }
     const int64_t i0 = (int64_t)(blockIdx.x / tiles_n) * 32, j0 = (int64_t)(blockIdx.x % tiles_n) * 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -204,7 +240,7 @@ static int orthogonalize(int64_t batch, int64_t rows, int64_t columns, const T* 
     const int64_t enough = ((int64_t)sm_count() * 4 + batch - 1) / batch;
     if (slices > enough) slices = enough;
     if (slices > 256) slices = 256;
-    double* sums = reinterpret_cast<double*>(scratch.take((size_t)batch * slices * sizeof(double)));
+    double* sums = reinterpret_cast<double*>(scratch.take((size_t)batch * slices * kSquareSums<T> * sizeof(double)));
     if (!sums) return (int)cudaErrorMemoryAllocation;
     square_sums_kernel<T><<<dim3((unsigned)slices, (unsigned)batch), kBlock, 0, st>>>(G.p, G.batch, sr, sc_, along_k ? G.row : G.k, along_k ? G.k : G.row,
                                                                                   (int)slices, sums);

@@ -87,3 +87,41 @@ def test_sizes_of_values():
     got = linalg.orthogonalize(xp.SFloat.from_numpy(h), eps=1e-40).to_numpy()
     assert np.array_equal(got[:3], plain[:3])                     # powers of two leave every digit alone
     assert not got[3].any() and np.isnan(got[4]).all()
+
+
+@pytest.mark.parametrize("shape", [(40, 60), (60, 40), (2, 3, 17, 30)])
+def test_sizes_of_values_in_double_precision(shape):
+    """Norms whose squares are beyond 64 bits, above and below, and matrices that hold both."""
+    import cumo_b200 as xp
+    from cumo_b200 import linalg
+
+    D = xp.DFloat.from_numpy
+    g = np.random.default_rng(12).standard_normal(shape)
+    plain = linalg.orthogonalize(D(g), eps=0.0).to_numpy()
+    for power in (600, 1015, -600, -1000):                       # powers of two leave every digit alone
+        assert np.array_equal(linalg.orthogonalize(D(np.ldexp(g, power)), eps=0.0).to_numpy(), plain)
+    tol = 64 * 2.0 ** -53 * 3.4445 ** 5 * np.abs(plain).max()     # the norm's sum in another order: a few roundings, carried through five steps
+    for power in (500, 501, -500, -499):
+        assert np.abs(linalg.orthogonalize(D(np.ldexp(g, power)), eps=0.0).to_numpy() - plain).max() <= tol
+    # eps counts at any size: g / (|g| + |g|) is half of g / |g|
+    norm = np.sqrt((g * g).sum((-2, -1))).max()
+    for power in (0, 700, -700):
+        got = linalg.orthogonalize(D(np.ldexp(g, power)), steps=0, eps=float(np.ldexp(norm, power))).to_numpy()
+        n = np.sqrt((g * g).sum((-2, -1), keepdims=True))
+        assert np.abs(got - g / (n + norm)).max() <= 16 * 2.0 ** -53
+    # far below eps: g / eps
+    got = linalg.orthogonalize(D(np.ldexp(g, -700)), steps=0, eps=2.0 ** -100).to_numpy()
+    assert np.abs(got - np.ldexp(g, -600)).max() <= 16 * 2.0 ** -53 * 2.0 ** -600 * np.abs(g).max()
+    # one entry above everything else by more than the type's own range of squares; zero stays zero
+    h = g.copy()
+    h[..., 3, 5] = 2.0 ** 800
+    got = linalg.orthogonalize(D(h), steps=0, eps=0.0).to_numpy()
+    assert np.all(got[..., 3, 5] == 1)
+    got[..., 3, 5] = 0
+    want = np.ldexp(g, -800)
+    want[..., 3, 5] = 0
+    assert np.abs(got - want).max() <= 16 * 2.0 ** -53 * 2.0 ** -800 * np.abs(g).max()
+    h[...] = 0
+    assert not linalg.orthogonalize(D(h), eps=1e-300).to_numpy().any()
+    h[..., 0, 0] = np.inf
+    assert np.isnan(linalg.orthogonalize(D(h), eps=1e-300).to_numpy()).all()
