@@ -92,6 +92,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "cb200_na_linear_grad": (c_int, [H, H, H, c_int, H, POINTER(H), POINTER(H), POINTER(H)]),
         "cb200_na_orthogonalize": (H, [H, c_int, POINTER(c_double), c_double]),
         "cb200_product_status": (c_int, []),
+        "cb200_product_status_set": (c_int, []),
         "cb200_split_product_launches": (ctypes.c_ulonglong, [c_int, c_int]),
         "cb200_na_gated_cumsum": (H, [H, H, H, c_int]),
         "cb200_na_gated_cumsum_grad": (c_int, [H, H, H, H, c_int, POINTER(H), POINTER(H), POINTER(H)]),

@@ -629,8 +629,6 @@ static int launch_strip(GatedRuns& g) {
     const int cluster = cluster_for(strips, g.n, L * kStripWarps);
     if (strips * cluster > 0x7fffffff) return (int)cudaErrorInvalidValue;
     if (cluster > 1) {
-        const int late = product_gave_up();
-        if (late) return late;
         if (!gave_up_word(&g.gave_up)) return (int)cudaErrorMemoryAllocation;
     }
     constexpr size_t smem = strip_bytes<T, V, L, GM, GRAD>() + 2 * 8 * V * 32 * sizeof(double2);
@@ -706,6 +704,8 @@ static int launch_rows(const GatedRuns& g) {
 template <typename T, bool GRAD>
 static int gated_launch(GatedRuns& g) {
     if (g.n == 0 || g.runs == 0) return 0;
+    const int late = product_gave_up();
+    if (late) return late;
     // merge neighbouring outer dimensions that every operand walks evenly; drop extents of 1
     int nd = 0;
     for (int d = 0; d < g.nd; ++d) {

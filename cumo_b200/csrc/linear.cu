@@ -257,6 +257,8 @@ static int linear(int64_t m, int64_t n, int64_t k, const T* x, ssize_t x_row, ss
     CB200_TRACE_LAUNCH();
     if (m < 0 || n < 0 || k < 1 || activation < 0 || activation >= kActCount) return (int)cudaErrorInvalidValue;
     if (m == 0 || n == 0) return 0;
+    const int late = product_gave_up();
+    if (late) return late;
     constexpr ssize_t es = sizeof(T);
     if (x_row % es || x_col % es || w_row % es || w_col % es || bias_step % es || r_row % es || r_col % es) return (int)cudaErrorInvalidValue;
     Epilogue<T> e = {};
@@ -267,8 +269,6 @@ static int linear(int64_t m, int64_t n, int64_t k, const T* x, ssize_t x_row, ss
     e.y = y; e.ld = n; e.pre = pre;
     if constexpr (sizeof(T) == 4) {
         if (!few_rows(m, n, k) && worth_splitting(m, n, k)) {
-            const int late = product_gave_up();
-            if (late) return late;
             Scratch scratch(current_stream());
             SplitSet set;
             const int ix = set.add(SplitSource{x, x_row / es, x_col / es, nullptr, 0, 0, kActNone}, m, k);
@@ -297,13 +297,14 @@ static int linear_grad(int64_t m, int64_t n, int64_t k, const T* grad, ssize_t g
         if (dbias && r == cudaSuccess) r = cudaMemsetAsync(dbias, 0, (size_t)n * es, st);
         return (int)r;
     }
+    const int late = product_gave_up();
+    if (late) return late;
     Scratch scratch(st);
     Steps2<T> g = {grad, g_row / es, g_col / es}, p = {pre, p_row / es, p_col / es};
     Operand<T> dz = {grad, g.row, g.col, 0};
     if constexpr (sizeof(T) == 4) {
         if ((dx || dw) && worth_splitting(m, n, k)) {
-            int rc = product_gave_up();
-            if (rc) return rc;
+            int rc = 0;
             if (dbias) rc = launch_dz<T>(m, n, g, p, activation, nullptr, dbias, scratch, st);
             if (rc) return rc;
             SplitSet set;

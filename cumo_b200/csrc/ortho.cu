@@ -177,8 +177,6 @@ join_planes_kernel(int64_t m, int64_t n, int64_t tiles_n, const uint16_t* planes
 
 static int orthogonalize_split(int64_t batch, int64_t m, int64_t n, bool tall, const Operand<float>& G, int steps, const double* coefs, double eps, int slices,
                                const double* sums, float* out, Scratch& scratch, cudaStream_t st) {
-    int rc = product_gave_up();
-    if (rc) return rc;
     const int64_t ldx = planes_ld(n), ldp = planes_ld(m), px = batch * m * ldx, pp = batch * m * ldp;
     uint16_t* x = reinterpret_cast<uint16_t*>(scratch.take((size_t)px * 6));
     uint16_t* x2 = reinterpret_cast<uint16_t*>(scratch.take((size_t)px * 6));
@@ -190,7 +188,7 @@ static int orthogonalize_split(int64_t batch, int64_t m, int64_t n, bool tall, c
     const dim3 grid((unsigned)(tm * tn), (unsigned)batch);
     scale_planes_kernel<<<grid, kBlock, 0, st>>>(G, m, n, tn, slices, sums, eps, x, ldx, px);
     count_launch();
-    rc = (int)cudaGetLastError();
+    int rc = (int)cudaGetLastError();
     for (int s = 0; s < steps && rc == 0; ++s) {
         const float a = (float)coefs[3 * s], b = (float)coefs[3 * s + 1], c = (float)coefs[3 * s + 2];
         const Planes X = {x, m, n, batch, ldx, true}, Xn = {x, n, m, batch, ldx, false}, P = {p, m, m, batch, ldp, true}, Q = {q, m, m, batch, ldp, true};
@@ -220,6 +218,8 @@ static int orthogonalize(int64_t batch, int64_t rows, int64_t columns, const T* 
     if (batch < 0 || rows < 0 || columns < 0 || steps < 0 || (steps && !coefs) || g_batch % es || g_row % es || g_col % es)
         return (int)cudaErrorInvalidValue;
     if (batch == 0 || rows == 0 || columns == 0) return 0;
+    const int late = product_gave_up();
+    if (late) return late;
     constexpr int64_t kMostBatch = 32768;                       // (grids count the matrices in 16 bits)
     if (batch > kMostBatch) {
         for (int64_t b = 0; b < batch; b += kMostBatch) {

@@ -568,22 +568,24 @@ split_product_kernel(const SplitArgs g, const __grid_constant__ CUtensorMap map_
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
 // One word of mapped host memory per process that a kernel sets when a bounded wait ran out; read without synchronising.
+static std::atomic<int*> word_on_host{nullptr};
 int* gave_up_word(int** dev) {
     static std::mutex mu;
-    static int* host = nullptr;
+    int* host = word_on_host.load(std::memory_order_acquire);
     static int* on_device[64] = {};
     int d = 0;
     if (dev && cudaGetDevice(&d) != cudaSuccess) return nullptr;
     if (d < 0 || d >= 64) return nullptr;
-    std::lock_guard<std::mutex> lock(mu);
     if (host && !dev) return host;
+    std::lock_guard<std::mutex> lock(mu);
+    host = word_on_host.load(std::memory_order_acquire);
     if (!host || !on_device[d]) {
         cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;       // the first call may come during a capture
         cudaThreadExchangeStreamCaptureMode(&mode);
         void* p = host;
         cudaError_t rc = cudaSuccess;
         if (!host) rc = cudaHostAlloc(&p, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
-        if (rc == cudaSuccess && !host) { host = static_cast<int*>(p); *host = 0; }
+        if (rc == cudaSuccess && !host) { host = static_cast<int*>(p); *host = 0; word_on_host.store(host, std::memory_order_release); }
         void* q = nullptr;
         if (rc == cudaSuccess && dev) rc = cudaHostGetDevicePointer(&q, host, 0);
         cudaThreadExchangeStreamCaptureMode(&mode);
@@ -595,7 +597,7 @@ int* gave_up_word(int** dev) {
 }
 
 int product_gave_up() {
-    const int* w = gave_up_word(nullptr);
+    const int* w = word_on_host.load(std::memory_order_acquire);     // (none yet: nothing that waits has been launched)
     return w && *const_cast<const volatile int*>(w) ? (int)cudaErrorLaunchTimeout : 0;
 }
 
@@ -747,7 +749,15 @@ int launch_split_product(const Planes& a, const Planes& b, const PlaneEpilogue& 
 
 }  // namespace cb200
 
-// 0: no bounded wait of the tensor-core product has run out in this process since the last call; 1: one did, and results since
+// As if a bounded wait had run out: for a program that tests what it does then.
+extern "C" int cb200_product_status_set(void) {
+    int* w = cb200::gave_up_word(nullptr);
+    if (!w) return -1;
+    *const_cast<volatile int*>(w) = 1;
+    return 0;
+}
+
+// 0: no bounded wait of the tensor-core product or the recurrence has run out in this process since the last call; 1: one did, and results since
 // then are not valid; -1: the word could not be read.  Synchronises the device; clears the word.
 extern "C" int cb200_product_status(void) {
     int* w = cb200::gave_up_word(nullptr);

@@ -634,10 +634,14 @@ CB200_DECL_GATED(sfloat) CB200_DECL_GATED(dfloat)
         int steps, const double* coefs, double eps, C* out);
 CB200_DECL_LINEAR(sfloat, float) CB200_DECL_LINEAR(dfloat, double)
 
-/* The tensor-core product behind them waits for its copies and instructions with bounds.  0: no wait has run out in this
- * process since the last call; 1: one did, and results since then are not valid (the entry points above return
- * cudaErrorLaunchTimeout until this is called); -1: unknown.  Synchronises the device. */
+/* The tensor-core product behind them waits for its copies and instructions with bounds, the recurrence cut over a cluster for
+ * its neighbours' pairs.  0: no wait has run out in this process since the last call; 1: one did, and results since then are not
+ * valid; -1: unknown.  Synchronises the device.  A call whose own wait runs out has returned by then: the gated, linear and
+ * orthogonalize entry points of any size return cudaErrorLaunchTimeout from the moment the device has raised the word until this
+ * is called, and a program that hands results on without another such call asks here first.  The second function raises the word
+ * (0; -1 where it cannot be had), for a program that tests what it does then. */
 int cb200_product_status(void);
+int cb200_product_status_set(void);
 /* Launches of that product in this process with tiles of 256 (a pair of CTAs), 128 or 64 columns: those that compute one side of a
  * symmetric result, or the others. */
 unsigned long long cb200_split_product_launches(int columns, int symmetric);

@@ -246,3 +246,28 @@ def test_beyond_32_bits():
         state = gate[0, t // 2 + i].double() * state + x[0, t // 2 + i].double()
         want.append(state)
     assert float((torch.stack(want) - h[0, t // 2:t // 2 + 5].double()).abs().max()) <= 16 * 2.0 ** -24 * scale
+
+
+def test_a_wait_that_ran_out_is_reported_by_every_operator():
+    """Once the word is up, whatever its size and plan, each operator refuses until the status has been asked for."""
+    import cumo_b200 as xp
+    from cumo_b200 import _lib, linalg
+
+    lib = _lib.load()
+    f32 = lambda *s: xp.SFloat.ones(*s)
+    f64 = lambda *s: xp.DFloat.ones(*s)
+    calls = [lambda: f32(2, 3).gated_cumsum(0.5, axis=1), lambda: f32(1, 5000, 32).gated_cumsum(f32(1, 5000, 32), axis=1),
+             lambda: f64(4, 900).gated_cumsum_grad(f64(4, 900), f64(4, 900), axis=1), lambda: linalg.linear(f32(1, 64), f32(64, 8)),
+             lambda: linalg.linear(f32(300, 300), f32(300, 300)), lambda: linalg.linear(f64(9, 10), f64(10, 11)),
+             lambda: linalg.linear_grad(f32(3, 5), f32(3, 4), f32(4, 5)), lambda: linalg.linear_grad(f32(3, 5), f32(3, 4), f32(4, 5), want="bias"),
+             lambda: linalg.orthogonalize(f32(5, 7)), lambda: linalg.orthogonalize(f32(200, 300)), lambda: linalg.orthogonalize(f64(5, 7))]
+    assert lib.cb200_product_status() == 0
+    for call in calls:
+        call()
+        assert lib.cb200_product_status_set() == 0
+        for _ in range(2):
+            with pytest.raises(xp.CudaError, match="bounded wait"):
+                call()
+        assert lib.cb200_product_status() == 1 and lib.cb200_product_status() == 0
+        call()
+    assert (f32(2, 2) + f32(2, 2)).to_numpy().sum() == 8          # nothing is latched for what comes next
