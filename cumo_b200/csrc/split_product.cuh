@@ -53,7 +53,6 @@ struct Planes {
     bool k_major;
     int64_t outer() const { return k_major ? rows : k; }
     int64_t inner() const { return k_major ? k : rows; }
-    int64_t plane_elements() const { return batch * outer() * ld; }
 };
 inline int64_t planes_ld(int64_t inner) { return (inner + 7) / 8 * 8; }
 
