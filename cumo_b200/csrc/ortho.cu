@@ -246,9 +246,11 @@ static int orthogonalize(int64_t batch, int64_t rows, int64_t columns, const T* 
                                                                                   (int)slices, sums);
     count_launch();
     if constexpr (sizeof(T) == 4) {
-        // Matrices of few rows have short sums behind their results, and ordinary fp32 FMAs round those better than the tensor
-        // cores truncate them (80 x 1408: error 1.1e-6 against 1.8e-6); P's long sums are cut over clusters.
-        const bool few = m <= 128 && batch * m * m * n <= (1LL << 26);
+        // Few rows with long sums: a product on planes has one or a few tiles then, each with the whole of K before it, while the
+        // row products cut P's sums over clusters and cost little arithmetic.  Five steps in us, on planes and on the CUDA cores:
+        // 64 x 256 149 and 187, 128 x 1024 244 and 255, 128 x 2048 352 and 260, 128 x 16384 1914 and 582, 33 x 30000 3370 and 582;
+        // with more of them the arithmetic counts, 64 of 32 x 2000 632 and 561, 8 of 128 x 2048 409 and 578.  (Errors are alike.)
+        const bool few = m < 16 || (m <= 128 && n >= 9 * m && batch * m * m <= 65536);
         if (!few) return orthogonalize_split(batch, m, n, tall, G, steps, coefs, eps, (int)slices, sums, out, scratch, st);
     }
     T* x = reinterpret_cast<T*>(scratch.take((size_t)batch * m * n * es));

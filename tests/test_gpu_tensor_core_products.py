@@ -334,3 +334,24 @@ def test_more_steps_and_larger_coefficients_than_usual():
     got = linalg.orthogonalize(xp.SFloat.from_numpy(g), steps=2, coefs=[(1.0, 0.0, 0.0), (3e38, 0.0, 0.0)]).to_numpy()
     x = g.astype(np.float64) / (np.linalg.norm(g.astype(np.float64)) + 1e-7)
     assert np.all(np.abs(got - 3e38 * x) <= 1e-5 * np.abs(3e38 * x))
+
+
+@pytest.mark.parametrize("shape,on_planes", [((15, 300), False), ((16, 144), False), ((16, 143), True), ((143, 16), True), ((128, 1151), True), ((128, 1152), False), ((1152, 128), False),
+                                             ((4, 128, 1152), False), ((5, 128, 1152), True), ((129, 2000), True), ((64, 64), True), ((40, 17, 33), True)])
+def test_orthogonalize_few_rows(shape, on_planes):
+    """Both sides of the rule that sends matrices of few rows and long sums to the row products."""
+    import torch
+
+    import cumo_b200 as xp
+    from cumo_b200 import linalg
+
+    torch.backends.cuda.matmul.allow_tf32 = False
+    g = np.random.default_rng(sum(shape)).standard_normal(shape).astype(np.float32)
+    want, plain = in_64_bits(g, 5, MUON)
+    with Ran() as ran:
+        got = linalg.orthogonalize(xp.SFloat.from_numpy(g)).to_numpy()
+    assert bool(ran.tiles) == on_planes
+    # one matrix' error varies with its values: four times 32-bit arithmetic's over the whole batch, and never above the
+    # few roundings (64) that five steps' slopes of up to 3.4445 carry on from the first
+    off, most = np.sqrt(((got - want) ** 2).sum()), np.sqrt(((plain - want) ** 2).sum())
+    assert off <= 4 * most + 64 * U * np.sqrt((want ** 2).sum())
