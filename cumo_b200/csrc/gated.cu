@@ -531,9 +531,9 @@ gated_rows_kernel(const GatedRuns g, int cluster_size) {
             if (starts) A = 0.0;
             double B = (double)b;
             if (sizeof(T) == 4 && !(fabs(B) <= 3.4028235e38)) {  // (as in the strips: not from its own state, perhaps)
-                B = (double)x[0];
-#pragma unroll
-                for (int i = 1; i < I; ++i) B = fma((double)c[i], B, (double)x[i]);
+                B = (double)su[mine];
+#pragma unroll 1
+                for (int i = 1; i < I; ++i) B = fma((double)sa[mine + i], B, (double)su[mine + i]);
             }
             // pairs of this and all threads before it, within the warp
 #pragma unroll
