@@ -263,6 +263,8 @@ struct PlaneOut {
         for (int q = 0; q < 4; ++q) {
             const bool live = here && i0 + q * 8 + r0 < m;
             float* t = tile + (q * 8 + r0) * kSpStageCols + c0;
+            Ahead cur = d;
+            if (q < 3) ahead(d, lane, batch, i0 + (q + 1) * 8, j0, m, n);
             float v[8];
             if (live) {
 #pragma unroll
@@ -270,18 +272,17 @@ struct PlaneOut {
                 if (e.d) {
                     const uint32_t* part[kParts];
 #pragma unroll
-                    for (int w = 0; w < kParts; ++w) part[w] = reinterpret_cast<const uint32_t*>(&d.part[w]);
+                    for (int w = 0; w < kParts; ++w) part[w] = reinterpret_cast<const uint32_t*>(&cur.part[w]);
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {                // smallest part first: the sum is the number itself
-                        float lo = 0.f, hi = 0.f;
+                        float lo = bf16_at(part[kParts - 1][x]), hi = __uint_as_float(part[kParts - 1][x] & 0xffff0000u);
 #pragma unroll
-                        for (int w = kParts - 1; w >= 0; --w) { lo += bf16_at(part[w][x] & 0xffffu); hi += __uint_as_float(part[w][x] & 0xffff0000u); }
+                        for (int w = kParts - 2; w >= 0; --w) { lo += bf16_at(part[w][x]); hi += __uint_as_float(part[w][x] & 0xffff0000u); }
                         v[2 * x] = fmaf(e.beta, lo, v[2 * x]);
                         v[2 * x + 1] = fmaf(e.beta, hi, v[2 * x + 1]);
                     }
                 }
             }
-            if (q < 3) ahead(d, lane, batch, i0 + (q + 1) * 8, j0, m, n);
             if (!live) continue;
             store(v, at0 + q * 8 * e.ld);
             if (mirror)
@@ -302,12 +303,17 @@ struct PlaneOut {
     }
     __device__ __forceinline__ void store(const float (&v)[8], int64_t at) const {
         uint32_t out[kParts][4];
+        float none = 0.f;                                        // NaN once a number has no parts
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            uint32_t a0, b0, c0, a1, b1, c1;
-            split3_all(v[2 * x], a0, b0, c0);
-            split3_all(v[2 * x + 1], a1, b1, c1);
-            out[0][x] = a0 | a1 << 16; out[1][x] = b0 | b1 << 16; out[2][x] = c0 | c1 << 16;
+        for (int x = 0; x < 4; ++x) split3_pair(v[2 * x], v[2 * x + 1], out[0][x], out[1][x], out[2][x], none);
+        if (none != 0.f) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                uint32_t a0, b0, c0, a1, b1, c1;
+                split3_all(v[2 * x], a0, b0, c0);
+                split3_all(v[2 * x + 1], a1, b1, c1);
+                out[0][x] = a0 | a1 << 16; out[1][x] = b0 | b1 << 16; out[2][x] = c0 | c1 << 16;
+            }
         }
 #pragma unroll
         for (int w = 0; w < kParts; ++w) *reinterpret_cast<uint4*>(e.out + at + w * e.plane) = make_uint4(out[w][0], out[w][1], out[w][2], out[w][3]);

@@ -32,7 +32,18 @@ __device__ __forceinline__ bool split3(float v, uint32_t& a, uint32_t& b, uint32
     a = __bfloat16_as_ushort(x); b = __bfloat16_as_ushort(y); c = __bfloat16_as_ushort(z);
     return fine;
 }
-// The same for what must not be left out: infinities and NaN are their own first part, and what only rounds to infinity is cut off.
+// Two numbers' parts side by side in 32 bits each; `none` becomes NaN if one of them has no parts.
+__device__ __forceinline__ void split3_pair(float u, float v, uint32_t& a, uint32_t& b, uint32_t& c, float& none) {
+    auto pack = [](float lo, float hi) { const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi); return *reinterpret_cast<const uint32_t*>(&p); };
+    a = pack(u, v);
+    float r = u - __uint_as_float(a << 16), s = v - __uint_as_float(a & 0xffff0000u);
+    none = fmaf(r, 0.f, fmaf(s, 0.f, none));
+    b = pack(r, s);
+    r -= __uint_as_float(b << 16);
+    s -= __uint_as_float(b & 0xffff0000u);
+    c = pack(r, s);
+}
+// One number for which there is no leaving out: infinities and NaN are their own first part, and what only rounds to infinity is cut off.
 __device__ __forceinline__ void split3_all(float v, uint32_t& a, uint32_t& b, uint32_t& c) {
     if (split3(v, a, b, c)) return;
     const uint32_t bits = __float_as_uint(v), mag = bits & 0x7fffffffu;
