@@ -173,7 +173,8 @@ __device__ __forceinline__ double gates_times(double x, double y) {
 // count themselves in at the receiver's mbarrier: a cluster barrier would also wait for the outputs' way to memory), and leaves
 // each warp the state in front of its stretch.  The wait for the pairs is bounded.  Each thread's next steps are on their way
 // (asynchronous copies into slots of shared memory that only it reads) while all this happens, and two CTAs per SM cover each
-// other's exchanges.  1 x 50000 x 2048 SFloat: 285 us, 4.3 TB/s; 64 x 512 x 2048 (no cluster) 5.3 TB/s.
+// other's exchanges.  1 x 50000 x 2048 SFloat: 287 us, 4.3 TB/s; 64 x 512 x 2048 (no cluster) 5.1 TB/s.  Time is cut over one cluster
+// and no further: with few channels most SMs idle (1 x 50000 x 512 1.6 TB/s, 1 x 400000 x 64 0.23).
 constexpr int kStripWarps = 8;
 
 template <int BYTES>

@@ -11,10 +11,11 @@
 //               where tensor memory has room, else the next block's small products run meanwhile); at the end of a tile the
 //               small ones follow and the sums pass through a small shared-memory tile per warp, so that global memory is read
 //               and written along rows
-// What bounds it (cycles counted in the issuing thread): three parts at 8192^3 3257 cycles per K-block of 3072 tensor cycles,
-// 4.4 ms, the power limit (1480 TFLOP/s of bf16 products); two parts at 4096^3 2211 of 1536, 2868 of the surplus per chunk going
-// into waiting for the accumulator: reading one takes some 57 bytes per cycle, which is why a chunk is as long as truncation
-// allows; narrow tiles the operands' way through L2 and shared memory.
+// What bounds it: at 8192^3 3257 cycles per K-block of 3072 tensor cycles (counted in the issuing thread), 4.4 ms, the power limit
+// (1480 TFLOP/s of bf16 products).  At 4096^3 503 us, the tensor pipe 88 % busy, 632 MB read from memory and 4.2 GB through L2;
+// into planes 571 us and 74 %: writing a tile takes longer than the first chunk of the next one hides.  Reading an accumulator
+// takes some 57 bytes per cycle, which is why a chunk is as long as truncation allows.  A 128 x 64 tile's K-block takes about 2500
+// cycles of 1152 tensor cycles (8 x 256 x 1024 against x 256); what it waits for has not been established.
 // With CG = 2 two CTAs of a cluster share a 256 x 256 tile: each loads its 128 rows of A and its half of B, the first CTA
 // issues the instructions for both.  Shared memory feeds 64 bytes per cycle to the tensor cores then, instead of the 128 of
 // a 128 x 128 tile (its limit), and each operand byte loaded is used twice as often.  Small problems take 128-row tiles of one
@@ -681,8 +682,8 @@ static int launch_shape(const Planes& a, const Planes& b, const Out& out, bool s
 
 // The tile and the number of pieces K is cut into are those with the least estimated cycles: rounds over the SMs x K-blocks of
 // a piece x instructions x cycles per instruction -- measured at 4096^3, a 256 x 256 pair takes the tensor cores' 128, a
-// 128 x 128 tile 95 and a 128 x 64 tile 70 (bound by what L2 delivers), the latter two on twice as many slots -- plus, with
-// pieces, writing and adding up their results (about 2500 bytes per cycle) and one more launch.
+// 128 x 128 tile 95 and a 128 x 64 tile 70, the latter two on twice as many slots -- plus, with pieces, writing and adding up
+// their results (about 2500 bytes per cycle) and one more launch.
 struct Shape { int tile, splits; };
 
 static Shape choose_shape(const Planes& a, const Planes& b, bool symmetric, int most_splits) {

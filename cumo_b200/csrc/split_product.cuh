@@ -7,7 +7,7 @@
 // under a common power of two: rows of a matrix that are small beside the others would lose theirs.)  Products of two 16-bit
 // numbers are exact in the tensor core; what it adds them into is 32 bits wide but truncates, an error that leans one way and
 // grows with the number of additions (2e-8 of the accumulator each, measured).  So the large products a1 b1 have an
-// accumulator of their own, which takes 64 to 512 of K -- four to 32 additions -- before it is added into registers with
+// accumulator of their own, which takes 64 to 256 of K -- four to 16 additions -- before it is added into registers with
 // ordinary rounded additions; what truncation does to the accumulator of the small products is 2^-8 of that and less.
 #pragma once
 
@@ -20,8 +20,8 @@ namespace cb200 {
 constexpr int kParts = 3;
 
 // a = a1 + a2 + a3 with each part the bfloat16 nearest to what the parts before it leave: 8 bits each, so that three hold
-// all 24 (parts under 2^-126 are lost, which only operands under 2^-102 have).  What rounds to infinity in the first part has
-// no such parts: false, and zeros.
+// all 24.  (Parts under 2^-126 lose bits: products of operands that are all under 2^-112 do, 6e-7 off at 2^-114, 9e-6 at 2^-118.)
+// What rounds to infinity in the first part has no such parts: false, and zeros.
 __device__ __forceinline__ bool split3(float v, uint32_t& a, uint32_t& b, uint32_t& c) {
     const bool fine = (__float_as_uint(v) & 0x7fffffffu) < 0x7f7f8000u;
     if (!fine) v = 0.f;
@@ -114,8 +114,8 @@ struct SplitJob {
 struct SplitJobs { SplitJob job[3]; int count; };
 int launch_split(const SplitJobs& jobs, cudaStream_t st);
 
-// Outputs i, j with a[i] or b[j] marked, or hot_row[i] and hot_col[j], in float from the operands: element (row, k) of A at (row, k) of `a`, or (k, row)
-// if a_turned; B alike.  Returns at once on the device when nothing was marked.  Up to two products in one launch.
+// Outputs i, j with a[i] or b[j] marked, or hot_row[i] and hot_col[j], in float from the operands: element (row, k) of A at
+// (row, k) of `a`, or (k, row) if a_turned; B alike.  Returns at once on the device when nothing was marked.  Up to two products in one launch.
 struct FixJob {
     int64_t m, n, k;
     SplitSource a, b;
